@@ -261,13 +261,10 @@ def _own_fmt(sy, fmt):
     return sy.SY_FP8_E4M3 if fmt == "e4m3" else sy.SY_FP8_E5M2
 
 
-def _own_matmul(sy, s, a, a_scale, a_fmt, b, b_scale, b_fmt, b_block, m, n, k, out, add, stream):
-    need = sy.matmul_fp8_workspace(m, n, k)
-    if "work" not in s or s["work"].numel() < need:
-        s["work"] = torch.empty(need, dtype=torch.uint8, device="cuda")
+def _own_matmul(sy, a, a_scale, a_fmt, b, b_scale, b_fmt, b_block, m, n, k, out, add, stream):
     sy.matmul_fp8_device(a.data_ptr(), a_scale.data_ptr(), _own_fmt(sy, a_fmt), 1, b.data_ptr(), b_scale.data_ptr(),
                          _own_fmt(sy, b_fmt), b_block, m, n, k, out.data_ptr(), _own_type(sy, out.dtype), n, add,
-                         s["work"].data_ptr(), s["work"].numel(), stream=stream)
+                         stream=stream)
     return out
 
 
@@ -290,21 +287,21 @@ def _own(s):
     if kind == "serve":
         m, n, k = case["m"], case["n"], case["k"]
         q, sc, _, _ = _own_cast(sy, s["x"], "e4m3", 1, False, stream)
-        return _own_matmul(sy, s, q, sc, "e4m3", s["w"], s["w_scale"], "e4m3", 128, m, n, k,
+        return _own_matmul(sy, q, sc, "e4m3", s["w"], s["w_scale"], "e4m3", 128, m, n, k,
                            _empty(m, n, s["x"].dtype), False, stream)
     if kind == "matmul":
         m, n, k = case["m"], case["n"], case["k"]
         out = s["c"] if case["add"] else _empty(m, n, _TORCH[case["out"]])
-        return _own_matmul(sy, s, s["a"], s["a_scale"], case["a"], s["b"], s["b_scale"], case["b"], case["wblock"], m, n,
+        return _own_matmul(sy, s["a"], s["a_scale"], case["a"], s["b"], s["b_scale"], case["b"], case["wblock"], m, n,
                            k, out, case["add"], stream)
     if kind == "linear":
         t, n, k = case["t"], case["n"], case["k"]
         x, xs, xt, xts = _own_cast(sy, s["x"], "e4m3", 1, True, stream)
         w, ws, wt, wts = _own_cast(sy, s["w"], "e4m3", 128, True, stream)
         d, ds, dt, dts = _own_cast(sy, s["dy"], "e5m2", 1, True, stream)
-        y = _own_matmul(sy, s, x, xs, "e4m3", w, ws, "e4m3", 128, t, n, k, _empty(t, n, s["x"].dtype), False, stream)
-        dx = _own_matmul(sy, s, d, ds, "e5m2", wt, wts, "e4m3", 128, t, k, n, _empty(t, k, s["x"].dtype), False, stream)
-        dw = _own_matmul(sy, s, dt, dts, "e5m2", xt, xts, "e4m3", 1, n, k, t, _empty(n, k, torch.float32), False, stream)
+        y = _own_matmul(sy, x, xs, "e4m3", w, ws, "e4m3", 128, t, n, k, _empty(t, n, s["x"].dtype), False, stream)
+        dx = _own_matmul(sy, d, ds, "e5m2", wt, wts, "e4m3", 128, t, k, n, _empty(t, k, s["x"].dtype), False, stream)
+        dw = _own_matmul(sy, dt, dts, "e5m2", xt, xts, "e4m3", 1, n, k, t, _empty(n, k, torch.float32), False, stream)
         return {"y": y, "dx": dx, "dw": dw}
     if kind == "ortho":
         rows, cols = case["rows"], case["cols"]
