@@ -9,7 +9,8 @@
  * optional NCCL gradient all-reduce and the SGD-momentum / AdamW update.
  *
  * Conventions: plain C types; host pointers unless a name says "device"; the caller owns every
- * buffer it passes and may reuse it as soon as a call returns (calls are synchronous).  Tensors
+ * buffer it passes and may reuse it as soon as a call returns (calls are synchronous, except the operators on
+ * device memory at the end, which are queued on the caller's stream).  Tensors
  * use the reference layouts: NCHW activations, OIHW weights, float32.  A session is not
  * reentrant (the C# host serialises calls, YoloTrainer.cs:163-168).
  *
@@ -59,6 +60,7 @@ typedef struct sy_block {
 
 #define SY_OPT_SGD 0
 #define SY_OPT_ADAMW 1
+#define SY_OPT_MUON 2         /* Muon on the dense conv weights, AdamW on every other parameter */
 /* Tensor-core precision of every convolution in the step.  3xTF32 splits each FP32 operand into a
  * TF32 value and a TF32 residual and sums three products (small x big, big x small, big x big),
  * which restores FP32-level agreement with the reference's FP32 arithmetic at 3x the MMA work. */
@@ -171,7 +173,7 @@ SY_API sy_status sy_cuda_tensor_info(const sy_session *session, int32_t index, s
 SY_API sy_status sy_cuda_set_tensor(sy_session *session, int32_t index, const float *host, int64_t count);
 SY_API sy_status sy_cuda_get_tensor(const sy_session *session, int32_t index, float *host, int64_t count);
 /* Optimizer state of a parameter tensor (TrainingParameter.Velocity, YoloTrainer.cs:135-141);
- * moment 0 = SGD velocity / AdamW first moment, 1 = AdamW second moment. */
+ * moment 0 = SGD velocity / AdamW first moment / Muon momentum, 1 = AdamW second moment. */
 SY_API sy_status sy_cuda_set_optimizer_state(sy_session *session, int32_t index, int32_t moment, const float *host,
                                       int64_t count);
 SY_API sy_status sy_cuda_get_optimizer_state(const sy_session *session, int32_t index, int32_t moment, float *host,
@@ -354,6 +356,89 @@ SY_API sy_status sy_cuda_wait_limit_selftest(int32_t device, int32_t spins, int3
  * the result is not finite.  has_grad == 0 leaves everything untouched. */
 SY_API sy_status sy_cuda_sgd_update(int32_t device, float *weight, float *velocity, float *grad, int64_t count, float lr,
                              float momentum, float weight_decay, int32_t images, int32_t has_grad);
+
+/* ---- operators on device memory ----
+ * Every pointer named below is memory of GPU `device` (checked); the work is queued on `stream` (a cudaStream_t
+ * of that device, NULL: the legacy default stream) and the call returns at once, without allocating or
+ * waiting, so it may be captured into a CUDA graph.  The caller's current device is left as it was.  Buffers stay
+ * alive and unchanged until the stream has passed the call; outputs must not overlap inputs; a workspace serves
+ * one call at a time (calls that may overlap on the GPU, and graphs that may replay at the same time, need one each).
+ * `status` (optional, int32 the caller sets to 0) receives SY_ERR_DEVICE when a bounded wait inside a kernel gave
+ * up and SY_ERR_NONFINITE where a call says so, and is otherwise left alone.
+ * Matrices are row-major; pitches count elements.  Sizes of 0 are allowed.  No counterpart in the reference. */
+#define SY_TYPE_F32 0
+#define SY_TYPE_BF16 1
+#define SY_TYPE_F16 2
+#define SY_FP8_E4M3 0
+#define SY_FP8_E5M2 1
+
+/* 8-bit matrices with a power-of-two scale per block.  Blocks are 128 columns of one row (block_rows 1) or of
+ * 128 rows (block_rows 128); a value is held as q * 2^e with e the smallest integer >= -126 for which the block's
+ * largest finite |x| is at most 448 * 2^e (e4m3) or 57344 * 2^e (e5m2), 0 for a block of zeros, and q rounded to
+ * nearest, ties to even.  NaN stays NaN; an infinity stays one in e5m2 and becomes NaN in e4m3.
+ * Layout of a rows x cols matrix: q bytes [rows][cols rounded up to 16], 16-byte aligned; scale bytes e + 127
+ * [rows / block_rows rounded up][ceil(cols / 128) rounded up to 4], 4-byte aligned.  sy_cuda_fp8_bytes and
+ * sy_cuda_fp8_scale_bytes give the sizes. */
+SY_API int64_t sy_cuda_fp8_bytes(int32_t rows, int32_t cols);
+SY_API int64_t sy_cuda_fp8_scale_bytes(int32_t rows, int32_t cols, int32_t block_rows);
+/* Casts x [rows][cols] (type SY_TYPE_*, x_pitch elements between rows) to 8 bits.  With qt and scale_t it also
+ * writes the transposed matrix [cols][rows], its blocks along the rows of x: the operand of a weight gradient,
+ * from the same read of x. */
+SY_API sy_status sy_cuda_quantize_fp8_device(int32_t device, const void *x, int32_t x_type, int64_t x_pitch, int32_t rows,
+                                             int32_t cols, int32_t format, int32_t block_rows, uint8_t *q,
+                                             uint8_t *scale, uint8_t *qt, uint8_t *scale_t, void *stream);
+/* The values q * 2^e, rounded to out_type. */
+SY_API sy_status sy_cuda_dequantize_fp8_device(int32_t device, const uint8_t *q, const uint8_t *scale, int32_t rows,
+                                               int32_t cols, int32_t format, int32_t block_rows, void *out,
+                                               int32_t out_type, int64_t out_pitch, void *stream);
+/* out[m][n] = a[m][k] * b[n][k]^T of two 8-bit matrices, either format and either block_rows each, accumulated in
+ * FP32; accumulate adds to what out holds (SY_TYPE_F32 only).  A linear layer y = x w^T with the casts of x, w, dy
+ * and their transposes: y = product(x, w), dx = product(dy, wt), dw = product(dyt, xt).  k = 0 gives zeros. */
+SY_API sy_status sy_cuda_matmul_fp8_device(int32_t device, const uint8_t *a, const uint8_t *a_scale, int32_t a_format,
+                                           int32_t a_block_rows, const uint8_t *b, const uint8_t *b_scale,
+                                           int32_t b_format, int32_t b_block_rows, int32_t m, int32_t n, int32_t k,
+                                           void *out, int32_t out_type, int64_t out_pitch, int32_t accumulate,
+                                           int32_t *status, void *stream);
+
+/* Orthogonalises x [rows][cols] by `steps` (1 .. 16; Muon uses 5) Newton-Schulz iterations: X = x / |x|_F
+ * (transposed while it has more rows than columns), then X <- a X + (b A + c A^2) X with A = X X^T and
+ * (a, b, c) = (3.4445, -4.7750, 2.0315).  A zero matrix gives zeros, one whose norm is not finite NaN.  With an
+ * SY_TYPE_F32 output the products carry 22 significant bits per operand, with 16-bit outputs 11 (as TF32 does).
+ * The workspace (sy_cuda_orthogonalize_workspace bytes, any alignment, no initial contents) is overwritten. */
+SY_API int64_t sy_cuda_orthogonalize_workspace(int32_t rows, int32_t cols, int32_t out_type);
+SY_API sy_status sy_cuda_orthogonalize_device(int32_t device, const void *x, int32_t x_type, int64_t x_pitch, int32_t rows,
+                                              int32_t cols, int32_t steps, void *out, int32_t out_type,
+                                              int64_t out_pitch, void *workspace, int64_t workspace_bytes,
+                                              int32_t *status, void *stream);
+/* One weight matrix of a Muon step: contiguous float [rows][cols] on the device. */
+typedef struct sy_muon_tensor {
+    float *weight, *momentum;
+    const float *grad;
+    int32_t rows, cols;
+} sy_muon_tensor;
+/* m <- momentum m + grad_scale g;  u = grad_scale g + momentum m (nesterov) or m;
+ * w <- w (1 - lr weight_decay) - lr rms sqrt(max(rows, cols)) orthogonalize(u).
+ * rms 0.2 gives updates the size of AdamW's, so that one learning rate serves both.  precision:
+ * SY_PRECISION_3XTF32 for products with 22 significant bits per operand, SY_PRECISION_TF32 for 11. */
+typedef struct sy_muon_options {
+    int32_t struct_size;        /* sizeof(sy_muon_options) */
+    float lr, momentum, weight_decay, rms, grad_scale;
+    int32_t nesterov, steps, precision;
+} sy_muon_options;
+/* The Muon step of `count` matrices in one set of launches (tensors is host memory, read before the call
+ * returns; no two tensors share memory).  *status receives SY_ERR_NONFINITE when a new weight is not finite. */
+SY_API int64_t sy_cuda_muon_workspace(const sy_muon_tensor *tensors, int32_t count, const sy_muon_options *options);
+SY_API sy_status sy_cuda_muon_update_device(int32_t device, const sy_muon_tensor *tensors, int32_t count,
+                                            const sy_muon_options *options, void *workspace, int64_t workspace_bytes,
+                                            int32_t *status, void *stream);
+
+/* The same two on host buffers, beside sy_cuda_matmul and sy_cuda_sgd_update.  C[m,n] = A[m,k] * B[k,n] with A cast
+ * to 8 bits in blocks of 1 x 128 and B in blocks of 128 x 128.  The Muon step on one weight matrix [rows][cols]
+ * returns SY_ERR_NONFINITE (weight and momentum written) when a new weight is not finite; grad is not cleared. */
+SY_API sy_status sy_cuda_matmul_fp8(int32_t device, const float *a, const float *b, float *c, int32_t m, int32_t n,
+                                    int32_t k, int32_t format);
+SY_API sy_status sy_cuda_muon_update(int32_t device, float *weight, float *momentum, const float *grad, int32_t rows,
+                                     int32_t cols, const sy_muon_options *options);
 
 #ifdef __cplusplus
 }

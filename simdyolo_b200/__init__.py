@@ -25,6 +25,7 @@ SY_ERR_DEVICE = 5
 SY_ERR_OUT_OF_MEMORY = 6
 SY_OPT_SGD = 0
 SY_OPT_ADAMW = 1
+SY_OPT_MUON = 2
 SY_PRECISION_TF32 = 0
 SY_PRECISION_3XTF32 = 1
 SY_BACKBONE_NONE = 0
@@ -132,6 +133,22 @@ class TensorInfo(C.Structure):
                 ("numel", C.c_int64)]
 
 
+SY_TYPE_F32, SY_TYPE_BF16, SY_TYPE_F16 = 0, 1, 2
+SY_FP8_E4M3, SY_FP8_E5M2 = 0, 1
+
+
+class MuonTensor(C.Structure):
+    """One weight matrix of a Muon step: device addresses of contiguous float [rows][cols]."""
+    _fields_ = [("weight", C.c_void_p), ("momentum", C.c_void_p), ("grad", C.c_void_p), ("rows", C.c_int32),
+                ("cols", C.c_int32)]
+
+
+class MuonOptions(C.Structure):
+    _fields_ = [("struct_size", C.c_int32), ("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float),
+                ("rms", C.c_float), ("grad_scale", C.c_float), ("nesterov", C.c_int32), ("steps", C.c_int32),
+                ("precision", C.c_int32)]
+
+
 _lib = None
 
 
@@ -208,6 +225,23 @@ def lib():
                                               fp]
         L.sy_cuda_decode_detections.argtypes = [C.c_int32, fp, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                                 C.c_int32, lp, op, dp, ip]
+        i32, i64 = C.c_int32, C.c_int64
+        L.sy_cuda_fp8_bytes.argtypes = [i32, i32]
+        L.sy_cuda_fp8_scale_bytes.argtypes = [i32, i32, i32]
+        L.sy_cuda_quantize_fp8_device.argtypes = [i32, vp, i32, i64, i32, i32, i32, i32, vp, vp, vp, vp, vp]
+        L.sy_cuda_dequantize_fp8_device.argtypes = [i32, vp, vp, i32, i32, i32, i32, vp, i32, i64, vp]
+        L.sy_cuda_matmul_fp8_device.argtypes = [i32, vp, vp, i32, i32, vp, vp, i32, i32, i32, i32, i32, vp, i32, i64,
+                                                i32, vp, vp]
+        L.sy_cuda_orthogonalize_workspace.argtypes = [i32, i32, i32]
+        L.sy_cuda_orthogonalize_device.argtypes = [i32, vp, i32, i64, i32, i32, i32, vp, i32, i64, vp, i64, vp, vp]
+        mt, mo = C.POINTER(MuonTensor), C.POINTER(MuonOptions)
+        L.sy_cuda_muon_workspace.argtypes = [mt, i32, mo]
+        L.sy_cuda_muon_update_device.argtypes = [i32, mt, i32, mo, vp, i64, vp, vp]
+        L.sy_cuda_matmul_fp8.argtypes = [i32, fp, fp, fp, i32, i32, i32, i32]
+        L.sy_cuda_muon_update.argtypes = [i32, fp, fp, fp, i32, i32, mo]
+        for name in ("sy_cuda_fp8_bytes", "sy_cuda_fp8_scale_bytes", "sy_cuda_orthogonalize_workspace",
+                     "sy_cuda_muon_workspace"):
+            getattr(L, name).restype = i64
         _lib = L
     return _lib
 
@@ -224,7 +258,10 @@ EXPORTED = ["sy_cuda_nccl_unique_id", "sy_cuda_create", "sy_cuda_destroy", "sy_c
             "sy_cuda_conv_profile_launches", "sy_cuda_get_optimizer_steps", "sy_cuda_set_optimizer_steps",
             "sy_cuda_wait_limit_selftest", "sy_cuda_detect", "sy_cuda_detect_features",
             "sy_cuda_get_last_head_outputs", "sy_cuda_head_decode", "sy_cuda_end_to_end_topk",
-            "sy_cuda_decode_detections", "sy_cuda_prefetch_images"]
+            "sy_cuda_decode_detections", "sy_cuda_prefetch_images", "sy_cuda_fp8_bytes", "sy_cuda_fp8_scale_bytes",
+            "sy_cuda_quantize_fp8_device", "sy_cuda_dequantize_fp8_device", "sy_cuda_matmul_fp8_device",
+            "sy_cuda_orthogonalize_workspace", "sy_cuda_orthogonalize_device", "sy_cuda_muon_workspace",
+            "sy_cuda_muon_update_device", "sy_cuda_matmul_fp8", "sy_cuda_muon_update"]
 
 
 def _check(status: int, session=None):
@@ -863,3 +900,93 @@ def matmul(a, b, device=0):
 def sgd_update(w, v, g, lr, momentum, wd, images, has_grad=True, device=0):
     """TrainingParameter.Update on float32 arrays in place; raises NonFinite like the reference."""
     _check(lib().sy_cuda_sgd_update(device, _fp(w), _fp(v), _fp(g), w.size, lr, momentum, wd, images, int(has_grad)))
+
+
+def matmul_fp8(a, b, fmt: int = SY_FP8_E4M3, device: int = 0):
+    """C = A @ B in 8-bit floating point: A cast in blocks of 1 x 128, B in blocks of 128 x 128."""
+    a = np.ascontiguousarray(a, np.float32)
+    b = np.ascontiguousarray(b, np.float32)
+    m, k = a.shape
+    n = b.shape[1]
+    c = np.zeros((m, n), np.float32)
+    _check(lib().sy_cuda_matmul_fp8(device, _fp(a), _fp(b), _fp(c), m, n, k, fmt))
+    return c
+
+
+def muon_options(lr: float, momentum: float = 0.95, weight_decay: float = 0.0, rms: float = 0.2, grad_scale: float = 1.0,
+                 nesterov: bool = True, steps: int = 5, precision: int = SY_PRECISION_3XTF32) -> MuonOptions:
+    """The Muon update's settings (sy_muon_options)."""
+    return MuonOptions(C.sizeof(MuonOptions), lr, momentum, weight_decay, rms, grad_scale, int(nesterov), steps, precision)
+
+
+def muon_update(w, m, g, options: MuonOptions, device: int = 0):
+    """The Muon step on float32 matrices w and m in place, beside sgd_update; raises NonFinite like it."""
+    rows, cols = w.shape
+    _check(lib().sy_cuda_muon_update(device, _fp(w), _fp(m), _fp(g), rows, cols, C.byref(options)))
+
+
+# ------------------------------------------------------------------ operators on device memory
+# Device addresses as integers, queued on `stream` (an integer cudaStream_t, 0: the legacy default stream);
+# include/simdyolo_cuda.h has the layouts and what a call may and may not do.
+
+def fp8_pitch(cols: int) -> int:
+    """Bytes between rows of an 8-bit matrix."""
+    return (cols + 15) // 16 * 16
+
+
+def fp8_scale_pitch(cols: int) -> int:
+    """Bytes between rows of an 8-bit matrix's scales (one per 128 columns)."""
+    return ((cols + 127) // 128 + 3) // 4 * 4
+
+
+def quantize_fp8_device(x: int, x_type: int, x_pitch: int, rows: int, cols: int, fmt: int, block_rows: int, q: int,
+                        scale: int, qt: int = 0, scale_t: int = 0, stream: int = 0, device: int = 0):
+    """Casts x [rows][cols] to 8 bits with a scale per block of block_rows x 128; qt / scale_t: the transposed copy."""
+    _check(lib().sy_cuda_quantize_fp8_device(device, x, x_type, x_pitch, rows, cols, fmt, block_rows, q, scale, qt,
+                                             scale_t, stream))
+
+
+def dequantize_fp8_device(q: int, scale: int, rows: int, cols: int, fmt: int, block_rows: int, out: int, out_type: int,
+                          out_pitch: int, stream: int = 0, device: int = 0):
+    """The values of an 8-bit matrix, rounded to out_type."""
+    _check(lib().sy_cuda_dequantize_fp8_device(device, q, scale, rows, cols, fmt, block_rows, out, out_type, out_pitch,
+                                               stream))
+
+
+def matmul_fp8_device(a: int, a_scale: int, a_fmt: int, a_block_rows: int, b: int, b_scale: int, b_fmt: int,
+                      b_block_rows: int, m: int, n: int, k: int, out: int, out_type: int, out_pitch: int,
+                      accumulate: bool = False, status: int = 0, stream: int = 0, device: int = 0):
+    """out [m][n] (+)= a [m][k] b [n][k]^T of two 8-bit matrices."""
+    _check(lib().sy_cuda_matmul_fp8_device(device, a, a_scale, a_fmt, a_block_rows, b, b_scale, b_fmt, b_block_rows, m, n,
+                                           k, out, out_type, out_pitch, int(accumulate), status, stream))
+
+
+def orthogonalize_workspace(rows: int, cols: int, out_type: int) -> int:
+    """Bytes orthogonalize_device needs."""
+    return int(lib().sy_cuda_orthogonalize_workspace(rows, cols, out_type))
+
+
+def orthogonalize_device(x: int, x_type: int, x_pitch: int, rows: int, cols: int, steps: int, out: int, out_type: int,
+                         out_pitch: int, workspace: int, workspace_bytes: int, status: int = 0, stream: int = 0,
+                         device: int = 0):
+    """Newton-Schulz orthogonalisation of x [rows][cols]."""
+    _check(lib().sy_cuda_orthogonalize_device(device, x, x_type, x_pitch, rows, cols, steps, out, out_type, out_pitch,
+                                              workspace, workspace_bytes, status, stream))
+
+
+def muon_tensors(entries):
+    """Packs (weight, momentum, grad, rows, cols) entries (device addresses) for muon_update_device."""
+    entries = list(entries)
+    return (MuonTensor * len(entries))(*[MuonTensor(*e) for e in entries])
+
+
+def muon_workspace(tensors, options: MuonOptions) -> int:
+    """Bytes muon_update_device needs for these tensors."""
+    return int(lib().sy_cuda_muon_workspace(tensors, len(tensors), C.byref(options)))
+
+
+def muon_update_device(tensors, options: MuonOptions, workspace: int, workspace_bytes: int, status: int = 0,
+                       stream: int = 0, device: int = 0):
+    """The Muon step of every tensor in the list (muon_tensors)."""
+    _check(lib().sy_cuda_muon_update_device(device, tensors, len(tensors), C.byref(options), workspace, workspace_bytes,
+                                            status, stream))

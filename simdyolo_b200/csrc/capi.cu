@@ -99,6 +99,92 @@ void check_device(int device) {
     CK(cudaSetDevice(device));
 }
 
+// Argument checks of the operators on device memory: everything is checked before anything is queued.
+[[noreturn]] void fail(const char* what, const std::string& why) {
+    throw sy::SyError(SY_ERR_INVALID_ARGUMENT, std::string(what) + ": " + why);
+}
+
+size_t element_bytes(int type) { return type == SY_TYPE_F32 ? 4 : 2; }
+
+void check_matrix(int type, int rows, int cols, int64_t pitch, const char* what) {
+    if (type != SY_TYPE_F32 && type != SY_TYPE_BF16 && type != SY_TYPE_F16) fail(what, "unknown element type");
+    if (rows < 0 || cols < 0) fail(what, "negative size");
+    if (pitch < cols) fail(what, "pitch below the row length");
+    if (rows > 0 && pitch > INT64_MAX / 16 / rows) fail(what, "pitch out of range");
+}
+
+void check_format(int format, const char* what) {
+    if (format != SY_FP8_E4M3 && format != SY_FP8_E5M2) fail(what, "unknown 8-bit format");
+}
+
+void check_block_rows(int block_rows, const char* what) {
+    if (block_rows != 1 && block_rows != 128) fail(what, "block_rows must be 1 or 128");
+}
+
+void check_steps(int steps, const char* what) {
+    if (steps < 1 || steps > 16) fail(what, "steps must be 1 .. 16");
+}
+
+// Tile counts of the products are 32-bit: 2^31 tiles of 128 x 128.
+void check_ns_size(int rows, int cols, const char* what) {
+    if (std::min(rows, cols) > (1 << 20) || (int64_t)rows * cols > ((int64_t)1 << 40))
+        throw sy::SyError(SY_ERR_UNSUPPORTED_SHAPE, std::string(what) + ": matrix too large");
+}
+
+void check_aligned(const void* p, size_t bytes, const char* what, const char* name) {
+    if (!p) fail(what, std::string(name) + " is null");
+    if (reinterpret_cast<uintptr_t>(p) % bytes) fail(what, std::string(name) + " is not aligned");
+}
+
+// A host pointer, or one of another GPU, is refused here instead of faulting in a kernel.  Null is passed over.
+void check_on_device(const void* p, int device, const char* what) {
+    if (!p) return;
+    cudaPointerAttributes a{};
+    CK(cudaPointerGetAttributes(&a, p));
+    if ((a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) || a.device != device)
+        fail(what, "pointer is not memory of the device");
+}
+
+// Makes `device` current for the call and restores the caller's device after it.
+struct DeviceScope {
+    int before = 0;
+    explicit DeviceScope(int device) {
+        int count = 0;
+        if (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count)
+            throw sy::SyError(SY_ERR_INVALID_ARGUMENT, "invalid CUDA device");
+        CK(cudaGetDevice(&before));
+        if (before != device) CK(cudaSetDevice(device));
+        current = device;
+    }
+    ~DeviceScope() {
+        if (before != current) cudaSetDevice(before);
+    }
+    int current = 0;
+};
+
+sy::MuonRule muon_rule(const sy_muon_options* o, const char* what) {
+    if (!o || o->struct_size != (int32_t)sizeof(sy_muon_options)) fail(what, "bad options");
+    for (float v : {o->lr, o->momentum, o->weight_decay, o->rms, o->grad_scale})
+        if (!std::isfinite(v)) fail(what, "options must be finite");
+    if (!(o->lr >= 0) || !(o->momentum >= 0 && o->momentum < 1) || !(o->weight_decay >= 0) || !(o->rms >= 0))
+        fail(what, "bad hyper-parameters");
+    check_steps(o->steps, what);
+    if (o->precision != SY_PRECISION_TF32 && o->precision != SY_PRECISION_3XTF32) fail(what, "unknown precision");
+    return sy::MuonRule{o->lr,         o->momentum,         o->weight_decay, o->rms,
+                        o->grad_scale, o->nesterov ? 1 : 0, o->steps,        o->precision == SY_PRECISION_3XTF32};
+}
+
+std::vector<sy::MuonMatrix> muon_matrices(const sy_muon_tensor* t, int count, const char* what) {
+    if (count < 0 || (count > 0 && !t)) fail(what, "bad tensor list");
+    std::vector<sy::MuonMatrix> m;
+    for (int i = 0; i < count; i++) {
+        if (t[i].rows < 0 || t[i].cols < 0) fail(what, "negative size");
+        check_ns_size(t[i].rows, t[i].cols, what);
+        m.push_back({t[i].weight, t[i].momentum, t[i].grad, t[i].rows, t[i].cols});
+    }
+    return m;
+}
+
 }  // namespace
 
 extern "C" {
@@ -722,6 +808,230 @@ sy_status sy_cuda_sgd_update(int32_t device, float* weight, float* velocity, flo
         CK(cudaMemcpy(velocity, v, count * sizeof(float), cudaMemcpyDeviceToHost));
         if (bad) throw sy::SyError(SY_ERR_NONFINITE, "sgd_update: non-finite parameters");
         CK(cudaMemcpy(grad, g, count * sizeof(float), cudaMemcpyDeviceToHost));
+        return SY_OK;
+    });
+}
+
+sy_status sy_cuda_matmul_fp8(int32_t device, const float* a, const float* b, float* c, int32_t m, int32_t n, int32_t k,
+                             int32_t format) {
+    return guarded(nullptr, [&] {
+        if (!a || !b || !c || m < 1 || n < 1 || k < 1)
+            throw sy::SyError(SY_ERR_INVALID_ARGUMENT, "matmul_fp8: bad arguments");
+        check_format(format, "matmul_fp8");
+        check_device(device);
+        Scratch s;
+        const size_t na = (size_t)m * k, nb = (size_t)k * n, nc = (size_t)m * n;
+        float* da = s.get<float>(na);
+        float* db = s.get<float>(nb);
+        float* dc = s.get<float>(nc);
+        int* status = s.get<int>(1);
+        uint8_t* qa = s.get<uint8_t>(sy_cuda_fp8_bytes(m, k));
+        uint8_t* sa = s.get<uint8_t>(sy_cuda_fp8_scale_bytes(m, k, 1));
+        uint8_t* qb = s.get<uint8_t>(sy_cuda_fp8_bytes(k, n));
+        uint8_t* sb = s.get<uint8_t>(sy_cuda_fp8_scale_bytes(k, n, 128));
+        uint8_t* qbt = s.get<uint8_t>(sy_cuda_fp8_bytes(n, k));
+        uint8_t* sbt = s.get<uint8_t>(sy_cuda_fp8_scale_bytes(n, k, 128));
+        CK(cudaMemcpy(da, a, na * sizeof(float), cudaMemcpyHostToDevice));
+        CK(cudaMemcpy(db, b, nb * sizeof(float), cudaMemcpyHostToDevice));
+        const bool e5m2 = format == SY_FP8_E5M2;
+        sy::fp8_quantize(da, sy::kTypeF32, k, m, k, e5m2, 1, qa, sa, nullptr, nullptr, 0);
+        sy::fp8_quantize(db, sy::kTypeF32, n, k, n, e5m2, 128, qb, sb, qbt, sbt, 0);
+        sy::fp8_matmul({qa, sa, m, e5m2, 1}, {qbt, sbt, n, e5m2, 128}, k, dc, sy::kTypeF32, n, false, status, 0);
+        CK(cudaMemcpy(c, dc, nc * sizeof(float), cudaMemcpyDeviceToHost));
+        int e = 0;
+        CK(cudaMemcpy(&e, status, sizeof(int), cudaMemcpyDeviceToHost));
+        if (e) throw sy::SyError(e, "matmul_fp8 kernel wait limit exceeded");
+        return SY_OK;
+    });
+}
+
+sy_status sy_cuda_muon_update(int32_t device, float* weight, float* momentum, const float* grad, int32_t rows,
+                              int32_t cols, const sy_muon_options* options) {
+    return guarded(nullptr, [&] {
+        if (!weight || !momentum || !grad || rows < 1 || cols < 1)
+            throw sy::SyError(SY_ERR_INVALID_ARGUMENT, "muon_update: bad arguments");
+        const sy::MuonRule rule = muon_rule(options, "muon_update");
+        check_device(device);
+        Scratch s;
+        const size_t n = (size_t)rows * cols;
+        float* w = s.get<float>(n);
+        float* v = s.get<float>(n);
+        float* g = s.get<float>(n);
+        int* status = s.get<int>(1);
+        CK(cudaMemcpy(w, weight, n * sizeof(float), cudaMemcpyHostToDevice));
+        CK(cudaMemcpy(v, momentum, n * sizeof(float), cudaMemcpyHostToDevice));
+        CK(cudaMemcpy(g, grad, n * sizeof(float), cudaMemcpyHostToDevice));
+        const sy::MuonMatrix mat{w, v, g, rows, cols};
+        uint8_t* ws = s.get<uint8_t>(sy::muon_workspace_bytes(&mat, 1, rule.split));
+        sy::muon_update(&mat, 1, rule, ws, status, 0);
+        int e = 0;
+        CK(cudaMemcpy(&e, status, sizeof(int), cudaMemcpyDeviceToHost));
+        CK(cudaMemcpy(weight, w, n * sizeof(float), cudaMemcpyDeviceToHost));
+        CK(cudaMemcpy(momentum, v, n * sizeof(float), cudaMemcpyDeviceToHost));
+        if (e == SY_ERR_NONFINITE) throw sy::SyError(e, "muon_update: non-finite parameters");
+        if (e) throw sy::SyError(SY_ERR_DEVICE, "muon_update kernel wait limit exceeded");
+        return SY_OK;
+    });
+}
+
+// ---- operators on device memory ----
+
+int64_t sy_cuda_fp8_bytes(int32_t rows, int32_t cols) {
+    return rows < 0 || cols < 0 ? 0 : (int64_t)rows * sy::fp8_pitch(cols);
+}
+
+int64_t sy_cuda_fp8_scale_bytes(int32_t rows, int32_t cols, int32_t block_rows) {
+    if (rows < 0 || cols < 0 || (block_rows != 1 && block_rows != 128)) return 0;
+    return ((int64_t)rows + block_rows - 1) / block_rows * sy::fp8_scale_pitch(cols);
+}
+
+sy_status sy_cuda_quantize_fp8_device(int32_t device, const void* x, int32_t x_type, int64_t x_pitch, int32_t rows,
+                                      int32_t cols, int32_t format, int32_t block_rows, uint8_t* q, uint8_t* scale,
+                                      uint8_t* qt, uint8_t* scale_t, void* stream) {
+    return guarded(nullptr, [&] {
+        const char* what = "quantize_fp8_device";
+        check_matrix(x_type, rows, cols, x_pitch, what);
+        check_format(format, what);
+        check_block_rows(block_rows, what);
+        if (!qt != !scale_t) fail(what, "qt and scale_t come together");
+        if (rows == 0 || cols == 0) return SY_OK;
+        check_aligned(x, element_bytes(x_type), what, "x");
+        check_aligned(q, 16, what, "q");
+        check_aligned(scale, 4, what, "scale");
+        if (qt) {
+            check_aligned(qt, 16, what, "qt");
+            check_aligned(scale_t, 4, what, "scale_t");
+        }
+        DeviceScope scope(device);
+        for (const void* p : {x, (const void*)q, (const void*)scale, (const void*)qt, (const void*)scale_t})
+            check_on_device(p, device, what);
+        sy::fp8_quantize(x, x_type, x_pitch, rows, cols, format == SY_FP8_E5M2, block_rows, q, scale, qt, scale_t,
+                         static_cast<cudaStream_t>(stream));
+        return SY_OK;
+    });
+}
+
+sy_status sy_cuda_dequantize_fp8_device(int32_t device, const uint8_t* q, const uint8_t* scale, int32_t rows,
+                                        int32_t cols, int32_t format, int32_t block_rows, void* out, int32_t out_type,
+                                        int64_t out_pitch, void* stream) {
+    return guarded(nullptr, [&] {
+        const char* what = "dequantize_fp8_device";
+        check_matrix(out_type, rows, cols, out_pitch, what);
+        check_format(format, what);
+        check_block_rows(block_rows, what);
+        if (rows == 0 || cols == 0) return SY_OK;
+        check_aligned(q, 16, what, "q");
+        check_aligned(scale, 4, what, "scale");
+        check_aligned(out, element_bytes(out_type), what, "out");
+        DeviceScope scope(device);
+        for (const void* p : {(const void*)q, (const void*)scale, (const void*)out}) check_on_device(p, device, what);
+        sy::fp8_dequantize(q, scale, rows, cols, format == SY_FP8_E5M2, block_rows, out, out_type, out_pitch,
+                           static_cast<cudaStream_t>(stream));
+        return SY_OK;
+    });
+}
+
+sy_status sy_cuda_matmul_fp8_device(int32_t device, const uint8_t* a, const uint8_t* a_scale, int32_t a_format,
+                                    int32_t a_block_rows, const uint8_t* b, const uint8_t* b_scale, int32_t b_format,
+                                    int32_t b_block_rows, int32_t m, int32_t n, int32_t k, void* out, int32_t out_type,
+                                    int64_t out_pitch, int32_t accumulate, int32_t* status, void* stream) {
+    return guarded(nullptr, [&] {
+        const char* what = "matmul_fp8_device";
+        check_matrix(out_type, m, n, out_pitch, what);
+        check_format(a_format, what);
+        check_format(b_format, what);
+        check_block_rows(a_block_rows, what);
+        check_block_rows(b_block_rows, what);
+        if (k < 0) fail(what, "negative size");
+        if (accumulate && out_type != SY_TYPE_F32) fail(what, "accumulate needs an SY_TYPE_F32 output");
+        if (m == 0 || n == 0) return SY_OK;
+        check_aligned(out, element_bytes(out_type), what, "out");
+        if (k > 0) {
+            check_aligned(a, 16, what, "a");
+            check_aligned(b, 16, what, "b");
+            check_aligned(a_scale, 4, what, "a_scale");
+            check_aligned(b_scale, 4, what, "b_scale");
+        }
+        if (status) check_aligned(status, 4, what, "status");
+        DeviceScope scope(device);
+        if (k > 0)
+            for (const void* p : {a, b, a_scale, b_scale}) check_on_device(p, device, what);
+        check_on_device(out, device, what);
+        check_on_device(status, device, what);
+        sy::fp8_matmul({a, a_scale, m, a_format == SY_FP8_E5M2, a_block_rows},
+                       {b, b_scale, n, b_format == SY_FP8_E5M2, b_block_rows}, k, out, out_type, out_pitch,
+                       accumulate != 0, status, static_cast<cudaStream_t>(stream));
+        return SY_OK;
+    });
+}
+
+int64_t sy_cuda_orthogonalize_workspace(int32_t rows, int32_t cols, int32_t out_type) {
+    return rows < 0 || cols < 0 ? 0 : (int64_t)sy::orthogonalize_workspace_bytes(rows, cols, out_type);
+}
+
+sy_status sy_cuda_orthogonalize_device(int32_t device, const void* x, int32_t x_type, int64_t x_pitch, int32_t rows,
+                                       int32_t cols, int32_t steps, void* out, int32_t out_type, int64_t out_pitch,
+                                       void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+    return guarded(nullptr, [&] {
+        const char* what = "orthogonalize_device";
+        check_matrix(x_type, rows, cols, x_pitch, what);
+        check_matrix(out_type, rows, cols, out_pitch, what);
+        check_steps(steps, what);
+        if (rows == 0 || cols == 0) return SY_OK;
+        check_ns_size(rows, cols, what);
+        check_aligned(x, element_bytes(x_type), what, "x");
+        check_aligned(out, element_bytes(out_type), what, "out");
+        check_aligned(workspace, 1, what, "workspace");
+        if (workspace_bytes < sy_cuda_orthogonalize_workspace(rows, cols, out_type)) fail(what, "workspace too small");
+        if (status) check_aligned(status, 4, what, "status");
+        DeviceScope scope(device);
+        for (const void* p : {x, (const void*)out, (const void*)workspace, (const void*)status})
+            check_on_device(p, device, what);
+        sy::orthogonalize(x, x_type, x_pitch, rows, cols, steps, out, out_type, out_pitch, workspace, status,
+                          static_cast<cudaStream_t>(stream));
+        return SY_OK;
+    });
+}
+
+int64_t sy_cuda_muon_workspace(const sy_muon_tensor* tensors, int32_t count, const sy_muon_options* options) {
+    int64_t bytes = 0;
+    guarded(nullptr, [&] {
+        const sy::MuonRule rule = muon_rule(options, "muon_workspace");
+        const std::vector<sy::MuonMatrix> m = muon_matrices(tensors, count, "muon_workspace");
+        bytes = (int64_t)sy::muon_workspace_bytes(m.data(), count, rule.split);
+        return SY_OK;
+    });
+    return bytes;
+}
+
+sy_status sy_cuda_muon_update_device(int32_t device, const sy_muon_tensor* tensors, int32_t count,
+                                     const sy_muon_options* options, void* workspace, int64_t workspace_bytes,
+                                     int32_t* status, void* stream) {
+    return guarded(nullptr, [&] {
+        const char* what = "muon_update_device";
+        const sy::MuonRule rule = muon_rule(options, what);
+        const std::vector<sy::MuonMatrix> m = muon_matrices(tensors, count, what);
+        bool any = false;
+        for (const auto& t : m)
+            if (t.rows && t.cols) {
+                any = true;
+                check_aligned(t.weight, 4, what, "weight");
+                check_aligned(t.momentum, 4, what, "momentum");
+                check_aligned(t.grad, 4, what, "grad");
+            }
+        if (!any) return SY_OK;
+        check_aligned(workspace, 1, what, "workspace");
+        if (workspace_bytes < (int64_t)sy::muon_workspace_bytes(m.data(), count, rule.split))
+            fail(what, "workspace too small");
+        if (status) check_aligned(status, 4, what, "status");
+        DeviceScope scope(device);
+        for (const auto& t : m)
+            if (t.rows && t.cols)
+                for (const void* p : {(const void*)t.weight, (const void*)t.momentum, (const void*)t.grad})
+                    check_on_device(p, device, what);
+        check_on_device(workspace, device, what);
+        check_on_device(status, device, what);
+        sy::muon_update(m.data(), count, rule, workspace, status, static_cast<cudaStream_t>(stream));
         return SY_OK;
     });
 }

@@ -262,6 +262,43 @@ __device__ __forceinline__ void mma_tf32(uint32_t d_tmem, uint64_t adesc, uint64
         : "memory");
 }
 
+// Untiled bulk copy of `bytes` (a multiple of 16) from global memory into this CTA's own shared memory; both
+// addresses 16-byte aligned.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// D[tmem] (+)= A[smem desc] * B[smem desc], kind::f16 (both operands fp16), one CTA.
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// The same for 8-bit operands whose rows carry a UE8M0 scale per 32 elements along K, read from TMEM.
+__device__ __forceinline__ void mma_mxf8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
+        : "memory");
+}
+
+// 32 rows x 128 bits from shared memory to TMEM, repeated in all four 32-lane quarters (scale factors).
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t sdesc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+
 // Arrive on an mbarrier when all previously issued tcgen05.mma of this thread complete.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -335,7 +372,8 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
 //     accepts.  Each K row holds 128 B (32 elements) along MN, 32 B chunks XOR-ed with (row % 4),
 //     4-row K groups SBO apart, successive 128 B MN blocks LBO apart.  Matches TMA
 //     SWIZZLE_128B_ATOM_32B.
-constexpr uint32_t kLayoutSw128 = 2, kLayoutSw128Base32 = 1;
+//   K-major, no swizzle (layout type 0): 8-row x 16-byte core matrices, contiguous, SBO apart along the rows.
+constexpr uint32_t kLayoutNone = 0, kLayoutSw128 = 2, kLayoutSw128Base32 = 1;
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes, uint32_t layout) {
     uint64_t d = 0;
     d |= (uint64_t)((addr >> 4) & 0x3FFFu);
@@ -350,6 +388,18 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo_bytes,
 __host__ __device__ constexpr uint32_t idesc_tf32(int n, int a_mn_major, int b_mn_major) {
     return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)a_mn_major << 15) | ((uint32_t)b_mn_major << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// D f32, A/B f16, M = 128, A K-major.
+__host__ __device__ constexpr uint32_t idesc_f16(int n, int b_mn_major) {
+    return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// Block-scaled 8-bit operands (format 0 e4m3, 1 e5m2), UE8M0 scales, D f32, M = 128, both K-major; the byte of
+// the scale words that an instruction uses (0..3) is or-ed in at bits 4 (B) and 29 (A).
+__host__ __device__ constexpr uint32_t idesc_mxf8(int n, int a_format, int b_format) {
+    return ((uint32_t)a_format << 7) | ((uint32_t)b_format << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) |
+           ((uint32_t)(128 >> 4) << 24);
 }
 
 }  // namespace sy

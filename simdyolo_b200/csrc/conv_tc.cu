@@ -59,6 +59,8 @@ static CUtensorMap make_map_2d(const float* base, long inner, long outer, long p
     return map;
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() { return get_encode(); }
+
 static int num_sms() {
     static int n = 0;
     if (!n) {
@@ -68,6 +70,8 @@ static int num_sms() {
     }
     return n;
 }
+
+int device_sms() { return num_sms(); }
 
 // ------------------------------------------------------------------ forward / dgrad kernel
 // A CTA tile is T consecutive 128-row sub-tiles (M = 128 T output rows).  The taps are split into

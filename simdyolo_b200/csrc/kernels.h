@@ -2,6 +2,7 @@
 // activations use the padded channels-last layout described in common.cuh (sy::Grid).
 #pragma once
 #include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -55,6 +56,9 @@ struct View {
     int channels;
     long rows;
 };
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
+int device_sms();
 
 // ---------------------------------------------------------------- convolution (tcgen05)
 // Implicit-GEMM convolution over the padded layout, stride 1, k in {1,3}:
@@ -367,5 +371,51 @@ void check_finite(const float* v, long n, int* flag, cudaStream_t stream);
 // part[kAbsSumBlocks] = block partial sums of |v| (fixed order, summed on the host)
 constexpr int kAbsSumBlocks = 64;
 void abs_sum_partials(const float* v, long n, double* part, cudaStream_t stream);
+
+// ---------------------------------------------------------------- 8-bit casts and product (fp8.cu)
+// Element types of the device-pointer operators (SY_TYPE_*), and what their kernels write to *status (the
+// sy_status values): a wait that gave up, a result that is not finite.
+constexpr int kTypeF32 = 0, kTypeBF16 = 1, kTypeF16 = 2;
+constexpr int kStatusNonFinite = 3, kStatusWait = 5;
+
+// Row pitches in bytes of an 8-bit matrix and of its scales (one per 128 columns).
+inline long fp8_pitch(long cols) { return (cols + 15) / 16 * 16; }
+inline long fp8_scale_pitch(long cols) { return ((cols + 127) / 128 + 3) / 4 * 4; }
+// q [rows][fp8_pitch(cols)], scale [rows / block_rows rounded up][fp8_scale_pitch(cols)]; qt / scale_t (optional)
+// the same for the transposed matrix.
+void fp8_quantize(const void* x, int x_type, long x_pitch, int rows, int cols, bool e5m2, int block_rows, uint8_t* q,
+                  uint8_t* scale, uint8_t* qt, uint8_t* scale_t, cudaStream_t stream);
+void fp8_dequantize(const uint8_t* q, const uint8_t* scale, int rows, int cols, bool e5m2, int block_rows, void* out,
+                    int out_type, long out_pitch, cudaStream_t stream);
+struct Fp8Operand {
+    const uint8_t *q, *scale;
+    int rows;
+    bool e5m2;
+    int block_rows;
+};
+// out[i * out_pitch + j] (+)= sum_k a[i, k] b[j, k]; accumulate needs a float output.
+void fp8_matmul(const Fp8Operand& a, const Fp8Operand& b, int k, void* out, int out_type, long out_pitch,
+                bool accumulate, int* status, cudaStream_t stream);
+
+// ---------------------------------------------------------------- Newton-Schulz orthogonalisation, Muon (muon.cu)
+// One matrix [rows][cols] of a call.  Muon: momentum <- mu momentum + grad_scale grad, the direction u is
+// grad_scale grad + mu momentum (nesterov) or momentum, weight <- weight (1 - lr decay) - rate O(u).
+// Orthogonalisation alone (weight null): u is `in`, out receives O(u).
+struct MuonMatrix {
+    float *weight, *momentum;
+    const float* grad;
+    int rows, cols;
+};
+struct MuonRule {
+    float lr, momentum, decay, rms, grad_scale;
+    int nesterov, steps;
+    bool split;     // operands as fp16 pairs (22 bits) and three products, or single fp16 (11 bits)
+};
+size_t muon_workspace_bytes(const MuonMatrix* m, int count, bool split);
+void muon_update(const MuonMatrix* m, int count, const MuonRule& rule, void* workspace, int* status,
+                 cudaStream_t stream);
+size_t orthogonalize_workspace_bytes(int rows, int cols, int out_type);
+void orthogonalize(const void* in, int in_type, long in_pitch, int rows, int cols, int steps, void* out, int out_type,
+                   long out_pitch, void* workspace, int* status, cudaStream_t stream);
 
 }  // namespace sy

@@ -1,0 +1,256 @@
+"""Casts to 8 bits and the block-scaled product on the GPU against their definitions in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import simdyolo_b200 as sy
+from tests import device_ops as D
+
+pytestmark = pytest.mark.gpu
+
+
+def spread(rows, cols, seed, dtype=torch.float32):
+    """Values over a wide range of sizes: per-row and per-column factors, some zeros."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp(2 * torch.randn(rows, 1, generator=g))
+    x = x * torch.exp(torch.randn(1, cols, generator=g))
+    x[torch.rand(rows, cols, generator=g) < 0.02] = 0
+    return x.to(dtype)
+
+
+# ------------------------------------------------------------------ casts: equal to the definition, bit for bit
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows, cols", [(1, 1), (1, 300), (3, 127), (127, 5), (128, 128), (129, 257), (200, 640)])
+def test_cast_both_ways(rows, cols, dtype, block_rows, fmt):
+    x = spread(rows, cols, rows * 1000 + cols, dtype)
+    q, e = D.cast_reference(x, fmt, block_rows)
+    qt, et = D.cast_reference(x.T, fmt, block_rows)
+    one = D.quantize(x.cuda(), fmt, block_rows)
+    h, t = D.quantize(x.cuda(), fmt, block_rows, both=True)
+    for got in (one, h):
+        assert torch.equal(got.exponents(), e)
+        assert torch.equal(got.data().view(torch.uint8), q.view(torch.uint8))
+    assert torch.equal(t.exponents(), et)
+    assert torch.equal(t.data().view(torch.uint8), qt.view(torch.uint8))
+    assert torch.equal(D.dequantize(h, torch.float32).cpu().double(), D.values(q, e, block_rows))
+    assert torch.equal(D.dequantize(t, dtype).cpu(), D.values(qt, et, block_rows).float().to(dtype))
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("offset, pitch", [(0, 208), (1, 201), (8, 216)])
+def test_cast_of_strided_rows(offset, pitch, block_rows):
+    base = spread(40, pitch + 16, 5, torch.bfloat16).cuda()
+    x = base.view(-1)[offset:].as_strided((40, 200), (pitch, 1))
+    q, e = D.cast_reference(x.cpu(), "e4m3", block_rows)
+    h, t = D.quantize(x, "e4m3", block_rows, both=True)
+    assert torch.equal(h.data().view(torch.uint8), q.view(torch.uint8)) and torch.equal(h.exponents(), e)
+    qt, _ = D.cast_reference(x.cpu().T, "e4m3", block_rows)
+    assert torch.equal(t.data().view(torch.uint8), qt.view(torch.uint8))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("both", [False, True])
+def test_cast_of_extreme_values(fmt, both):
+    x = torch.zeros(130, 300)
+    x[0, :130] = torch.finfo(torch.float32).max
+    x[1, 5] = torch.finfo(torch.float32).smallest_normal
+    x[1, 200] = 2.0 ** -149
+    x[2, 3], x[2, 4], x[2, 5], x[2, 6] = float("inf"), -float("inf"), float("nan"), 3.0
+    x[3, 128:256] = float("nan")
+    x[4, :4] = torch.tensor([448.0, 449.0, 57344.0, 57345.0])
+    x[5, 0], x[5, 130] = 448.0, 57344.0
+    x[6, 0], x[6, 130] = -448.0 * (1 + 2.0 ** -23), 57344.0 * (1 + 2.0 ** -23)
+    x[7, 0], x[7, 1] = 1.0, -0.0
+    for block_rows in (1, 128):
+        q, e = D.cast_reference(x, fmt, block_rows)
+        h = D.quantize(x.cuda(), fmt, block_rows, both=both)
+        h = h[0] if both else h
+        assert torch.equal(h.exponents(), e)
+        a, b = h.data().float(), q.float()
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a[~a.isnan()], b[~b.isnan()])
+
+
+def test_dequantize_takes_any_scale_byte_and_leaves_the_rows_padding():
+    h = D.Held(4, 130, "e4m3", 1)
+    h.q[:] = torch.arange(4 * h.q.shape[1], dtype=torch.int64, device="cuda").view(4, -1).remainder(127).to(torch.uint8)
+    h.scale[:] = 127
+    h.scale[1, 0], h.scale[2, 0], h.scale[3, 1] = 0, 255, 254
+    out = D.dequantize(h, torch.float32, pitch=140).cpu()
+    assert (out[:, 130:] == 7).all()
+    assert out[2, :128].isnan().all() and not out[2, 128:].isnan().any()
+    want = h.values()
+    want[2, :128] = float("nan")
+    assert torch.equal(out[1, :130].double(), want[1].float().double())
+    assert torch.equal(out[3, :130].double(), want[3].float().double())
+
+
+# ------------------------------------------------------------------ products
+
+def operands(m, n, k, a_fmt="e4m3", b_fmt="e4m3", a_block=1, b_block=128, seed=0):
+    a = D.quantize(spread(m, k, seed + 1).cuda(), a_fmt, a_block)
+    b = D.quantize(spread(n, k, seed + 2).cuda(), b_fmt, b_block)
+    return a, b
+
+
+def check(a, b, dtype, got, start=None):
+    va, vb = a.values(), b.values()
+    want = va @ vb.T
+    bound = D.product_bound(va, vb, dtype, want)
+    if start is not None:
+        want = want + start.double().cpu()
+        bound = bound + D.HALF_STEP[dtype] * want.abs()
+    got = got.double().cpu()
+    if dtype == torch.float16:
+        fits = want.abs() < 65000
+        got, want, bound = got[fits], want[fits], bound[fits] + 2.0 ** -25   # below 2^-14 the step is 2^-24
+    assert ((got - want).abs() <= bound).all(), ((got - want).abs() / bound).max()
+
+
+@pytest.mark.parametrize("m, n, k", [
+    (1, 1, 1), (1, 16, 128), (1, 300, 1000), (2, 129, 127), (16, 128, 129), (17, 257, 513), (33, 1000, 2000),
+    (65, 130, 4100), (127, 255, 640), (128, 128, 128), (129, 64, 200), (200, 33, 8000), (300, 1, 384), (513, 300, 256),
+    (1000, 1000, 700), (2300, 2500, 300)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_product_sizes(m, n, k, dtype):
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    a, b = operands(m, n, k)
+    check(a, b, dtype, D.matmul(a, b, dtype, status=status))
+    assert status.item() == 0
+
+
+@pytest.mark.parametrize("a_fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("b_fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("a_block, b_block", [(1, 1), (1, 128), (128, 1), (128, 128)])
+@pytest.mark.parametrize("m, n, k", [(40, 300, 900), (300, 40, 900), (260, 390, 520)])
+def test_product_formats_and_blocks(m, n, k, a_fmt, b_fmt, a_block, b_block):
+    a, b = operands(m, n, k, a_fmt, b_fmt, a_block, b_block)
+    check(a, b, torch.float16, D.matmul(a, b, torch.float16))
+    check(a, b, torch.float32, D.matmul(a, b, torch.float32))
+
+
+@pytest.mark.parametrize("m, n, k", [(5, 300, 1100), (300, 5, 1100), (300, 500, 300)])
+@pytest.mark.parametrize("pad", [0, 3, 4])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_product_into_strided_rows_leaves_the_rest(m, n, k, pad, dtype):
+    a, b = operands(m, n, k)
+    buf = torch.full((m + 2, n + pad), 7.0, dtype=dtype, device="cuda")
+    D.matmul(a, b, dtype, out=buf)
+    check(a, b, dtype, buf[:m, :n])
+    assert (buf[m:] == 7).all() and (buf[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("m, n, k", [(3, 200, 3000), (200, 3, 3000), (400, 300, 500), (130, 140, 0)])
+def test_product_accumulates(m, n, k):
+    start = torch.randn(m, n, generator=torch.Generator().manual_seed(3))
+    out = start.cuda()
+    if k == 0:
+        e = torch.empty(16, dtype=torch.uint8, device="cuda")
+        for add, want in ((True, start), (False, start * 0)):
+            sy.matmul_fp8_device(e.data_ptr(), e.data_ptr(), 0, 1, e.data_ptr(), e.data_ptr(), 0, 1, m, n, 0,
+                                 out.data_ptr(), sy.SY_TYPE_F32, n, add, stream=D.stream())
+            assert torch.equal(out.cpu(), want)
+        return
+    a, b = operands(m, n, k)
+    D.matmul(a, b, torch.float32, out=out, accumulate=True)
+    check(a, b, torch.float32, out, start)
+
+
+def test_product_is_the_same_every_time():
+    a, b = operands(7, 900, 8000)
+    first = D.matmul(a, b, torch.float32)
+    for _ in range(5):
+        assert torch.equal(D.matmul(a, b, torch.float32), first)
+
+
+@pytest.mark.parametrize("m, n", [(4, 300), (300, 200)])
+def test_nan_reaches_its_own_row_and_column_only(m, n):
+    x, w = spread(m, 500, 1), spread(n, 500, 2)
+    x[2, 77], w[5, 400] = float("nan"), float("nan")
+    a, b = D.quantize(x.cuda(), "e4m3", 1), D.quantize(w.cuda(), "e4m3", 1)
+    out = D.matmul(a, b, torch.float32).cpu()
+    bad = torch.zeros(m, n, dtype=torch.bool)
+    bad[2], bad[:, 5] = True, True
+    assert torch.equal(out.isnan(), bad)
+
+
+def test_unused_bytes_of_the_operands_do_not_matter():
+    """Bytes past a row's end and scales past its last block hold anything."""
+    a, b = operands(30, 140, 130)
+    want = D.matmul(a, b, torch.float32)
+    for h in (a, b):
+        h.q[:, h.cols:] = 0x7f
+        h.scale[:, -(-h.cols // 128):] = 0xff
+    assert torch.equal(D.matmul(a, b, torch.float32), want)
+
+
+def test_host_form():
+    rng = np.random.default_rng(0)
+    x, w = rng.standard_normal((50, 300)).astype(np.float32), rng.standard_normal((300, 70)).astype(np.float32)
+    for fmt in ("e4m3", "e5m2"):
+        qa, ea = D.cast_reference(torch.from_numpy(x), fmt, 1)
+        qb, eb = D.cast_reference(torch.from_numpy(w.T.copy()), fmt, 128)
+        va, vb = D.values(qa, ea, 1), D.values(qb, eb, 128)
+        got = torch.from_numpy(sy.matmul_fp8(x, w, D.FORMATS[fmt][0])).double()
+        assert ((got - va @ vb.T).abs() <= D.product_bound(va, vb, torch.float32, va @ vb.T)).all()
+
+
+def test_host_pointers_are_refused():
+    x = np.zeros((4, 256), np.float32)
+    h = D.Held(4, 256, "e4m3", 1)
+    with pytest.raises(sy.InvalidArgument, match="memory of the device"):
+        sy.quantize_fp8_device(x.ctypes.data, sy.SY_TYPE_F32, 256, 4, 256, 0, 1, h.q.data_ptr(), h.scale.data_ptr())
+
+
+def test_graph_replays_follow_their_inputs_and_streams():
+    """Two captured chains (cast, product) on two streams, replayed with new inputs in the same buffers."""
+    chains = []
+    for seed in (1, 2):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            x = spread(20, 700, seed).cuda()
+            w = D.quantize(spread(300, 700, seed + 5).cuda(), "e4m3", 128)
+            out = torch.empty(20, 300, device="cuda")
+            D.matmul(D.quantize(x, "e4m3", 1), w, torch.float32, out=out)
+            s.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                h = D.quantize(x, "e4m3", 1)
+                D.matmul(h, w, torch.float32, out=out)
+        chains.append((s, g, x, w, out, h))
+    torch.cuda.synchronize()
+    for turn in range(3):
+        fresh = [spread(20, 700, 10 * turn + i).cuda() for i in range(2)]
+        torch.cuda.synchronize()
+        for (s, g, x, *_), f in zip(chains, fresh):
+            with torch.cuda.stream(s):
+                x.copy_(f)
+                g.replay()
+        torch.cuda.synchronize()
+        for (_, _, x, w, out, h), f in zip(chains, fresh):
+            assert torch.equal(out, D.matmul(D.quantize(f, "e4m3", 1), w, torch.float32))
+
+
+def test_a_linear_layers_gradients_against_formula_and_differences():
+    """y = x w^T in 8 bits with its three products, and differences of the loss sum(dy * y) of the cast operands:
+    linear in each operand, so a difference is exact but for the rounding of its terms."""
+    t, n, k = 96, 160, 200
+    x, w, dy = spread(t, k, 1).cuda(), spread(n, k, 2).cuda() / 14, spread(t, n, 3).cuda()
+    hx, hxt = D.quantize(x, "e4m3", 1, both=True)
+    hw, hwt = D.quantize(w, "e4m3", 128, both=True)
+    hd, hdt = D.quantize(dy, "e5m2", 1, both=True)
+    y, dx, dw = D.matmul(hx, hw, torch.float32), D.matmul(hd, hwt, torch.float32), D.matmul(hdt, hxt, torch.float32)
+    check(hx, hw, torch.float32, y)
+    check(hd, hwt, torch.float32, dx)
+    check(hdt, hxt, torch.float32, dw)
+    vw, vd = hw.values(), hd.values()
+    loss = lambda v: (vd * (v @ vw.T)).sum()
+    vx = hx.values()
+    bound = D.product_bound(vd, hwt.values(), torch.float32, vd @ vw)
+    for i, j in [(0, 0), (50, 130), (95, 199)]:
+        step = torch.zeros_like(vx)
+        step[i, j] = 1.0
+        diff = (loss(vx + step) - loss(vx - step)) / 2
+        assert abs(dx[i, j].item() - diff) <= bound[i, j] + 1e-9 * loss(vx.abs()).abs()

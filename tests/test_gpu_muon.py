@@ -1,0 +1,225 @@
+"""Newton-Schulz orthogonalisation and the Muon step on the GPU against their definitions in 64 bits.
+
+Tolerances (relative 2-norm of a whole matrix).  22-bit operands: an iteration's three products each round two
+operands to 2^-22 and drop lo * lo (2^-22), so five iterations are within 5 * 3 * 3 * 2^-22 = 1.1e-5 in the
+directions whose singular values the iteration flattens, which hold nearly all of a random matrix's norm; twice
+that covers the FP32 accumulation.  11-bit operands: the same count with 2^-11 / 2 per rounding (no dropped term)
+is 5 * 3 * 2 * 2^-12 = 7.3e-3.  Outputs add half a step of their type.
+"""
+import numpy as np
+import pytest
+import torch
+
+import simdyolo_b200 as sy
+from tests import device_ops as D
+
+pytestmark = pytest.mark.gpu
+SPLIT_TOL, SINGLE_TOL = 2.2e-5, 7.3e-3
+
+
+def update(rows, cols, seed, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    k = min(8, rows, cols)
+    low = torch.randn(rows, k, generator=g) @ torch.randn(k, cols, generator=g)
+    return (1e-3 * (low + torch.randn(rows, cols, generator=g))).to(dtype)
+
+
+SHAPES = [(1, 1), (1, 300), (300, 1), (2, 2), (17, 5), (64, 576), (80, 720), (127, 129), (128, 128), (129, 640),
+          (576, 64), (700, 333), (130, 2304), (512, 512)]
+
+
+@pytest.mark.parametrize("rows, cols", SHAPES)
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_orthogonalize_shapes(rows, cols, out):
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    u = update(rows, cols, rows + cols)
+    got = D.orthogonalize(u.cuda(), out, status=status)
+    tol = SPLIT_TOL if out == torch.float32 else SINGLE_TOL + D.HALF_STEP[out]
+    assert D.rel(got, D.orthogonal_reference(u)) <= tol
+    assert status.item() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows, cols", [(64, 200), (200, 64)])
+def test_orthogonalize_reads_types_and_strides_and_leaves_padding(dtype, rows, cols):
+    base = torch.zeros(rows, cols + 13, dtype=dtype)
+    base[:, 1:cols + 1] = update(rows, cols, 4).to(dtype)
+    x = base.cuda()[:, 1:cols + 1]
+    got = D.orthogonalize(x, torch.float32, pitch=cols + 3)
+    assert D.rel(got[:, :cols], D.orthogonal_reference(base[:, 1:cols + 1])) <= SPLIT_TOL
+    assert (got[:, cols:] == 7).all()
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 6])
+def test_orthogonalize_steps(steps):
+    u = update(90, 150, 1)
+    assert D.rel(D.orthogonalize(u.cuda(), torch.float32, steps), D.orthogonal_reference(u, steps)) <= SPLIT_TOL
+
+
+@pytest.mark.parametrize("scale", [1e-38, 1e-30, 1e30, 3e37])
+def test_orthogonalize_does_not_depend_on_the_scale(scale):
+    u = update(100, 180, 2).double() * 1e3
+    u = (u / u.abs().max() * scale).float()
+    assert D.rel(D.orthogonalize(u.cuda(), torch.float32), D.orthogonal_reference(u)) <= SPLIT_TOL
+
+
+def test_orthogonalize_of_zero_and_of_values_that_are_not_finite():
+    z = torch.zeros(70, 90, device="cuda")
+    for out in (torch.float32, torch.bfloat16):
+        assert (D.orthogonalize(z, out) == 0).all()
+    for v in (float("nan"), float("inf")):
+        z[3, 4] = v
+        assert D.orthogonalize(z, torch.bfloat16).isnan().all()
+
+
+def test_orthogonalize_a_few_strong_directions():
+    """A matrix of rank 3 (its other singular values are zero) and one diagonal matrix with a wide spectrum."""
+    g = torch.Generator().manual_seed(0)
+    low = torch.randn(200, 3, generator=g) @ torch.randn(3, 300, generator=g)
+    diag = torch.diag(2.0 ** -torch.arange(64, dtype=torch.float32))
+    # the null directions of `low` hold only its own FP32 rounding (2^-24), which the iteration raises 485 times
+    assert D.rel(D.orthogonalize(low.cuda(), torch.float32), D.orthogonal_reference(low)) <= SPLIT_TOL + 485 * 2.0 ** -22
+    assert D.rel(D.orthogonalize(diag.cuda(), torch.float32), D.orthogonal_reference(diag)) <= SPLIT_TOL
+
+
+def lists(shapes, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    w = [torch.randn(r, c, generator=g) / c ** 0.5 for r, c in shapes]
+    m = [update(r, c, seed + i) for i, (r, c) in enumerate(shapes)]
+    d = [update(r, c, seed + 100 + i) for i, (r, c) in enumerate(shapes)]
+    return w, m, d
+
+
+def check_muon(shapes, opts, options, tol_o, seed=0):
+    w, m, d = lists(shapes, seed)
+    cw, cm, cd = ([x.cuda() for x in v] for v in (w, m, d))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    keep = D.muon(cw, cm, cd, options, status)
+    for i in range(len(shapes)):
+        want_w, want_m = D.muon_reference(w[i], m[i], d[i], **opts)
+        # the step may be off by tol_o of itself, the weight by two FP32 roundings
+        step = (want_w - w[i].double() * (1 - opts["lr"] * opts.get("weight_decay", 0.0))).norm()
+        off = (cw[i].cpu().double() - want_w).norm()
+        assert off <= tol_o * step + 3 * 2.0 ** -24 * (want_w.norm() + step), shapes[i]
+        assert D.rel(cm[i], want_m) <= 3 * 2.0 ** -24
+        assert torch.equal(cd[i].cpu(), d[i])
+    assert status.item() == 0
+    return keep
+
+
+@pytest.mark.parametrize("opts", [
+    dict(lr=0.02), dict(lr=0.02, momentum=0.9, weight_decay=0.1, nesterov=False),
+    dict(lr=0.5, momentum=0.0, rms=1.0, grad_scale=0.125, steps=3)])
+@pytest.mark.parametrize("precision, tol", [(sy.SY_PRECISION_3XTF32, SPLIT_TOL), (sy.SY_PRECISION_TF32, SINGLE_TOL)])
+def test_muon_list(opts, precision, tol):
+    shapes = [(64, 576), (1, 7), (300, 40), (80, 80), (129, 130), (5, 1)]
+    check_muon(shapes, opts, sy.muon_options(precision=precision, **opts), tol)
+
+
+def test_muon_of_more_matrices_than_one_launch_takes():
+    shapes = [(8 + i, 200 - 2 * i) for i in range(70)]
+    check_muon(shapes, dict(lr=0.02), sy.muon_options(0.02), SPLIT_TOL)
+
+
+def test_muon_list_equals_its_matrices_one_by_one():
+    shapes = [(64, 300), (150, 70), (256, 256)]
+    w, m, d = lists(shapes, 9)
+    o = sy.muon_options(0.02)
+    cw, cm, cd = ([x.cuda() for x in v] for v in (w, m, d))
+    keep = [D.muon(cw, cm, cd, o)]
+    for i in range(3):
+        a, b = w[i].cuda(), m[i].cuda()
+        keep.append(D.muon([a], [b], [cd[i]], o))
+        assert torch.equal(a, cw[i]) and torch.equal(b, cm[i])
+
+
+def test_muon_skips_empty_matrices_and_reports_values_that_are_not_finite():
+    w, m, d = ([x.cuda() for x in v] for v in lists([(16, 20), (30, 8)], 3))
+    e = torch.zeros(0, 4, device="cuda")
+    d[1][3, 3] = float("inf")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    keep = D.muon([w[0], e, w[1]], [m[0], e, m[1]], [d[0], e, d[1]], sy.muon_options(0.02), status)
+    assert status.item() == sy.SY_ERR_NONFINITE
+    assert w[0].isfinite().all() and w[1].isnan().all()
+    del keep
+
+
+def test_graphs_with_their_own_workspaces_replay_side_by_side():
+    o = sy.muon_options(0.02, weight_decay=0.01)
+    runs = []
+    for seed in (1, 2):
+        w, m, d = ([x.cuda() for x in v] for v in lists([(64, 200), (100, 60)], seed))
+        t = sy.muon_tensors([(a.data_ptr(), b.data_ptr(), c.data_ptr(), *a.shape) for a, b, c in zip(w, m, d)])
+        work = torch.empty(sy.muon_workspace(t, o), dtype=torch.uint8, device="cuda")
+        s = torch.cuda.Stream()
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            sy.muon_update_device(t, o, work.data_ptr(), work.numel(), stream=torch.cuda.current_stream().cuda_stream)
+        runs.append((s, g, w, m, d, work, t))
+    del t   # the list is read during the call
+    eager = [[[x.clone() for x in v] for v in r[2:5]] for r in runs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, g, *_ in runs:
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for r, (w, m, d) in zip(runs, eager):
+        keep = [D.muon(w, m, d, o) for _ in range(3)]
+        torch.cuda.synchronize()
+        for a, b in zip(r[2], w):
+            assert torch.equal(a, b)
+        del keep
+
+
+def test_workspace_of_any_alignment():
+    w, m, d = ([x.cuda() for x in v] for v in lists([(50, 90)], 5))
+    w2, m2 = w[0].clone(), m[0].clone()
+    o = sy.muon_options(0.02)
+    keep = D.muon(w, m, d, o)
+    t = sy.muon_tensors([(w2.data_ptr(), m2.data_ptr(), d[0].data_ptr(), 50, 90)])
+    need = sy.muon_workspace(t, o)
+    work = torch.full((need + 77,), 0x7f, dtype=torch.uint8, device="cuda")
+    sy.muon_update_device(t, o, work.data_ptr() + 7, need, stream=D.stream())
+    assert torch.equal(w2, w[0])
+    assert (work[:7] == 0x7f).all() and (work[7 + need:] == 0x7f).all()
+    del keep
+
+
+def test_host_form_matches_the_device_form():
+    w, m, d = lists([(60, 100)], 6)
+    o = sy.muon_options(0.02, weight_decay=0.05)
+    cw, cm = w[0].cuda(), m[0].cuda()
+    keep = D.muon([cw], [cm], [d[0].cuda()], o)
+    hw, hm, hg = (x[0].numpy().copy() for x in (w, m, d))
+    sy.muon_update(hw, hm, hg, o)
+    assert np.array_equal(hw, cw.cpu().numpy()) and np.array_equal(hm, cm.cpu().numpy())
+    hg[0, 0] = np.nan
+    with pytest.raises(sy.NonFinite):
+        sy.muon_update(hw, hm, hg, o)
+    del keep
+
+
+def test_an_8_bit_layer_trained_by_muon():
+    """Forward, backward and update as a training step runs them, on one stream, against the same in 64 bits."""
+    t, n, k = 256, 160, 192
+    g = torch.Generator().manual_seed(1)
+    x, target = torch.randn(t, k, generator=g), torch.randn(t, n, generator=g)
+    w, m = torch.randn(n, k, generator=g) / k ** 0.5, torch.zeros(n, k)
+    cx, ct, cw, cm = x.cuda(), target.cuda(), w.cuda(), m.cuda()
+    o = sy.muon_options(0.02)
+    keep = []
+    for _ in range(3):
+        hx, hxt = D.quantize(cx, "e4m3", 1, both=True)
+        y = D.matmul(hx, D.quantize(cw, "e4m3", 128), torch.float32)
+        hd, hdt = D.quantize(y - ct, "e5m2", 1, both=True)
+        dw = D.matmul(hdt, hxt, torch.float32)
+        before, mom = cw.cpu(), cm.cpu()
+        keep.append(D.muon([cw], [cm], [dw], o))
+        want, want_m = D.muon_reference(before, mom, dw.cpu(), 0.02)
+        step = (want - before.double()).norm()
+        assert (cw.cpu().double() - want).norm() <= SPLIT_TOL * step + 3 * 2.0 ** -24 * (want.norm() + step)
+        assert D.rel(cm, want_m) <= 3 * 2.0 ** -24
+        want_dw = hdt.values() @ hxt.values().T
+        assert ((dw.cpu().double() - want_dw).abs() <= D.product_bound(hdt.values(), hxt.values(), torch.float32, want_dw)).all()
