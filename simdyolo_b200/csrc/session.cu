@@ -646,7 +646,8 @@ void Session::build_head() {
             const std::string path = prefix + "." + block_path(i, n);
             const long wn = (long)b.oc * (b.ic / b.groups) * b.k * b.k;
             auto add_param = [&](const std::string& name, std::vector<int> shape, long numel, int decay) {
-                TensorEntry e{name, 0, shape, poff, numel, branch.group, decay};
+                const bool muon = cfg.optimizer == SY_OPT_MUON && decay && b.groups == 1;
+                TensorEntry e{name, 0, shape, poff, numel, branch.group, decay, muon};
                 tensors.push_back(e);
                 long off = poff;
                 poff += numel;
@@ -677,13 +678,13 @@ void Session::build_head() {
             if (!hb.b.has_bn) continue;
             const std::string path = prefix + "." + block_path(i, n);
             hb.rm_off = qoff;
-            tensors.push_back(TensorEntry{path + ".bn.running_mean", 1, {hb.b.oc}, qoff, hb.b.oc, 0, 0});
+            tensors.push_back(TensorEntry{path + ".bn.running_mean", 1, {hb.b.oc}, qoff, hb.b.oc, 0, 0, false});
             qoff += hb.b.oc;
             hb.rv_off = qoff;
-            tensors.push_back(TensorEntry{path + ".bn.running_var", 1, {hb.b.oc}, qoff, hb.b.oc, 0, 0});
+            tensors.push_back(TensorEntry{path + ".bn.running_var", 1, {hb.b.oc}, qoff, hb.b.oc, 0, 0, false});
             qoff += hb.b.oc;
             hb.nt_off = qoff;
-            tensors.push_back(TensorEntry{path + ".bn.num_batches_tracked", 1, {}, qoff, 1, 0, 0});
+            tensors.push_back(TensorEntry{path + ".bn.num_batches_tracked", 1, {}, qoff, 1, 0, 0, false});
             qoff += 1;
         }
     }
@@ -703,10 +704,20 @@ void Session::build_head() {
                     for (int c = 0; c < hb.b.oc; c++) init[hb.rv_off + c] = 1.0f;
         SY_CUDA(cudaMemcpy(buffers_, init.data(), sizeof(float) * n_buffers, cudaMemcpyHostToDevice));
     }
-    // optimizer segments: one per parameter tensor
+    // optimizer segments: one per parameter tensor; Muon takes its matrices out of them
     std::vector<ParamSegment> segs;
-    for (auto& t : tensors)
-        if (t.kind == 0) segs.push_back(ParamSegment{t.offset, t.numel, t.decay, t.group});
+    for (auto& t : tensors) {
+        if (t.kind != 0) continue;
+        if (t.muon) {
+            muon_.push_back(MuonMatrix{params_ + t.offset, vel_ + t.offset, grads_ + t.offset, t.shape[0],
+                                       (int)(t.numel / t.shape[0])});
+            muon_group_.push_back(t.group);
+        } else {
+            segs.push_back(ParamSegment{t.offset, t.numel, t.decay, t.group});
+        }
+    }
+    if (!muon_.empty())
+        muon_ws_ = dalloc(muon_workspace_bytes(muon_.data(), (int)muon_.size(), cfg.precision == SY_PRECISION_3XTF32));
     nsegs_ = (int)segs.size();
     d_segs_ = static_cast<ParamSegment*>(dalloc(sizeof(ParamSegment) * segs.size()));
     SY_CUDA(cudaMemcpy(d_segs_, segs.data(), sizeof(ParamSegment) * segs.size(), cudaMemcpyHostToDevice));
@@ -1329,14 +1340,23 @@ int Session::step(const uint8_t* rgb, bool rgb_on_device, const float* const* fe
     const int has[3] = {1, connected & 1, (connected >> 1) & 1};
     for (int gi = 0; gi < 3; gi++) {
         h_flags_[2 + gi] = has[gi];
-        if (cfg.optimizer == SY_OPT_ADAMW && has[gi]) adam_steps_[gi]++;
+        if (cfg.optimizer != SY_OPT_SGD && has[gi]) adam_steps_[gi]++;
         h_flags_[5 + gi] = adam_steps_[gi];
     }
     h_flags_[1] = 0;
     SY_CUDA(cudaMemcpyAsync(d_flags_ + 1, h_flags_ + 1, sizeof(int) * 7, cudaMemcpyHostToDevice, stream_));
-    optimizer_step(cfg.optimizer, params_, vel_, vel2_, grads_, d_segs_, nsegs_, d_flags_ + 2, d_flags_ + 5, cfg.lr,
-                   cfg.momentum, cfg.weight_decay, cfg.beta1, cfg.beta2, cfg.adam_eps, 1.0f / (float)global_images,
-                   d_flags_ + 1, stream_);
+    optimizer_step(cfg.optimizer == SY_OPT_SGD ? SY_OPT_SGD : SY_OPT_ADAMW, params_, vel_, vel2_, grads_, d_segs_,
+                   nsegs_, d_flags_ + 2, d_flags_ + 5, cfg.lr, cfg.momentum, cfg.weight_decay, cfg.beta1, cfg.beta2,
+                   cfg.adam_eps, 1.0f / (float)global_images, d_flags_ + 1, stream_);
+    if (!muon_.empty()) {
+        std::vector<MuonMatrix> active;
+        for (size_t i = 0; i < muon_.size(); i++)
+            if (has[muon_group_[i]]) active.push_back(muon_[i]);
+        const MuonRule rule{cfg.lr, cfg.momentum, cfg.weight_decay, 0.2f, 1.0f / (float)global_images, 1, 5,
+                            cfg.precision == SY_PRECISION_3XTF32};
+        muon_update(active.data(), (int)active.size(), rule, muon_ws_, d_flags_ + 1, stream_);
+        SY_CUDA(cudaMemsetAsync(grads_, 0, sizeof(float) * n_params, stream_));
+    }
     refresh_head_weights();
     SY_CUDA(cudaMemcpyAsync(h_flags_, d_flags_, sizeof(int) * 2, cudaMemcpyDeviceToHost, stream_));
     SY_CUDA(cudaEventRecord(ev1_, stream_));
@@ -1356,7 +1376,7 @@ int Session::step(const uint8_t* rgb, bool rgb_on_device, const float* const* fe
         out->device_ms = ms;
         out->near_ties = near_ties;
     }
-    if (h_flags_[0]) throw SyError(SY_ERR_DEVICE, "device wait limit exceeded");
+    if (h_flags_[0] || h_flags_[1] == kStatusWait) throw SyError(SY_ERR_DEVICE, "device wait limit exceeded");
     if (h_flags_[1]) throw SyError(SY_ERR_NONFINITE, "non-finite parameters after the update");
     return SY_OK;
 }

@@ -31,6 +31,7 @@ struct TensorEntry {
     long numel;
     int group;           // parameters: 0 always connected, 1 box branch
     int decay;
+    bool muon;           // dense conv weight updated by Muon (SY_OPT_MUON)
 };
 
 struct HeadBlock {
@@ -270,7 +271,10 @@ private:
     double* h_abs_ = nullptr;
     ParamSegment* d_segs_ = nullptr;
     int nsegs_ = 0;
-    int adam_steps_[3] = {0, 0, 0};   // AdamW steps per optimizer group
+    std::vector<MuonMatrix> muon_;      // SY_OPT_MUON: the dense conv weights as [oc][ic * k * k], and the
+    std::vector<int> muon_group_;       // optimizer group of each
+    void* muon_ws_ = nullptr;
+    int adam_steps_[3] = {0, 0, 0};   // AdamW steps per optimizer group (also of SY_OPT_MUON)
     int n_sets_ = 1;                  // 2 with the one-to-one branches
     bool progressive_ = false;        // end-to-end with reg_max 1 (TrainingHeadSchema.Progressive)
     int epoch_ = 0;

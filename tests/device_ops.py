@@ -113,6 +113,29 @@ def orthogonal_reference(u, steps=5):
     return x
 
 
+def orthogonal_bound(u, unit, steps=5):
+    """How far ||O - reference||_F may be when every operand (X, A, B) carries a relative rounding error `unit`.
+    The iteration maps singular values by p(s) = a s + b s^3 + c s^5; on [0, 1.203], where they stay, |p'| <= 3.97
+    (at s = 1.203), and the derivative of such a map of a matrix is bounded in the Frobenius norm by that slope
+    (Daleckii-Krein: its factors are quotients (p(s) -+ p(t)) / (s -+ t)).  An error made in one iteration is
+    therefore raised at most 3.97 times by each later one.  One iteration adds, with ||X||_2 <= 1.203 and
+    ||A||_2 <= 1.447: unit ||X'||_F for storing X', unit ||B||_F ||X||_2 for B, and unit ||A||_F times the slope of
+    b A + c A^2 (|b| + 2 |c| ||A||_2 = 10.66) times ||X||_2 for A; the first X is rounded once."""
+    x = u.double()
+    x = x.T if x.shape[0] > x.shape[1] else x
+    norm = x.norm()
+    if norm == 0:
+        return 0.0
+    x = x / norm
+    total = unit * x.norm()
+    for _ in range(steps):
+        a = x @ x.T
+        b = NS[1] * a + NS[2] * a @ a
+        x = NS[0] * x + b @ x
+        total = 3.97 * total + unit * (x.norm() + 1.203 * (b.norm() + 10.66 * a.norm()))
+    return total.item()
+
+
 def orthogonalize(x, dtype, steps=5, pitch=None, status=None):
     rows, cols = x.shape
     out = torch.full((rows, pitch or cols), 7.0, dtype=dtype, device="cuda")
