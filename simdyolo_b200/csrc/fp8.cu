@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(256)
 
 constexpr int kTileRows = 128, kBlockK = 128;
 constexpr int kScaleSlots = 4;   // groups of four K blocks whose scale words are in flight
-constexpr int kThreads = 256;    // TMA, MMA, scales, TMEM allocation, then four epilogue warps
+constexpr int kThreads = 256;    // TMA, MMA, scales, MMA-side waits, then four epilogue warps
+constexpr int kStageBar = 1;     // named barrier: a stage is loaded (the waiting warp and the MMA warp)
 
 struct ProductParams {
     int rows[2];                 // [0] the MMA's M side, [1] its N side
@@ -367,8 +368,9 @@ __device__ __forceinline__ void put_row32(const ProductParams& p, int i, int j, 
 }
 
 // c = a b^T on 128 x BN tiles, one CTA per tile and K split.  Both operands stream through shared memory in
-// blocks of 128 along K (one scale per row and block, 128-byte swizzled rows); one thread issues four
-// 128 x BN x 32 block-scaled MMAs per block.  A warp gathers the rows' scale words (four K blocks each) into
+// blocks of 128 along K (one scale per row and block, 128-byte swizzled rows); one warp issues four
+// 128 x BN x 32 block-scaled MMAs per block and touches no shared memory itself: a warp that has MMAs in flight
+// waits ~1,200 cycles for any shared-memory access, an mbarrier wait included, so another warp does its waiting.  A warp gathers the rows' scale words (four K blocks each) into
 // 512-byte atoms, which the MMA thread copies to TMEM ahead of the MMAs that use them.  K splits form a cluster:
 // each CTA leaves its partial tile in its shared memory and sums a share of the tile over the cluster in rank
 // order, so the result does not depend on timing and no workspace is needed.
@@ -429,38 +431,43 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = max(0, i - S::kStages); j < i; j++)
                 mbar_wait(&full[j % S::kStages], (j / S::kStages) & 1, p.status, kStatusWait);
         }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t st0 = smem_u32(smem), sc0 = smem_u32(ssm);
-            int group = 0;
-            bool ok = true;
-            for (int i = 0; ok && i < k1 - k0; i++) {
-                const int s = i % S::kStages, kb = k0 + i, slot = group % kScaleSlots;
-                const uint32_t tsc = tmem + BN + slot * S::kScaleCols;
-                if (i == 0 || (kb & 3) == 0) {
-                    if (!(ok = mbar_wait(&sfull[slot], (group / kScaleSlots) & 1, p.status, kStatusWait))) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int a = 0; a < 1 + S::kScaleRows; a++)
-                        tmem_cp_scales(tsc + 4 * a,
-                                       smem_desc(sc0 + slot * S::kScaleBytes + a * 512, 0, 128, kLayoutNone));
-                }
-                if (!(ok = mbar_wait(&full[s], (i / S::kStages) & 1, p.status, kStatusWait))) break;
-                tc_fence_after();
-                const uint64_t da = smem_desc(st0 + s * S::kStageBytes, 0, 1024, kLayoutSw128);
-                const uint64_t db = smem_desc(st0 + s * S::kStageBytes + kTileRows * kBlockK, 0, 1024, kLayoutSw128);
-                const uint32_t idesc = p.idesc | (uint32_t)(kb & 3) << 4 | (uint32_t)(kb & 3) << 29;
-#pragma unroll
-                for (int k = 0; k < kBlockK / 32; k++)
-                    mma_mxf8(tmem, da + 2 * k, db + 2 * k, idesc, tsc, tsc + 4, (i | k) != 0);
-                mma_commit(&empty[s]);
-                if ((kb & 3) == 3) {
-                    mma_commit(&sempty[slot]);
-                    group++;
-                }
-            }
-            mma_commit(done);
+    } else if (warp == 3) {
+        // every wait of the MMA side; after one that gave up the hand-offs go on, so that every warp finishes
+        bool live = true;
+        for (int i = 0, group = 0; i < k1 - k0; i++) {
+            const int s = i % S::kStages, kb = k0 + i;
+            if (live && (i == 0 || (kb & 3) == 0))
+                live = mbar_wait(&sfull[group % kScaleSlots], (group / kScaleSlots) & 1, p.status, kStatusWait);
+            if (live) live = mbar_wait(&full[s], (i / S::kStages) & 1, p.status, kStatusWait);
+            if ((kb & 3) == 3) group++;
+            named_bar_sync(kStageBar, 64);
         }
+    } else if (warp == 1) {
+        const uint32_t st0 = smem_u32(smem), sc0 = smem_u32(ssm);
+        int group = 0;
+        for (int i = 0; i < k1 - k0; i++) {
+            const int s = i % S::kStages, kb = k0 + i, slot = group % kScaleSlots;
+            const uint32_t tsc = tmem + BN + slot * S::kScaleCols;
+            named_bar_sync(kStageBar, 64);   // stage (and its scales) loaded
+            tc_fence_after();
+            if (i == 0 || (kb & 3) == 0)
+#pragma unroll
+                for (int a = 0; a < 1 + S::kScaleRows; a++)
+                    tmem_cp_scales_elect(tsc + 4 * a,
+                                         smem_desc(sc0 + slot * S::kScaleBytes + a * 512, 0, 128, kLayoutNone));
+            const uint64_t da = smem_desc(st0 + s * S::kStageBytes, 0, 1024, kLayoutSw128);
+            const uint64_t db = smem_desc(st0 + s * S::kStageBytes + kTileRows * kBlockK, 0, 1024, kLayoutSw128);
+            const uint32_t idesc = p.idesc | (uint32_t)(kb & 3) << 4 | (uint32_t)(kb & 3) << 29;
+#pragma unroll
+            for (int k = 0; k < kBlockK / 32; k++)
+                mma_mxf8_elect(tmem, da + 2 * k, db + 2 * k, idesc, tsc, tsc + 4, (i | k) != 0);
+            mma_commit_elect(&empty[s]);
+            if ((kb & 3) == 3) {
+                mma_commit_elect(&sempty[slot]);
+                group++;
+            }
+        }
+        mma_commit_elect(done);
     } else if (warp == 2) {
         // lane l gathers rows l, l + 32, l + 64, l + 96: the four words of 16-byte row l of the atom
         const int g0 = k0 >> 2, g1 = (k1 + 3) >> 2;

@@ -39,34 +39,42 @@ constexpr int kMaxJobs = 32;                        // matrices per launch (kern
 constexpr int kMaxNormParts = 512;
 constexpr int kThreads = 256;
 
-struct Job {
-    uint8_t *x[2], *a, *b;      // hi tiles; the lo tiles follow at x_bytes / a_bytes
-    long x_bytes, a_bytes;
-    const double* norm;         // partial sums of squares of U
+// One matrix as the caller has it.
+struct Source {
     const void* in;             // orthogonalisation: U;  Muon: grad
-    float *weight, *momentum;
-    void* out;
+    float *weight, *momentum;   // Muon
+    void* out;                  // orthogonalisation
     long in_pitch, out_pitch;
     int r, c;                   // X is r x c
-    int rb, cb;                 // 128-row blocks of X; 64-column blocks (padded to a whole tile)
     int tall;                   // X is U transposed
     int p;                      // X is held times 2^p
     int in_type, out_type;
     float rate;                 // Muon: factor of O in the update
-    int tri0, full0;            // first tile of this job in the symmetric and in the full products
+    int vec;                    // rows of every matrix start on 16 bytes (8 for 16-bit types)
 };
 
-struct Jobs {
-    int count, tri_tiles, full_tiles, norm_parts;
+struct Settings {
     int steps, nesterov;
     float lr, momentum, decay, grad_scale;
     int* status;
+};
+
+struct Job : Source {
+    uint8_t *x[2], *a, *b;      // hi tiles; the lo tiles follow at x_bytes / a_bytes
+    long x_bytes, a_bytes;
+    const double* norm;         // partial sums of squares of U
+    int rb, cb;                 // 128-row blocks of X; 64-column blocks (padded to a whole tile)
+    int tri0, full0;            // first tile of this job in the symmetric and in the full products
+};
+
+struct Jobs : Settings {
+    int count, tri_tiles, full_tiles, norm_parts;
     Job job[kMaxJobs];
 };
 static_assert(sizeof(Jobs) <= 32000, "job table exceeds the kernel parameters");
 
 // element (row, col) of U: the orthogonalisation's input or Muon's direction
-__device__ __forceinline__ float direction(const Jobs& q, const Job& j, long row, long col) {
+__device__ __forceinline__ float direction(const Settings& q, const Source& j, long row, long col) {
     const long at = row * j.in_pitch + col;
     if (j.weight) {
         const float m = j.momentum[at];
@@ -226,20 +234,51 @@ __device__ __forceinline__ void write32(uint8_t* hi, uint8_t* lo, int row, int c
     }
 }
 
-// value v of O at (row, col) of X's orientation: the output, or the weight update
-__device__ __forceinline__ void finish(const Jobs& q, const Job& j, int row, int col, float v, bool& bad) {
+// N consecutive values of a row of O (X's orientation) from `col` on: the output, or the weight update.  The old
+// weights are all loaded before the first is stored, so that the loads overlap.
+template <int N>
+__device__ __forceinline__ void finish(const Settings& q, const Source& j, int row, int col, const float* v, bool& bad) {
     if (row >= j.r || col >= j.c) return;
-    const long at = j.tall ? col * j.out_pitch + row : row * j.out_pitch + col;
+    const int n = min(N, j.c - col);
+    const long at = j.tall ? col * j.out_pitch + row : row * j.out_pitch + col, step = j.tall ? j.out_pitch : 1;
     if (j.weight) {
-        const float w = j.weight[at] * (1.0f - q.lr * q.decay) - j.rate * v;
-        bad |= !(fabsf(w) <= 3.402823466e38f);
-        j.weight[at] = w;
+        float w[N];
+        const float keep = 1.0f - q.lr * q.decay;
+        if (!j.tall && j.vec && n == N) {
+            float4* p = reinterpret_cast<float4*>(j.weight + at);
+#pragma unroll
+            for (int k = 0; k < N / 4; k++) *reinterpret_cast<float4*>(w + 4 * k) = p[k];
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                w[k] = w[k] * keep - j.rate * v[k];
+                bad |= !(fabsf(w[k]) <= 3.402823466e38f);
+            }
+#pragma unroll
+            for (int k = 0; k < N / 4; k++) p[k] = *reinterpret_cast<const float4*>(w + 4 * k);
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) w[k] = k < n ? j.weight[at + k * step] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            w[k] = w[k] * keep - j.rate * v[k];
+            if (k < n) {
+                bad |= !(fabsf(w[k]) <= 3.402823466e38f);
+                j.weight[at + k * step] = w[k];
+            }
+        }
     } else if (j.out_type == kTypeF32) {
-        static_cast<float*>(j.out)[at] = v;
-    } else if (j.out_type == kTypeBF16) {
-        static_cast<__nv_bfloat16*>(j.out)[at] = __float2bfloat16_rn(v);
+        float* o = static_cast<float*>(j.out) + at;
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (k < n) o[k * step] = v[k];
     } else {
-        static_cast<__half*>(j.out)[at] = __float2half_rn(v);
+        uint16_t* o = static_cast<uint16_t*>(j.out) + at;
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (k < n)
+                o[k * step] = j.out_type == kTypeBF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v[k]))
+                                                      : __half_as_ushort(__float2half_rn(v[k]));
     }
 }
 
@@ -386,7 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1) ns_kernel(const __grid_constant__
                 if (LAST) {
                     const int row = at.i * kTile + r, col = at.j * kTile + c;
 #pragma unroll
-                    for (int k = 0; k < 32; k++) finish(q, j, row, col + k, v[k] * out_f, bad);
+                    for (int k = 0; k < 32; k++) v[k] *= out_f;
+                    finish<32>(q, j, row, col, v, bad);
                     continue;
                 }
                 uint8_t* dst = PHASE == kGram ? j.a : PHASE == kSquare ? j.b : j.x[src ^ 1];
@@ -417,6 +457,433 @@ __global__ void __launch_bounds__(kThreads, 1) ns_kernel(const __grid_constant__
     }
 }
 
+// ------------------------------------------------------------------ short matrices: one cluster each
+//
+// A matrix of at most 128 rows (of X) stays on chip for the whole call.  The CTAs of a cluster hold a slab of
+// columns each, in shared memory as operand tiles of `rows` x 64 (rows = r rounded up to 16).  Per iteration every
+// CTA forms X X^T over its columns, the cluster sums the partial products (each CTA a share of the rows, in rank
+// order) and hands every CTA the whole of A; A^2, B and B X are then local.  Three products and two cluster
+// barriers per iteration instead of three launches, and U is read and O written once.
+// The MMA always takes 128 rows: those past `rows` read whatever follows the tile in shared memory and land in
+// accumulator rows that nothing reads.
+
+constexpr int kSlabThreads = 256;
+constexpr int kSlabRound = 384;      // columns of B X in TMEM at a time, beside 128 for the products of A
+constexpr int kMaxSmem = 227 * 1024;
+
+struct SlabJob : Source {
+    int rows;                        // r rounded up to 16
+    int width;                       // columns per CTA, a multiple of 64
+    int first, ranks;                // its CTAs, all of one cluster
+};
+template <int N>
+struct SlabJobs : Settings {
+    int count;
+    SlabJob job[N];
+};
+
+__host__ __device__ constexpr int slab_x_bytes(int rows, int width) { return width / 64 * rows * 128; }   // one half
+__host__ __device__ constexpr int slab_a_bytes(int rows) { return (rows + 63) / 64 * rows * 128; }
+__host__ __device__ constexpr int slab_part_bytes(int rows) { return rows * (rows + 4) * 4; }
+int slab_smem(int rows, int width, bool split) {
+    const int tiles = (slab_x_bytes(rows, width) + slab_a_bytes(rows)) * (split ? 2 : 1);
+    // the last operand tile may be read for 128 rows
+    return 1024 + std::max(tiles + slab_part_bytes(rows), tiles - rows * 128 + 128 * 128);
+}
+
+__device__ __forceinline__ void slab_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float4 peer_load4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ void peer_store4(uint32_t addr, uint4 v) {
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                 : "memory");
+}
+__device__ __forceinline__ double peer_load_d(uint32_t addr) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// Four values of U from (row, col) on along its contiguous axis of `n` values; `raw` as stored (Muon: grad).
+__device__ __forceinline__ float4 load_u4(const void* in, int type, long at, int n, bool vec) {
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (n <= 0) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (type == kTypeF32) {
+        const float* p = static_cast<const float*>(in) + at;
+        if (vec && n >= 4) return *reinterpret_cast<const float4*>(p);
+        for (int i = 0; i < 4; i++)
+            if (i < n) v[i] = p[i];
+    } else {
+        const uint16_t* p = static_cast<const uint16_t*>(in) + at;
+        uint16_t h[4] = {0, 0, 0, 0};
+        if (vec && n >= 4) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            h[0] = (uint16_t)u.x, h[1] = (uint16_t)(u.x >> 16), h[2] = (uint16_t)u.y, h[3] = (uint16_t)(u.y >> 16);
+        } else {
+            for (int i = 0; i < 4; i++)
+                if (i < n) h[i] = p[i];
+        }
+        for (int i = 0; i < 4; i++)
+            v[i] = type == kTypeBF16 ? __uint_as_float((uint32_t)h[i] << 16) : __half2float(__ushort_as_half(h[i]));
+    }
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// byte offset of element (row, col) in slab tiles
+__device__ __forceinline__ int slab_offset(int row, int col, int rows) {
+    return (col >> 6) * rows * 128 + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
+}
+
+// 16 consecutive columns (a multiple of 16) of a row: value of hi + lo
+template <bool SPLIT>
+__device__ __forceinline__ void slab_read16(const uint8_t* hi, int lo, int row, int col, int rows, float* v) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint8_t* p = hi + slab_offset(row, col + 8 * k, rows);
+        const uint4 h = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+        for (int l = 0; l < 4; l++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[l]));
+            v[8 * k + 2 * l] = f.x, v[8 * k + 2 * l + 1] = f.y;
+        }
+        if (SPLIT) {
+            const uint4 g = *reinterpret_cast<const uint4*>(p + lo);
+            const uint32_t x[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+            for (int l = 0; l < 4; l++) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[l]));
+                v[8 * k + 2 * l] += f.x, v[8 * k + 2 * l + 1] += f.y;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void pack8(const float* v, uint4& hi, uint4& lo) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+        __half2 a, b;
+        split_half(v[2 * m], a.x, b.x);
+        split_half(v[2 * m + 1], a.y, b.y);
+        h[m] = *reinterpret_cast<const uint32_t*>(&a);
+        l[m] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+    lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+template <bool SPLIT>
+__device__ __forceinline__ void slab_write16(uint8_t* hi, int lo, int row, int col, int rows, const float* v) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        uint8_t* p = hi + slab_offset(row, col + 8 * k, rows);
+        uint4 h, l;
+        pack8(v + 8 * k, h, l);
+        *reinterpret_cast<uint4*>(p) = h;
+        if (SPLIT) *reinterpret_cast<uint4*>(p + lo) = l;
+    }
+}
+
+// D += A B over 16 K elements of operands held as hi (+ lo at byte distance `a_lo`, `b_lo`)
+template <bool SPLIT>
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t a_lo, uint64_t b, uint64_t b_lo, uint32_t idesc,
+                                         bool accumulate) {
+    mma_f16(d, a, b, idesc, accumulate);
+    if (SPLIT) {
+        mma_f16(d, a, b + b_lo, idesc, 1);
+        mma_f16(d, a + a_lo, b, idesc, 1);
+    }
+}
+
+template <bool SPLIT, int N>
+__global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_constant__ SlabJobs<N> q) {
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ double red[kSlabThreads / 32], norm;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int index = 0;
+    while (index < q.count && (int)blockIdx.x >= q.job[index].first + q.job[index].ranks) index++;
+    if (index == q.count || (int)blockIdx.x < q.job[index].first) {
+        // a cluster's CTA without a matrix takes part in its barriers
+        for (int i = 0; i < 2 + 2 * q.steps; i++) slab_cluster_sync();
+        return;
+    }
+    const SlabJob& j = q.job[index];
+    const int ranks = j.ranks, rank = blockIdx.x - j.first;
+    uint32_t peer0;                  // the matrix's first CTA within the cluster
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(peer0));
+    peer0 -= rank;
+    const int rows = j.rows, col0 = rank * j.width;
+    const int cols = min(j.width, max(0, j.c - col0));            // this CTA's columns, and as whole tiles
+    const int tiles = (cols + 63) / 64;
+    const int x_lo = slab_x_bytes(rows, j.width), a_lo = slab_a_bytes(rows);
+    uint8_t* x = smem;
+    uint8_t* a = smem + x_lo * (SPLIT ? 2 : 1);
+    float* part = reinterpret_cast<float*>(a + a_lo * (SPLIT ? 2 : 1));
+    const int pp = rows + 4;                                       // pitch of `part`
+
+    if (tid == 0) {
+        mbar_init(&bar, 1);
+        fence_barrier_init();
+    }
+    if (warp == 0) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+
+    // momentum and |U|^2: units of four values along U's contiguous axis (X's columns, or its rows when tall)
+    const int across = j.tall ? cols : rows, along = j.tall ? rows : tiles * 64;
+    const int live_across = j.tall ? cols : j.r, live_along = j.tall ? j.r : cols;
+    const int per = along / 4, units = across * per;
+    double s = 0.0;
+    for (int base = tid; base < units; base += 4 * kSlabThreads) {
+        float4 g[4], m[4];
+        long at[4];
+        int n[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int u = base + i * kSlabThreads, line = u / per, k = (u - line * per) * 4;
+            n[i] = u < units && line < live_across ? live_along - k : 0;
+            at[i] = (j.tall ? col0 + line : (long)line) * j.in_pitch + (j.tall ? k : col0 + k);
+            g[i] = load_u4(j.in, j.in_type, at[i], n[i], j.vec);
+            if (j.weight) m[i] = load_u4(j.momentum, kTypeF32, at[i], n[i], j.vec);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float v[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+            if (j.weight) {
+                float w[4] = {m[i].x, m[i].y, m[i].z, m[i].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    w[k] = q.momentum * w[k] + q.grad_scale * v[k];
+                    v[k] = q.nesterov ? q.grad_scale * v[k] + q.momentum * w[k] : w[k];
+                }
+                if (j.vec && n[i] >= 4) {
+                    *reinterpret_cast<float4*>(j.momentum + at[i]) = make_float4(w[0], w[1], w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (k < n[i]) j.momentum[at[i] + k] = w[k];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) s += (double)v[k] * v[k];
+        }
+    }
+    s = warp_sum_d(s);
+    if (lane == 0) red[warp] = s;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    if (tid == 0) {
+        double t = 0.0;
+        for (int w = 0; w < kSlabThreads / 32; w++) t += red[w];
+        norm = t;
+    }
+    slab_cluster_sync();
+    s = 0.0;
+    for (int i = 0; i < ranks; i++) s += peer_load_d(peer_addr(smem_u32(&norm), peer0 + i));
+    // a norm of zero gives zeros; one that is not finite gives NaN everywhere
+    const double scale = s == 0.0 ? 0.0 : s <= 1.7e308 ? exp2((double)j.p) / sqrt(s) : nan("");
+
+    // X0 = U / |U| times 2^p; zero outside the matrix
+    for (int base = tid; base < units; base += 4 * kSlabThreads) {
+        float4 g[4], m[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int u = base + i * kSlabThreads, line = u / per, k = (u - line * per) * 4;
+            const int n = u < units && line < live_across ? live_along - k : 0;
+            const long at = (j.tall ? col0 + line : (long)line) * j.in_pitch + (j.tall ? k : col0 + k);
+            g[i] = load_u4(j.in, j.in_type, at, n, j.vec);
+            if (j.weight) m[i] = load_u4(j.momentum, kTypeF32, at, n, j.vec);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int u = base + i * kSlabThreads, line = u / per, k0 = (u - line * per) * 4;
+            if (u >= units) continue;
+            const float v[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+            const float w[4] = {m[i].x, m[i].y, m[i].z, m[i].w};
+            __half hi[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float d = !j.weight ? v[k] : q.nesterov ? q.grad_scale * v[k] + q.momentum * w[k] : w[k];
+                const bool inside = line < live_across && k0 + k < live_along;
+                split_half(inside ? (float)(scale * (double)d) : 0.0f, hi[k], lo[k]);
+            }
+            if (j.tall) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    *reinterpret_cast<__half*>(x + slab_offset(k0 + k, line, rows)) = hi[k];
+                    if (SPLIT) *reinterpret_cast<__half*>(x + x_lo + slab_offset(k0 + k, line, rows)) = lo[k];
+                }
+            } else {
+                uint8_t* p = x + slab_offset(line, k0, rows);
+                *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(hi);
+                if (SPLIT) *reinterpret_cast<uint2*>(p + x_lo) = *reinterpret_cast<const uint2*>(lo);
+            }
+        }
+    }
+    if (j.tall)   // columns past the matrix in the last tile
+        for (int i = tid; i < (tiles * 64 - cols) * rows; i += kSlabThreads) {
+            const int off = slab_offset(i % rows, cols + i / rows, rows);
+            *reinterpret_cast<__half*>(x + off) = __half(0.0f);
+            if (SPLIT) *reinterpret_cast<__half*>(x + x_lo + off) = __half(0.0f);
+        }
+    fence_proxy_async();
+    __syncthreads();
+
+    const uint32_t xs = smem_u32(x), as = smem_u32(a), ps = smem_u32(part);
+    const uint64_t dx = smem_desc(xs, 0, 1024, kLayoutSw128), da = smem_desc(as, 0, 1024, kLayoutSw128);
+    const uint64_t dx_mn = smem_desc(xs, rows * 128, 1024, kLayoutSw128);
+    const uint64_t tile = rows * 128 / 16, dx_lo = x_lo / 16, da_lo = a_lo / 16;   // descriptor units
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;      // accumulator row; warps share its columns
+    const uint32_t trow = (uint32_t)((warp & 3) * 32) << 16;
+    const float gram_f = exp2f((float)(kGramExp - 2 * j.p)), back_f = exp2f((float)-kGramExp), out_f = exp2f((float)-j.p);
+    uint32_t phase = 0;
+    bool bad = false;
+    for (int step = 0; step < q.steps; step++) {
+        // X X^T over this CTA's columns
+        if (tid == 0) {
+            tc_fence_after();
+            for (int t = 0; t < tiles; t++)
+                for (int kk = 0; kk < 4; kk++) {
+                    const uint64_t d = dx + t * tile + 2 * kk;
+                    mma_pair<SPLIT>(tmem, d, dx_lo, d, dx_lo, idesc_f16(rows, 0), (t | kk) != 0);
+                }
+            mma_commit(&bar);
+        }
+        __syncwarp();
+        mbar_wait(&bar, phase, q.status, kStatusWait);
+        phase ^= 1;
+        tc_fence_after();
+        for (int c = half * 16; c < rows; c += 32) {
+            float v[16];
+            __syncwarp();
+            tmem_ld16(tmem + trow + c, v);
+            if (row < rows)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    *reinterpret_cast<float4*>(part + row * pp + c + 4 * k) =
+                        tiles ? make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3])
+                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        tc_fence_before();
+        slab_cluster_sync();
+        // A = the sum over the cluster: this CTA's share of the rows, handed to everyone
+        const int share = rows / ranks, chunks = rows / 8;
+        for (int u = tid; u < share * chunks; u += kSlabThreads) {
+            const int r = rank * share + u / chunks, c = u % chunks;
+            float v[8] = {};
+            for (int i = 0; i < ranks; i++) {
+                const uint32_t from = peer_addr(ps + (r * pp + c * 8) * 4, peer0 + i);
+                const float4 f = peer_load4(from), g = peer_load4(from + 16);
+                v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+                v[4] += g.x, v[5] += g.y, v[6] += g.z, v[7] += g.w;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] *= gram_f;
+            uint4 hi, lo;
+            pack8(v, hi, lo);
+            const uint32_t to = as + slab_offset(r, c * 8, rows);
+            for (int i = 0; i < ranks; i++) {
+                peer_store4(peer_addr(to, peer0 + i), hi);
+                if (SPLIT) peer_store4(peer_addr(to + a_lo, peer0 + i), lo);
+            }
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");
+        slab_cluster_sync();
+        // B = b A + c A^2, over A
+        if (tid == 0) {
+            asm volatile("fence.proxy.async;" ::: "memory");
+            tc_fence_after();
+            for (int kk = 0; kk < rows / 16; kk++) {
+                const uint64_t d = da + (kk >> 2) * tile + 2 * (kk & 3);
+                mma_pair<SPLIT>(tmem, d, da_lo, d, da_lo, idesc_f16(rows, 0), kk != 0);
+            }
+            mma_commit(&bar);
+        }
+        __syncwarp();
+        mbar_wait(&bar, phase, q.status, kStatusWait);
+        phase ^= 1;
+        tc_fence_after();
+        for (int c = half * 16; c < rows; c += 32) {
+            float v[16], old[16];
+            __syncwarp();
+            tmem_ld16(tmem + trow + c, v);
+            if (row < rows) {
+                slab_read16<SPLIT>(a, a_lo, row, c, rows, old);
+#pragma unroll
+                for (int k = 0; k < 16; k++) v[k] = kNsB * old[k] + kNsC * (v[k] * back_f);
+                slab_write16<SPLIT>(a, a_lo, row, c, rows, v);
+            }
+        }
+        fence_proxy_async();
+        tc_fence_before();
+        __syncthreads();
+        // X <- a X + B X
+        const bool last = step + 1 == q.steps;
+        for (int c0 = 0; c0 < tiles * 64; c0 += kSlabRound) {
+            const int n = min(kSlabRound, tiles * 64 - c0);
+            if (tid == 0) {
+                tc_fence_after();
+                for (int n0 = 0; n0 < n; n0 += 256) {
+                    const uint64_t b = dx_mn + (c0 + n0) / 64 * tile;
+                    for (int kk = 0; kk < rows / 16; kk++)
+                        mma_pair<SPLIT>(tmem + 128 + n0, da + (kk >> 2) * tile + 2 * (kk & 3), da_lo, b + kk * (2048 / 16),
+                                        dx_lo, idesc_f16(min(256, n - n0), 1), kk != 0);
+                }
+                mma_commit(&bar);
+            }
+            __syncwarp();
+            mbar_wait(&bar, phase, q.status, kStatusWait);
+            phase ^= 1;
+            tc_fence_after();
+            for (int c = half * 16; c < n; c += 32) {
+                float v[16], old[16];
+                __syncwarp();
+                tmem_ld16(tmem + 128 + trow + c, v);
+                if (row >= rows) continue;
+                slab_read16<SPLIT>(x, x_lo, row, c0 + c, rows, old);
+#pragma unroll
+                for (int k = 0; k < 16; k++) v[k] = kNsA * old[k] + v[k] * back_f;
+                if (!last) {
+                    slab_write16<SPLIT>(x, x_lo, row, c0 + c, rows, v);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; k++) v[k] *= out_f;
+                    finish<16>(q, j, row, col0 + c0 + c, v, bad);
+                }
+            }
+            fence_proxy_async();
+            tc_fence_before();
+            __syncthreads();
+        }
+    }
+    if (bad && q.status) atomicExch(q.status, kStatusNonFinite);
+    slab_cluster_sync();   // no CTA leaves while a peer may read its shared memory
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
 // ------------------------------------------------------------------ host side
 
 struct Shape {
@@ -437,8 +904,12 @@ constexpr long kNormBytes = (long)kMaxJobs * kMaxNormParts * sizeof(double);
 
 long round_up(long v, long to) { return (v + to - 1) / to * to; }
 
+int scale_exponent(const Shape& s) {
+    return std::min(15, (int)std::floor(0.5 * std::log2((double)s.r * s.c)));
+}
+
 void layout_job(Job& j, const Shape& s, bool split, uint8_t*& at, const double* norm, int index) {
-    j.r = s.r, j.c = s.c, j.rb = s.rb, j.cb = s.cb;
+    j.rb = s.rb, j.cb = s.cb;
     j.x_bytes = s.x_bytes, j.a_bytes = s.a_bytes;
     const int halves = split ? 2 : 1;
     j.x[0] = at;
@@ -446,7 +917,6 @@ void layout_job(Job& j, const Shape& s, bool split, uint8_t*& at, const double* 
     j.a = j.x[1] + halves * s.x_bytes;
     j.b = j.a + halves * s.a_bytes;
     at = j.b + halves * s.a_bytes;
-    j.p = std::min(15, (int)std::floor(0.5 * std::log2((double)s.r * s.c)));
     j.norm = norm + (long)index * kMaxNormParts;
 }
 
@@ -488,79 +958,166 @@ void run_jobs(Jobs& q, double* parts, cudaStream_t stream) {
     }
 }
 
+// CTAs a matrix takes on the cluster path (a power of two up to 8), 0 where it does not fit.  One per 64 columns,
+// which shortens every pass over X, but no more than 128 / matrices where they fit: 128 CTAs is what clusters of eight
+// with one CTA per SM can hold at a time (two in each of the GPU's eight groups of SMs).
+int slab_ranks(const Shape& s, bool split, size_t matrices) {
+    if (s.r > 128) return 0;
+    const int rows = (s.r + 15) / 16 * 16;
+    for (int ranks = 1; ranks <= 8; ranks *= 2) {
+        const int width = (s.c + 64 * ranks - 1) / (64 * ranks) * 64;
+        if (slab_smem(rows, width, split) > kMaxSmem - 1024) continue;
+        if (ranks == 8 || width == 64 || 2 * ranks * matrices > 128) return ranks;
+    }
+    return 0;
+}
+
+template <bool SPLIT, int N>
+void launch_slabs(const Settings& set, const std::vector<SlabJob>& list, cudaStream_t stream) {
+    SlabJobs<N> q{};
+    static_cast<Settings&>(q) = set;
+    // Jobs come in falling order of their ranks, all powers of two, so none straddles a cluster.
+    const int size = list[0].ranks;
+    // One CTA per SM: a second one would wait for the TMEM of the first, which may be waiting for it in a cluster barrier.
+    int smem = kMaxSmem / 2 + 1024, ctas = 0;
+    for (const SlabJob& s : list) {
+        SlabJob& j = q.job[q.count++] = s;
+        j.first = ctas;
+        ctas += j.ranks;
+        smem = std::max(smem, slab_smem(j.rows, j.width, SPLIT));
+    }
+    static PerDeviceOnce once;
+    once_per_device(once, [] { set_max_dynamic_smem(slab_kernel<SPLIT, N>, kMaxSmem - 1024, "slab_kernel"); });
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((ctas + size - 1) / size * size);
+    cfg.blockDim = dim3(kSlabThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, slab_kernel<SPLIT, N>, q);
+    launch_check("slab_kernel");
+}
+
+template <bool SPLIT>
+void run_sources(const Settings& set, const std::vector<Source>& list, void* workspace, cudaStream_t stream) {
+    std::vector<SlabJob> slabs;
+    std::vector<Source> tiled;
+    for (const Source& s : list) {
+        SlabJob j{};
+        static_cast<Source&>(j) = s;
+        j.ranks = slab_ranks(Shape(s.r, s.c), SPLIT, list.size());
+        if (!j.ranks) {
+            tiled.push_back(s);
+            continue;
+        }
+        j.rows = (s.r + 15) / 16 * 16;
+        j.width = (s.c + 64 * j.ranks - 1) / (64 * j.ranks) * 64;
+        slabs.push_back(j);
+    }
+    std::stable_sort(slabs.begin(), slabs.end(), [](const SlabJob& a, const SlabJob& b) {
+        return a.ranks != b.ranks ? a.ranks > b.ranks : (long)a.rows * a.width > (long)b.rows * b.width;
+    });
+    for (size_t first = 0; first < slabs.size(); first += kMaxJobs) {
+        const std::vector<SlabJob> part(slabs.begin() + first,
+                                        slabs.begin() + std::min<size_t>(slabs.size(), first + kMaxJobs));
+        if (part.size() == 1)
+            launch_slabs<SPLIT, 1>(set, part, stream);
+        else
+            launch_slabs<SPLIT, kMaxJobs>(set, part, stream);
+    }
+    double* parts = reinterpret_cast<double*>(round_up(reinterpret_cast<intptr_t>(workspace), 1024));
+    Jobs q{};
+    static_cast<Settings&>(q) = set;
+    uint8_t* at = nullptr;
+    for (size_t i = 0; i < tiled.size(); i++) {
+        if (q.count == 0) at = reinterpret_cast<uint8_t*>(parts) + kNormBytes;
+        Job& j = q.job[q.count];
+        j = Job{};
+        static_cast<Source&>(j) = tiled[i];
+        layout_job(j, Shape(j.r, j.c), SPLIT, at, parts, q.count);
+        if (++q.count == kMaxJobs || i + 1 == tiled.size()) {
+            run_jobs<SPLIT>(q, parts, stream);
+            q.count = 0;
+        }
+    }
+}
+
+// Bytes of the tiled path for these shapes; its chunks of kMaxJobs matrices run one after another in the same
+// memory.  A call whose matrices all take the cluster path needs none, but the size may not depend on which
+// matrices of a list are active, so every matrix counts.
+size_t tiled_bytes(const std::vector<Shape>& shapes, bool split) {
+    long sum = 0;
+    for (const Shape& s : shapes) sum += s.bytes(split);
+    return (size_t)(kNormBytes + sum + 1024);
+}
+
+bool aligned16(const void* p, long pitch_bytes, int bytes) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && pitch_bytes % bytes == 0;
+}
+
 }  // namespace
 
 size_t muon_workspace_bytes(const MuonMatrix* m, int count, bool split) {
-    // chunks of kMaxJobs matrices run one after another in the same memory
-    long most = 0, sum = 0;
-    int n = 0;
-    for (int i = 0; i < count; i++) {
-        if (m[i].rows == 0 || m[i].cols == 0) continue;
-        sum += Shape(m[i].rows, m[i].cols).bytes(split);
-        most = std::max(most, sum);
-        if (++n == kMaxJobs) n = 0, sum = 0;
-    }
-    return (size_t)(kNormBytes + most + 1024);
+    std::vector<Shape> shapes;
+    for (int i = 0; i < count; i++)
+        if (m[i].rows && m[i].cols) shapes.emplace_back(m[i].rows, m[i].cols);
+    return tiled_bytes(shapes, split);
 }
 
 void muon_update(const MuonMatrix* m, int count, const MuonRule& rule, void* workspace, int* status,
                  cudaStream_t stream) {
-    double* parts = reinterpret_cast<double*>(round_up(reinterpret_cast<intptr_t>(workspace), 1024));
-    Jobs q{};
-    q.steps = rule.steps;
-    q.nesterov = rule.nesterov;
-    q.lr = rule.lr, q.momentum = rule.momentum, q.decay = rule.decay, q.grad_scale = rule.grad_scale;
-    q.status = status;
-    uint8_t* at = nullptr;
-    auto flush = [&] {
-        if (!q.count) return;
-        if (rule.split)
-            run_jobs<true>(q, parts, stream);
-        else
-            run_jobs<false>(q, parts, stream);
-        q.count = 0;
-    };
+    const Settings set{rule.steps, rule.nesterov, rule.lr, rule.momentum, rule.decay, rule.grad_scale, status};
+    std::vector<Source> list;
     for (int i = 0; i < count; i++) {
         if (m[i].rows == 0 || m[i].cols == 0) continue;
-        if (q.count == 0) at = reinterpret_cast<uint8_t*>(parts) + kNormBytes;
-        Job& j = q.job[q.count];
-        j = Job{};
-        layout_job(j, Shape(m[i].rows, m[i].cols), rule.split, at, parts, q.count);
-        j.tall = m[i].rows > m[i].cols;
-        j.in = m[i].grad;
-        j.weight = m[i].weight;
-        j.momentum = m[i].momentum;
-        j.in_pitch = j.out_pitch = m[i].cols;
-        j.rate = (float)((double)rule.lr * rule.rms * std::sqrt((double)std::max(m[i].rows, m[i].cols)));
-        if (++q.count == kMaxJobs) flush();
+        const Shape shape(m[i].rows, m[i].cols);
+        Source s{};
+        s.in = m[i].grad, s.weight = m[i].weight, s.momentum = m[i].momentum;
+        s.in_pitch = s.out_pitch = m[i].cols;
+        s.r = shape.r, s.c = shape.c;
+        s.tall = m[i].rows > m[i].cols;
+        s.p = scale_exponent(shape);
+        s.rate = (float)((double)rule.lr * rule.rms * std::sqrt((double)shape.c));
+        s.vec = aligned16(s.in, s.in_pitch * 4, 16) && aligned16(s.momentum, s.in_pitch * 4, 16) &&
+                aligned16(s.weight, s.in_pitch * 4, 16);
+        list.push_back(s);
     }
-    flush();
+    if (rule.split)
+        run_sources<true>(set, list, workspace, stream);
+    else
+        run_sources<false>(set, list, workspace, stream);
 }
 
 size_t orthogonalize_workspace_bytes(int rows, int cols, int out_type) {
     if (rows == 0 || cols == 0) return 0;
-    return (size_t)(kNormBytes + Shape(rows, cols).bytes(out_type == kTypeF32) + 1024);
+    return tiled_bytes({Shape(rows, cols)}, out_type == kTypeF32);
 }
 
 void orthogonalize(const void* in, int in_type, long in_pitch, int rows, int cols, int steps, void* out, int out_type,
                    long out_pitch, void* workspace, int* status, cudaStream_t stream) {
     if (rows == 0 || cols == 0) return;
-    const bool split = out_type == kTypeF32;
-    double* parts = reinterpret_cast<double*>(round_up(reinterpret_cast<intptr_t>(workspace), 1024));
-    uint8_t* at = reinterpret_cast<uint8_t*>(parts) + kNormBytes;
-    Jobs q{};
-    q.count = 1;
-    q.steps = steps;
-    q.status = status;
-    Job& j = q.job[0];
-    layout_job(j, Shape(rows, cols), split, at, parts, 0);
-    j.tall = rows > cols;
-    j.in = in, j.in_type = in_type, j.in_pitch = in_pitch;
-    j.out = out, j.out_type = out_type, j.out_pitch = out_pitch;
-    if (split)
-        run_jobs<true>(q, parts, stream);
+    Settings set{};
+    set.steps = steps;
+    set.status = status;
+    const Shape shape(rows, cols);
+    Source s{};
+    s.in = in, s.in_type = in_type, s.in_pitch = in_pitch;
+    s.out = out, s.out_type = out_type, s.out_pitch = out_pitch;
+    s.r = shape.r, s.c = shape.c;
+    s.tall = rows > cols;
+    s.p = scale_exponent(shape);
+    const int bytes = in_type == kTypeF32 ? 4 : 2;
+    s.vec = aligned16(in, in_pitch * bytes, 4 * bytes);
+    if (out_type == kTypeF32)
+        run_sources<true>(set, {s}, workspace, stream);
     else
-        run_jobs<false>(q, parts, stream);
+        run_sources<false>(set, {s}, workspace, stream);
 }
 
 }  // namespace sy
