@@ -12,10 +12,10 @@
 // entries near 1, A and B times 2^14; all factors are powers of two.  Where the caller wants FP32 accuracy every
 // operand is a pair hi + lo of fp16 values (22 bits) and each product is hi hi + hi lo + lo hi.
 //
-// Operands live in the workspace as 128 x 64 tiles of 16 KB in the swizzled form the tensor core reads
-// (128-byte rows, 16-byte chunks XOR-ed with row % 8), so a stage of the pipeline is one contiguous bulk copy
-// per tile, and the same X tile serves as a K-major operand of X X^T and as an MN-major operand of B X.
-// All matrices of a call share the launches: one per product, tiles of all matrices in one persistent grid.
+// Operands are kept as tiles of 64 columns in the swizzled form the tensor core reads (128-byte rows, 16-byte chunks
+// XOR-ed with row % 8), so that the same X tile serves as a K-major operand of X X^T and as an MN-major operand of
+// B X.  Matrices of at most 128 rows (of X) run on chip, one cluster each; larger ones run as tiles of all
+// matrices of the call in one persistent cooperative kernel.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -36,8 +36,6 @@ constexpr int kTile = 128, kChunk = 64;             // output tile; columns of a
 constexpr int kTileBytes = kTile * kChunk * 2;      // 16 KB
 constexpr int kGramExp = 14;                        // A and B are held times 2^14
 constexpr int kMaxJobs = 32;                        // matrices per launch (kernel parameters hold the table)
-constexpr int kMaxNormParts = 512;
-constexpr int kThreads = 256;
 
 // One matrix as the caller has it.
 struct Source {
@@ -59,56 +57,6 @@ struct Settings {
     int* status;
 };
 
-struct Job : Source {
-    uint8_t *x[2], *a, *b;      // hi tiles; the lo tiles follow at x_bytes / a_bytes
-    long x_bytes, a_bytes;
-    const double* norm;         // partial sums of squares of U
-    int rb, cb;                 // 128-row blocks of X; 64-column blocks (padded to a whole tile)
-    int tri0, full0;            // first tile of this job in the symmetric and in the full products
-};
-
-struct Jobs : Settings {
-    int count, tri_tiles, full_tiles, norm_parts;
-    Job job[kMaxJobs];
-};
-static_assert(sizeof(Jobs) <= 32000, "job table exceeds the kernel parameters");
-
-// element (row, col) of U: the orthogonalisation's input or Muon's direction
-__device__ __forceinline__ float direction(const Settings& q, const Source& j, long row, long col) {
-    const long at = row * j.in_pitch + col;
-    if (j.weight) {
-        const float m = j.momentum[at];
-        return q.nesterov ? q.grad_scale * static_cast<const float*>(j.in)[at] + q.momentum * m : m;
-    }
-    if (j.in_type == kTypeF32) return static_cast<const float*>(j.in)[at];
-    if (j.in_type == kTypeBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(j.in)[at]);
-    return __half2float(static_cast<const __half*>(j.in)[at]);
-}
-
-// Momentum update and the partial sums of squares of U (double: neither overflow nor lost terms for any scale
-// of the gradient; block sums in a fixed order).
-__global__ void __launch_bounds__(256) norm_kernel(const __grid_constant__ Jobs q, double* parts) {
-    const Job& j = q.job[blockIdx.y];
-    const long rows = j.tall ? j.c : j.r, cols = j.tall ? j.r : j.c;
-    double s = 0.0;
-    for (long i = blockIdx.x * 256L + threadIdx.x; i < rows * cols; i += gridDim.x * 256L) {
-        const long row = i / cols, col = i - row * cols;
-        if (j.weight)
-            j.momentum[i] = q.momentum * j.momentum[i] + q.grad_scale * static_cast<const float*>(j.in)[i];
-        const double u = direction(q, j, row, col);
-        s += u * u;
-    }
-    s = warp_sum_d(s);
-    __shared__ double red[8];
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int w = 0; w < 8; w++) t += red[w];
-        parts[blockIdx.y * kMaxNormParts + blockIdx.x] = t;
-    }
-}
-
 // byte offset of element (row, col) in a matrix of 128 x 64 tiles, `cb` tiles per row of tiles
 __device__ __forceinline__ long tile_offset(int row, int col, int cb) {
     return ((long)(row >> 7) * cb + (col >> 6)) * kTileBytes + (row & 127) * 128 +
@@ -120,118 +68,93 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
     lo = __float2half_rn(v - __half2float(hi));
 }
 
-// X0 tiles: U / |U| times 2^p, zero outside the matrix.  A norm of zero gives zeros; one that is not finite gives
-// NaN everywhere.
-template <bool SPLIT>
-__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Jobs q) {
-    const Job& j = q.job[blockIdx.y];
-    __shared__ double s_scale;
-    if (threadIdx.x < 32) {
-        double s = 0.0;
-        for (int i = threadIdx.x; i < q.norm_parts; i += 32) s += j.norm[i];
-        s = warp_sum_d(s);
-        if (threadIdx.x == 0) s_scale = s == 0.0 ? 0.0 : s <= 1.7e308 ? exp2((double)j.p) / sqrt(s) : nan("");
-    }
-    __syncthreads();
-    const double scale = s_scale;
-    const long tiles = (long)j.rb * j.cb;
-    for (long t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const int row0 = (int)(t / j.cb) * 128, col0 = (int)(t % j.cb) * 64;
-        for (int e = threadIdx.x; e < kTile * kChunk; e += 256) {
-            // lanes run along U's contiguous axis
-            const int row = row0 + (j.tall ? e & 127 : e >> 6), col = col0 + (j.tall ? e >> 7 : e & 63);
-            float v = 0.0f;
-            if (row < j.r && col < j.c)
-                v = (float)(scale * (double)(j.tall ? direction(q, j, col, row) : direction(q, j, row, col)));
-            __half hi, lo;
-            split_half(v, hi, lo);
-            const long at = tile_offset(row, col, j.cb);
-            *reinterpret_cast<__half*>(j.x[0] + at) = hi;
-            if (SPLIT) *reinterpret_cast<__half*>(j.x[0] + j.x_bytes + at) = lo;
+// Up to four consecutive values (the first n; the rest are zero).  Read past L1: Muon's momentum may just have been
+// written by another SM.
+__device__ __forceinline__ float4 load_u4(const void* in, int type, long at, int n, bool vec) {
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (n <= 0) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (type == kTypeF32) {
+        const float* p = static_cast<const float*>(in) + at;
+        if (vec && n >= 4) return __ldcg(reinterpret_cast<const float4*>(p));
+        for (int i = 0; i < 4; i++)
+            if (i < n) v[i] = __ldcg(p + i);
+    } else {
+        const uint16_t* p = static_cast<const uint16_t*>(in) + at;
+        uint16_t h[4] = {0, 0, 0, 0};
+        if (vec && n >= 4) {
+            const uint2 u = __ldcg(reinterpret_cast<const uint2*>(p));
+            h[0] = (uint16_t)u.x, h[1] = (uint16_t)(u.x >> 16), h[2] = (uint16_t)u.y, h[3] = (uint16_t)(u.y >> 16);
+        } else {
+            for (int i = 0; i < 4; i++)
+                if (i < n) h[i] = __ldcg(p + i);
         }
+        for (int i = 0; i < 4; i++)
+            v[i] = type == kTypeBF16 ? __uint_as_float((uint32_t)h[i] << 16) : __half2float(__ushort_as_half(h[i]));
     }
+    return make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// ------------------------------------------------------------------ products
-
-enum { kGram = 0, kSquare = 1, kApply = 2 };   // A = X X^T;  B = b A + c A A;  X <- a X + B X
-
-template <bool SPLIT>
-struct Stages {
-    static constexpr int kBytes = (SPLIT ? 4 : 2) * kTileBytes;
-    static constexpr int kCount = SPLIT ? 3 : 6;
-    static constexpr int kSmem = 1024 + kCount * kBytes + (2 * kCount + 4) * 8 + 16;
-};
-
-struct TileAt {
-    int job, i, j, kblocks;
-};
-
-// tile t of the launch: which matrix, which block of it
-template <int PHASE>
-__device__ __forceinline__ TileAt tile_at(const Jobs& q, int t) {
-    int n = q.count - 1;
-    while (n > 0 && t < (PHASE == kApply ? q.job[n].full0 : q.job[n].tri0)) n--;
-    const Job& j = q.job[n];
-    TileAt a;
-    a.job = n;
-    if (PHASE == kApply) {
-        const int u = t - j.full0;
-        a.j = u / j.rb;
-        a.i = u - a.j * j.rb;
-        a.kblocks = (j.r + 63) / 64;
-    } else {   // upper triangle by columns
-        const int u = t - j.tri0;
-        int c = (int)((sqrtf(8.0f * u + 1.0f) - 1.0f) * 0.5f);
-        while (c * (c + 1) / 2 > u) c--;
-        while ((c + 1) * (c + 2) / 2 <= u) c++;
-        a.j = c;
-        a.i = u - c * (c + 1) / 2;
-        a.kblocks = PHASE == kGram ? (j.c + 63) / 64 : (j.r + 63) / 64;
-    }
-    return a;
+// Muon's direction from the (scaled) gradient g and the new momentum m
+__device__ __forceinline__ float direction(const Settings& q, float g, float m) {
+    return q.nesterov ? q.grad_scale * g + q.momentum * m : m;
 }
 
-__device__ __forceinline__ void read32(const uint8_t* hi, const uint8_t* lo, int row, bool split, int chunk0, float* v) {
+// The momentum step of up to four values at `at`; v: the gradient, then the direction.
+__device__ __forceinline__ void update_momentum(const Settings& q, const Source& j, long at, int n, float* v,
+                                                const float4& old) {
+    float w[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const int off = ((chunk0 + k) ^ (row & 7)) << 4;
-        const uint4 h = *reinterpret_cast<const uint4*>(hi + off);
-        const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+        w[k] = q.momentum * w[k] + q.grad_scale * v[k];
+        v[k] = direction(q, v[k], w[k]);
+    }
+    if (j.vec && n >= 4) {
+        *reinterpret_cast<float4*>(j.momentum + at) = make_float4(w[0], w[1], w[2], w[3]);
+    } else {
 #pragma unroll
-        for (int l = 0; l < 4; l++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[l]));
-            v[8 * k + 2 * l] = f.x, v[8 * k + 2 * l + 1] = f.y;
-        }
-        if (split) {
-            const uint4 g = *reinterpret_cast<const uint4*>(lo + off);
-            const uint32_t x[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-            for (int l = 0; l < 4; l++) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[l]));
-                v[8 * k + 2 * l] += f.x, v[8 * k + 2 * l + 1] += f.y;
-            }
-        }
+        for (int k = 0; k < 4; k++)
+            if (k < n) j.momentum[at + k] = w[k];
     }
 }
 
-template <bool SPLIT>
-__device__ __forceinline__ void write32(uint8_t* hi, uint8_t* lo, int row, int chunk0, const float* v) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const int off = ((chunk0 + k) ^ (row & 7)) << 4;
-        uint32_t h[4], l[4];
-#pragma unroll
-        for (int m = 0; m < 4; m++) {
-            __half2 a, b;
-            split_half(v[8 * k + 2 * m], a.x, b.x);
-            split_half(v[8 * k + 2 * m + 1], a.y, b.y);
-            h[m] = *reinterpret_cast<const uint32_t*>(&a);
-            l[m] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        *reinterpret_cast<uint4*>(hi + off) = make_uint4(h[0], h[1], h[2], h[3]);
-        if (SPLIT) *reinterpret_cast<uint4*>(lo + off) = make_uint4(l[0], l[1], l[2], l[3]);
+// U after the momentum step: up to four values
+__device__ __forceinline__ float4 load_direction4(const Settings& q, const Source& j, long at, int n) {
+    float4 g = load_u4(j.in, j.in_type, at, n, j.vec);
+    if (j.weight) {
+        const float4 m = load_u4(j.momentum, kTypeF32, at, n, j.vec);
+        g.x = direction(q, g.x, m.x), g.y = direction(q, g.y, m.y);
+        g.z = direction(q, g.z, m.z), g.w = direction(q, g.w, m.w);
     }
+    return g;
+}
+
+// 2^p / |U| as two floats, applied one after the other (their product may leave the range of a float); 0 for |U| = 0
+// and NaN for a norm that is not finite.
+struct Scale {
+    float a, b;
+    __device__ __forceinline__ float operator()(float v) const { return v * a * b; }
+};
+__device__ __forceinline__ Scale scale_of(double sum_of_squares, int p) {
+    if (sum_of_squares == 0.0) return Scale{0.0f, 0.0f};
+    if (!(sum_of_squares <= 1.7e308)) return Scale{__int_as_float(0x7fffffff), 1.0f};
+    const double s = exp2((double)p) / sqrt(sum_of_squares);
+    int e;
+    frexp(s, &e);
+    return Scale{exp2f((float)(e / 2)), (float)(s * exp2((double)-(e / 2)))};
+}
+
+__device__ __forceinline__ void pack8(const float* v, uint4& hi, uint4& lo) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+        __half2 a, b;
+        split_half(v[2 * m], a.x, b.x);
+        split_half(v[2 * m + 1], a.y, b.y);
+        h[m] = *reinterpret_cast<const uint32_t*>(&a);
+        l[m] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+    lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
 // N consecutive values of a row of O (X's orientation) from `col` on: the output, or the weight update.  The old
@@ -282,181 +205,6 @@ __device__ __forceinline__ void finish(const Settings& q, const Source& j, int r
     }
 }
 
-// One product of every matrix of the call.  Persistent CTAs take 128 x 128 output tiles; one thread streams
-// operand tiles (64 along K) through a ring of stages, one thread issues the MMAs into one of two accumulators
-// in TMEM, four warps turn the other accumulator into the next operand.  The symmetric products compute the
-// upper triangle of tiles and write each tile twice.  `src` says which X buffer is current.
-template <int PHASE, bool SPLIT, bool LAST>
-__global__ void __launch_bounds__(kThreads, 1) ns_kernel(const __grid_constant__ Jobs q, const int src) {
-    using S = Stages<SPLIT>;
-    extern __shared__ uint8_t raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kCount * S::kBytes);
-    uint64_t *empty = full + S::kCount, *tfull = empty + S::kCount, *tempty = tfull + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tiles = PHASE == kApply ? q.full_tiles : q.tri_tiles;
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kCount; s++) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
-        }
-        for (int s = 0; s < 2; s++) {
-            mbar_init(&tfull[s], 1);
-            mbar_init(&tempty[s], 128);
-        }
-        fence_barrier_init();
-    }
-    if (warp == 3) {
-        tmem_alloc(tmem_slot, 256);
-        tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-
-    if (warp == 0) {
-        if (lane == 0) {
-            int n = 0;   // stages filled
-            bool ok = true;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-                const TileAt at = tile_at<PHASE>(q, t);
-                const Job& j = q.job[at.job];
-                const uint8_t* left = PHASE == kGram ? j.x[src] : PHASE == kSquare ? j.a : j.b;
-                const long left_lo = PHASE == kGram ? j.x_bytes : j.a_bytes;
-                const int lcb = PHASE == kGram ? j.cb : 2 * j.rb;
-                for (int k = 0; k < at.kblocks; k++, n++) {
-                    const int s = n % S::kCount;
-                    if (!(ok = mbar_wait(&empty[s], ((n / S::kCount) & 1) ^ 1, q.status, kStatusWait))) break;
-                    uint8_t* st = smem + s * S::kBytes;
-                    mbar_arrive_expect_tx(&full[s], S::kBytes);
-                    const uint8_t* a = left + ((long)at.i * lcb + k) * kTileBytes;
-                    bulk_load(st, a, kTileBytes, &full[s]);
-                    if (SPLIT) bulk_load(st + 2 * kTileBytes, a + left_lo, kTileBytes, &full[s]);
-                    if (PHASE == kApply) {
-                        // 64 rows of two neighbouring column blocks of X
-                        const uint8_t* b =
-                            j.x[src] + ((long)(k >> 1) * j.cb + 2 * at.j) * kTileBytes + (k & 1) * (kTileBytes / 2);
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            bulk_load(st + kTileBytes + h * (kTileBytes / 2), b + h * kTileBytes, kTileBytes / 2,
-                                      &full[s]);
-                            if (SPLIT)
-                                bulk_load(st + 3 * kTileBytes + h * (kTileBytes / 2), b + h * kTileBytes + j.x_bytes,
-                                          kTileBytes / 2, &full[s]);
-                        }
-                    } else {
-                        const uint8_t* b = left + ((long)at.j * lcb + k) * kTileBytes;
-                        bulk_load(st + kTileBytes, b, kTileBytes, &full[s]);
-                        if (SPLIT) bulk_load(st + 3 * kTileBytes, b + left_lo, kTileBytes, &full[s]);
-                    }
-                }
-            }
-            // no copy is in flight when the CTA ends, even after a wait that gave up
-            for (int i = max(0, n - S::kCount); i < n; i++)
-                mbar_wait(&full[i % S::kCount], (i / S::kCount) & 1, q.status, kStatusWait);
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = idesc_f16(kTile, PHASE == kApply);
-            int n = 0, done = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, done++) {
-                const TileAt at = tile_at<PHASE>(q, t);
-                const uint32_t d = tmem + (done & 1) * kTile;
-                if (!(ok = mbar_wait(&tempty[done & 1], ((done >> 1) & 1) ^ 1, q.status, kStatusWait))) break;
-                tc_fence_after();
-                for (int k = 0; k < at.kblocks; k++, n++) {
-                    const int s = n % S::kCount;
-                    if (!(ok = mbar_wait(&full[s], (n / S::kCount) & 1, q.status, kStatusWait))) break;
-                    tc_fence_after();
-                    const uint32_t st = smem_u32(smem + s * S::kBytes);
-                    const uint64_t ah = smem_desc(st, 0, 1024, kLayoutSw128);
-                    // MN-major: 64-column blocks 8 KB apart, groups of 8 K rows 1 KB apart, 16 K rows per MMA
-                    const uint64_t bh = smem_desc(st + kTileBytes, PHASE == kApply ? kTileBytes / 2 : 0, 1024, kLayoutSw128);
-                    constexpr int kStepB = PHASE == kApply ? 2048 / 16 : 2;
-                    constexpr uint64_t kLo = 2 * kTileBytes / 16;
-#pragma unroll
-                    for (int kk = 0; kk < kChunk / 16; kk++) {
-                        mma_f16(d, ah + 2 * kk, bh + kStepB * kk, idesc, (k | kk) != 0);
-                        if (SPLIT) {
-                            mma_f16(d, ah + 2 * kk, bh + kLo + kStepB * kk, idesc, 1);
-                            mma_f16(d, ah + kLo + 2 * kk, bh + kStepB * kk, idesc, 1);
-                        }
-                    }
-                    mma_commit(&empty[s]);
-                }
-                mma_commit(&tfull[done & 1]);
-            }
-        }
-    } else if (warp >= 4) {
-        const int w = warp & 3, r = w * 32 + lane;
-        int done = 0;
-        bool bad = false;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x, done++) {
-            const TileAt at = tile_at<PHASE>(q, t);
-            const Job& j = q.job[at.job];
-            if (!mbar_wait(&tfull[done & 1], (done >> 1) & 1, q.status, kStatusWait)) break;
-            tc_fence_after();
-            const uint32_t d = tmem + (done & 1) * kTile + ((uint32_t)(w * 32) << 16);
-            const int acb = 2 * j.rb;
-            // accumulator times: X X^T 2^2p -> A 2^14;  A A 2^28 -> 2^14;  B X 2^(14 + p) -> X 2^p
-            const float f = PHASE == kGram ? exp2f((float)(kGramExp - 2 * j.p))
-                                           : exp2f((float)-kGramExp) * (PHASE == kSquare ? kNsC : 1.0f);
-            const float out_f = exp2f((float)-j.p);
-#pragma unroll 1
-            for (int c = 0; c < kTile; c += 32) {
-                float v[32];
-                tmem_ld32(d + c, v);
-#pragma unroll
-                for (int k = 0; k < 32; k++) v[k] *= f;
-                const int cb = PHASE == kApply ? j.cb : acb;
-                const long off = ((long)at.i * cb + 2 * at.j + (c >> 6)) * kTileBytes + r * 128;
-                const int chunk = (c & 63) >> 3;
-                if (PHASE != kGram) {
-                    float x[32];
-                    const uint8_t* old = (PHASE == kSquare ? j.a : j.x[src]) + off;
-                    read32(old, old + (PHASE == kSquare ? j.a_bytes : j.x_bytes), r, SPLIT, chunk, x);
-#pragma unroll
-                    for (int k = 0; k < 32; k++) v[k] += (PHASE == kSquare ? kNsB : kNsA) * x[k];
-                }
-                if (LAST) {
-                    const int row = at.i * kTile + r, col = at.j * kTile + c;
-#pragma unroll
-                    for (int k = 0; k < 32; k++) v[k] *= out_f;
-                    finish<32>(q, j, row, col, v, bad);
-                    continue;
-                }
-                uint8_t* dst = PHASE == kGram ? j.a : PHASE == kSquare ? j.b : j.x[src ^ 1];
-                const long lo = PHASE == kApply ? j.x_bytes : j.a_bytes;
-                write32<SPLIT>(dst + off, dst + off + lo, r, chunk, v);
-                if (PHASE != kApply && at.i != at.j) {
-                    // the mirrored tile: lanes hold consecutive columns of its rows
-#pragma unroll
-                    for (int k = 0; k < 32; k++) {
-                        __half hi, l;
-                        split_half(v[k], hi, l);
-                        const long m = tile_offset(at.j * kTile + c + k, at.i * kTile + r, acb);
-                        *reinterpret_cast<__half*>(dst + m) = hi;
-                        if (SPLIT) *reinterpret_cast<__half*>(dst + m + lo) = l;
-                    }
-                }
-            }
-            tc_fence_before();
-            mbar_arrive(&tempty[done & 1]);
-        }
-        if (LAST && bad && q.status) atomicExch(q.status, kStatusNonFinite);
-    }
-    __syncwarp();
-    __syncthreads();
-    if (warp == 3) {
-        tc_fence_after();
-        tmem_dealloc(tmem, 256);
-    }
-}
-
 // ------------------------------------------------------------------ short matrices: one cluster each
 //
 // A matrix of at most 128 rows (of X) stays on chip for the whole call.  The CTAs of a cluster hold a slab of
@@ -467,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_kernel(const __grid_constant__
 // The MMA always takes 128 rows: those past `rows` read whatever follows the tile in shared memory and land in
 // accumulator rows that nothing reads.
 
-constexpr int kSlabThreads = 256;
+constexpr int kSlabThreads = 512;
 constexpr int kSlabRound = 384;      // columns of B X in TMEM at a time, beside 128 for the products of A
 constexpr int kMaxSmem = 227 * 1024;
 
@@ -517,31 +265,6 @@ __device__ __forceinline__ double peer_load_d(uint32_t addr) {
     return v;
 }
 
-// Four values of U from (row, col) on along its contiguous axis of `n` values; `raw` as stored (Muon: grad).
-__device__ __forceinline__ float4 load_u4(const void* in, int type, long at, int n, bool vec) {
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (n <= 0) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (type == kTypeF32) {
-        const float* p = static_cast<const float*>(in) + at;
-        if (vec && n >= 4) return *reinterpret_cast<const float4*>(p);
-        for (int i = 0; i < 4; i++)
-            if (i < n) v[i] = p[i];
-    } else {
-        const uint16_t* p = static_cast<const uint16_t*>(in) + at;
-        uint16_t h[4] = {0, 0, 0, 0};
-        if (vec && n >= 4) {
-            const uint2 u = *reinterpret_cast<const uint2*>(p);
-            h[0] = (uint16_t)u.x, h[1] = (uint16_t)(u.x >> 16), h[2] = (uint16_t)u.y, h[3] = (uint16_t)(u.y >> 16);
-        } else {
-            for (int i = 0; i < 4; i++)
-                if (i < n) h[i] = p[i];
-        }
-        for (int i = 0; i < 4; i++)
-            v[i] = type == kTypeBF16 ? __uint_as_float((uint32_t)h[i] << 16) : __half2float(__ushort_as_half(h[i]));
-    }
-    return make_float4(v[0], v[1], v[2], v[3]);
-}
-
 // byte offset of element (row, col) in slab tiles
 __device__ __forceinline__ int slab_offset(int row, int col, int rows) {
     return (col >> 6) * rows * 128 + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
@@ -570,20 +293,6 @@ __device__ __forceinline__ void slab_read16(const uint8_t* hi, int lo, int row, 
             }
         }
     }
-}
-
-__device__ __forceinline__ void pack8(const float* v, uint4& hi, uint4& lo) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int m = 0; m < 4; m++) {
-        __half2 a, b;
-        split_half(v[2 * m], a.x, b.x);
-        split_half(v[2 * m + 1], a.y, b.y);
-        h[m] = *reinterpret_cast<const uint32_t*>(&a);
-        l[m] = *reinterpret_cast<const uint32_t*>(&b);
-    }
-    hi = make_uint4(h[0], h[1], h[2], h[3]);
-    lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
 template <bool SPLIT>
@@ -651,6 +360,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
     const int across = j.tall ? cols : rows, along = j.tall ? rows : tiles * 64;
     const int live_across = j.tall ? cols : j.r, live_along = j.tall ? j.r : cols;
     const int per = along / 4, units = across * per;
+    const float per_inv = 1.0f / per;
     double s = 0.0;
     for (int base = tid; base < units; base += 4 * kSlabThreads) {
         float4 g[4], m[4];
@@ -658,7 +368,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         int n[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int u = base + i * kSlabThreads, line = u / per, k = (u - line * per) * 4;
+            const int u = base + i * kSlabThreads, line = fast_div(u, per_inv), k = (u - line * per) * 4;
             n[i] = u < units && line < live_across ? live_along - k : 0;
             at[i] = (j.tall ? col0 + line : (long)line) * j.in_pitch + (j.tall ? k : col0 + k);
             g[i] = load_u4(j.in, j.in_type, at[i], n[i], j.vec);
@@ -667,21 +377,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             float v[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
-            if (j.weight) {
-                float w[4] = {m[i].x, m[i].y, m[i].z, m[i].w};
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    w[k] = q.momentum * w[k] + q.grad_scale * v[k];
-                    v[k] = q.nesterov ? q.grad_scale * v[k] + q.momentum * w[k] : w[k];
-                }
-                if (j.vec && n[i] >= 4) {
-                    *reinterpret_cast<float4*>(j.momentum + at[i]) = make_float4(w[0], w[1], w[2], w[3]);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        if (k < n[i]) j.momentum[at[i] + k] = w[k];
-                }
-            }
+            if (j.weight) update_momentum(q, j, at[i], n[i], v, m[i]);
 #pragma unroll
             for (int k = 0; k < 4; k++) s += (double)v[k] * v[k];
         }
@@ -700,33 +396,26 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
     slab_cluster_sync();
     s = 0.0;
     for (int i = 0; i < ranks; i++) s += peer_load_d(peer_addr(smem_u32(&norm), peer0 + i));
-    // a norm of zero gives zeros; one that is not finite gives NaN everywhere
-    const double scale = s == 0.0 ? 0.0 : s <= 1.7e308 ? exp2((double)j.p) / sqrt(s) : nan("");
+    const Scale scale = scale_of(s, j.p);
 
     // X0 = U / |U| times 2^p; zero outside the matrix
     for (int base = tid; base < units; base += 4 * kSlabThreads) {
-        float4 g[4], m[4];
+        float4 d[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int u = base + i * kSlabThreads, line = u / per, k = (u - line * per) * 4;
+            const int u = base + i * kSlabThreads, line = fast_div(u, per_inv), k = (u - line * per) * 4;
             const int n = u < units && line < live_across ? live_along - k : 0;
-            const long at = (j.tall ? col0 + line : (long)line) * j.in_pitch + (j.tall ? k : col0 + k);
-            g[i] = load_u4(j.in, j.in_type, at, n, j.vec);
-            if (j.weight) m[i] = load_u4(j.momentum, kTypeF32, at, n, j.vec);
+            d[i] = load_direction4(
+                q, j, (j.tall ? col0 + line : (long)line) * j.in_pitch + (j.tall ? k : col0 + k), n);
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int u = base + i * kSlabThreads, line = u / per, k0 = (u - line * per) * 4;
+            const int u = base + i * kSlabThreads, line = fast_div(u, per_inv), k0 = (u - line * per) * 4;
             if (u >= units) continue;
-            const float v[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
-            const float w[4] = {m[i].x, m[i].y, m[i].z, m[i].w};
+            const float v[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
             __half hi[4], lo[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float d = !j.weight ? v[k] : q.nesterov ? q.grad_scale * v[k] + q.momentum * w[k] : w[k];
-                const bool inside = line < live_across && k0 + k < live_along;
-                split_half(inside ? (float)(scale * (double)d) : 0.0f, hi[k], lo[k]);
-            }
+            for (int k = 0; k < 4; k++) split_half(scale(v[k]), hi[k], lo[k]);
             if (j.tall) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -753,7 +442,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
     const uint64_t dx = smem_desc(xs, 0, 1024, kLayoutSw128), da = smem_desc(as, 0, 1024, kLayoutSw128);
     const uint64_t dx_mn = smem_desc(xs, rows * 128, 1024, kLayoutSw128);
     const uint64_t tile = rows * 128 / 16, dx_lo = x_lo / 16, da_lo = a_lo / 16;   // descriptor units
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;      // accumulator row; warps share its columns
+    const int row = (warp & 3) * 32 + lane, part_of = warp >> 2;   // accumulator row; warps share its columns
     const uint32_t trow = (uint32_t)((warp & 3) * 32) << 16;
     const float gram_f = exp2f((float)(kGramExp - 2 * j.p)), back_f = exp2f((float)-kGramExp), out_f = exp2f((float)-j.p);
     uint32_t phase = 0;
@@ -773,7 +462,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         mbar_wait(&bar, phase, q.status, kStatusWait);
         phase ^= 1;
         tc_fence_after();
-        for (int c = half * 16; c < rows; c += 32) {
+        for (int c = part_of * 16; c < rows; c += kSlabThreads / 8) {
             float v[16];
             __syncwarp();
             tmem_ld16(tmem + trow + c, v);
@@ -790,13 +479,20 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         const int share = rows / ranks, chunks = rows / 8;
         for (int u = tid; u < share * chunks; u += kSlabThreads) {
             const int r = rank * share + u / chunks, c = u % chunks;
+            float4 f[8], g[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < ranks) {
+                    const uint32_t from = peer_addr(ps + (r * pp + c * 8) * 4, peer0 + i);
+                    f[i] = peer_load4(from), g[i] = peer_load4(from + 16);
+                }
             float v[8] = {};
-            for (int i = 0; i < ranks; i++) {
-                const uint32_t from = peer_addr(ps + (r * pp + c * 8) * 4, peer0 + i);
-                const float4 f = peer_load4(from), g = peer_load4(from + 16);
-                v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
-                v[4] += g.x, v[5] += g.y, v[6] += g.z, v[7] += g.w;
-            }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < ranks) {
+                    v[0] += f[i].x, v[1] += f[i].y, v[2] += f[i].z, v[3] += f[i].w;
+                    v[4] += g[i].x, v[5] += g[i].y, v[6] += g[i].z, v[7] += g[i].w;
+                }
 #pragma unroll
             for (int k = 0; k < 8; k++) v[k] *= gram_f;
             uint4 hi, lo;
@@ -823,7 +519,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         mbar_wait(&bar, phase, q.status, kStatusWait);
         phase ^= 1;
         tc_fence_after();
-        for (int c = half * 16; c < rows; c += 32) {
+        for (int c = part_of * 16; c < rows; c += kSlabThreads / 8) {
             float v[16], old[16];
             __syncwarp();
             tmem_ld16(tmem + trow + c, v);
@@ -855,7 +551,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
             mbar_wait(&bar, phase, q.status, kStatusWait);
             phase ^= 1;
             tc_fence_after();
-            for (int c = half * 16; c < n; c += 32) {
+            for (int c = part_of * 16; c < n; c += kSlabThreads / 8) {
                 float v[16], old[16];
                 __syncwarp();
                 tmem_ld16(tmem + 128 + trow + c, v);
@@ -884,6 +580,532 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
     }
 }
 
+// ------------------------------------------------------------------ larger matrices: tiles of a persistent kernel
+//
+// One cooperative launch per call.  Phases (norm, packing, and per iteration X X^T, A^2, B X) are separated by grid
+// barriers.  In a product phase persistent CTAs take 128 x BN output tiles: one thread streams operand tiles (64
+// along K, each one contiguous bulk copy) through a ring of stages, a warp waits for them, a warp issues the MMAs
+// into one of two accumulators in TMEM, eight warps turn the other accumulator into the next operand.  The
+// symmetric products compute the upper triangle of tiles and write each tile twice; where X X^T has fewer tiles than
+// the GPU has SMs its K is split instead, and another phase adds the parts.
+// The tensor core's FP32 accumulator truncates, a bias that grows with the number of MMAs added into it; pairs of
+// fp16 therefore accumulate 512 elements along K at a time and add those sums in registers.
+
+struct Job : Source {
+    uint8_t *x[2], *a, *b;      // hi tiles; the lo tiles follow at x_bytes / a_bytes
+    long x_bytes, a_bytes;
+    int rb, cb;                 // 128-row blocks of X; 64-column blocks (padded to an even number)
+    int splits;                 // parts of X X^T's K
+    // first unit of this matrix in: packing (128 x 64 tiles), X X^T, A^2, B X, the sum of the split X X^T (16-byte
+    // pieces) and the parts' memory (128 x 128 tiles)
+    int pack0, gram0, square0, apply0, sum0, part0;
+};
+template <int N>
+struct Jobs : Settings {
+    int count;
+    int packs, grams, squares, applies, sums;   // units of each phase
+    double* norms;                              // [count][gridDim]
+    float* parts;
+    uint32_t* barrier;
+    Job job[N];
+};
+static_assert(sizeof(Jobs<kMaxJobs>) <= 32000, "job table exceeds the kernel parameters");
+
+enum { kGram = 0, kSquare = 1, kApply = 2 };   // A = X X^T;  B = b A + c A A;  X <- a X + B X
+constexpr int kEpilogueWarps = 8;
+constexpr int kTiledThreads = 32 * (4 + kEpilogueWarps);
+constexpr int kTiledBar = 1;                   // a stage is loaded: the waiting warp and the MMA warp
+constexpr int kSegment = 8;                    // stages (of 64 along K) per accumulator of pairs
+
+template <bool SPLIT, int BN>
+struct Stages {
+    static constexpr int kBytesB = BN / 128 * kTileBytes;
+    static constexpr int kHalf = kTileBytes + kBytesB;            // hi operands, then lo operands
+    static constexpr int kBytes = (SPLIT ? 2 : 1) * kHalf;
+    static constexpr int kCount = 196608 / kBytes;
+    static constexpr int kSmem = 1024 + kCount * kBytes + (2 * kCount + 4) * 8 + 16;
+};
+
+struct TileAt {
+    int job, i, j, k0, k1, split;   // 128-row block, BN-column block, stages along K
+};
+
+// unit t of a product phase: which matrix, which tile of it, which part of K
+template <int BN, int N>
+__device__ __forceinline__ TileAt tile_at(const Jobs<N>& q, int phase, int t) {
+    int n = q.count - 1;
+    while (n > 0 && t < (phase == kGram ? q.job[n].gram0 : phase == kSquare ? q.job[n].square0 : q.job[n].apply0)) n--;
+    const Job& j = q.job[n];
+    TileAt a;
+    a.job = n;
+    a.split = 0;
+    a.k0 = 0;
+    a.k1 = phase == kGram ? (j.c + 63) / 64 : (j.r + 63) / 64;
+    int u = t - (phase == kGram ? j.gram0 : phase == kSquare ? j.square0 : j.apply0);
+    if (phase == kApply) {
+        a.j = u / j.rb;
+        a.i = u - a.j * j.rb;
+    } else if (phase == kGram && j.splits > 1) {   // every tile, in parts
+        const int all = a.k1;
+        a.split = u % j.splits;
+        u /= j.splits;
+        a.j = u / j.rb;
+        a.i = u - a.j * j.rb;
+        a.k0 = (int)((long)all * a.split / j.splits);
+        a.k1 = (int)((long)all * (a.split + 1) / j.splits);
+    } else {   // the tiles that reach above the diagonal, by columns
+        constexpr int kW = BN / 128;               // column j holds row blocks 0 .. kW (j + 1) - 1
+        int c = (int)((sqrtf(8.0f / kW * u + 1.0f) - 1.0f) * 0.5f);
+        while (kW * c * (c + 1) / 2 > u) c--;
+        while (kW * (c + 1) * (c + 2) / 2 <= u) c++;
+        a.j = c;
+        a.i = u - kW * c * (c + 1) / 2;
+    }
+    return a;
+}
+
+template <bool SPLIT>
+__device__ __forceinline__ void read32(const uint8_t* hi, long lo, int row, int chunk0, float* v) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint8_t* p = hi + (((chunk0 + k) ^ (row & 7)) << 4);
+        const uint4 h = __ldcg(reinterpret_cast<const uint4*>(p));
+        const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+        for (int l = 0; l < 4; l++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[l]));
+            v[8 * k + 2 * l] = f.x, v[8 * k + 2 * l + 1] = f.y;
+        }
+        if (SPLIT) {
+            const uint4 g = __ldcg(reinterpret_cast<const uint4*>(p + lo));
+            const uint32_t x[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+            for (int l = 0; l < 4; l++) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[l]));
+                v[8 * k + 2 * l] += f.x, v[8 * k + 2 * l + 1] += f.y;
+            }
+        }
+    }
+}
+
+// 32 columns of a row of a tile, and with `mirror` the same values as a column of the transposed tile there: lanes hold
+// consecutive rows, so after an exchange with its neighbour each lane stores two rows of every other column.
+template <bool SPLIT>
+__device__ __forceinline__ void write32(uint8_t* hi, long lo, int row, int chunk0, const float* v, uint8_t* mirror,
+                                        int mirror_row) {
+    uint32_t h[16], l[16];
+#pragma unroll
+    for (int m = 0; m < 16; m++) {
+        __half2 a, b;
+        split_half(v[2 * m], a.x, b.x);
+        split_half(v[2 * m + 1], a.y, b.y);
+        h[m] = *reinterpret_cast<const uint32_t*>(&a);
+        l[m] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        uint8_t* p = hi + (((chunk0 + k) ^ (row & 7)) << 4);
+        *reinterpret_cast<uint4*>(p) = make_uint4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
+        if (SPLIT) *reinterpret_cast<uint4*>(p + lo) = make_uint4(l[4 * k], l[4 * k + 1], l[4 * k + 2], l[4 * k + 3]);
+    }
+    if (!mirror) return;
+    const bool odd = row & 1;
+#pragma unroll
+    for (int m = 0; m < 16; m++) {
+        // word m holds columns 2 m (low half) and 2 m + 1 of this row
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, h[m], 1);
+        const uint32_t w = odd ? __byte_perm(other, h[m], 0x7632) : __byte_perm(h[m], other, 0x5410);
+        const int tr = mirror_row + 2 * m + odd, tc = (row & 63) & ~1;    // row and column in the transposed tile
+        uint8_t* p = mirror + tr * 128 + (((tc >> 3) ^ (tr & 7)) << 4) + (tc & 7) * 2;
+        *reinterpret_cast<uint32_t*>(p) = w;
+        if (SPLIT) {
+            const uint32_t other_lo = __shfl_xor_sync(0xffffffffu, l[m], 1);
+            *reinterpret_cast<uint32_t*>(p + lo) =
+                odd ? __byte_perm(other_lo, l[m], 0x7632) : __byte_perm(l[m], other_lo, 0x5410);
+        }
+    }
+}
+
+// Barrier number `turn` (from 1) of the whole grid: what every CTA wrote before it is visible to every CTA after it,
+// to plain loads and to bulk copies.  Gives up after a bounded number of polls, like every wait here.
+__device__ __forceinline__ bool grid_barrier(uint32_t* counter, uint32_t turn, int* status, int* s_ok) {
+    asm volatile("fence.proxy.async;" ::: "memory");
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int ok = *s_ok;
+        atomicAdd(counter, 1);
+        for (uint32_t polls = 0; ok; polls++) {
+            uint32_t seen;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
+            if (seen >= turn * gridDim.x) break;
+            if (polls > kSpinLimit) {
+                ok = 0;
+                if (status) atomicExch(status, kStatusWait);
+            }
+        }
+        *s_ok = ok;
+    }
+    __syncthreads();
+    __threadfence();
+    asm volatile("fence.proxy.async;" ::: "memory");
+    return *s_ok;
+}
+
+template <bool SPLIT, int BN, int N>
+__global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_constant__ Jobs<N> q) {
+    using S = Stages<SPLIT, BN>;
+    extern __shared__ uint8_t raw[];
+    __shared__ double red[kTiledThreads / 32], s_norm;
+    __shared__ int s_ok;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kCount * S::kBytes);
+    uint64_t *empty = full + S::kCount, *tfull = empty + S::kCount, *tempty = tfull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int s = 0; s < S::kCount; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(&tfull[s], 1);
+            mbar_init(&tempty[s], 32 * kEpilogueWarps);
+        }
+        fence_barrier_init();
+        s_ok = 1;
+    }
+    if (warp == 3) {
+        tmem_alloc(tmem_slot, 2 * BN);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    uint32_t turn = 0;
+
+    // momentum and the partial sums of squares of U (double: no scale of the gradient overflows or loses terms)
+    for (int n = 0; n < q.count; n++) {
+        const Job& j = q.job[n];
+        const int lines = j.tall ? j.c : j.r, length = j.tall ? j.r : j.c, per = (length + 3) / 4;
+        const long units = (long)lines * per;
+        double s = 0.0;
+        for (long base = (long)blockIdx.x * kTiledThreads + tid; base < units; base += 4L * gridDim.x * kTiledThreads) {
+            float4 g[4], m[4];
+            long at[4];
+            int left[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const long u = base + (long)i * gridDim.x * kTiledThreads, line = u / per;
+                const int k = (int)(u - line * per) * 4;
+                left[i] = u < units ? length - k : 0;
+                at[i] = line * j.in_pitch + k;
+                g[i] = load_u4(j.in, j.in_type, at[i], left[i], j.vec);
+                if (j.weight) m[i] = load_u4(j.momentum, kTypeF32, at[i], left[i], j.vec);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float v[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+                if (j.weight) update_momentum(q, j, at[i], left[i], v, m[i]);
+#pragma unroll
+                for (int k = 0; k < 4; k++) s += (double)v[k] * v[k];
+            }
+        }
+        s = warp_sum_d(s);
+        if (lane == 0) red[warp] = s;
+        __syncthreads();
+        if (tid == 0) {
+            double t = 0.0;
+            for (int w = 0; w < kTiledThreads / 32; w++) t += red[w];
+            q.norms[(long)n * gridDim.x + blockIdx.x] = t;
+        }
+        __syncthreads();
+    }
+    bool ok = grid_barrier(q.barrier, ++turn, q.status, &s_ok);
+
+    // X0 tiles: U / |U| times 2^p, zero outside the matrix
+    for (int t = blockIdx.x, at_job = -1; ok && t < q.packs; t += gridDim.x) {
+        int n = q.count - 1;
+        while (n > 0 && t < q.job[n].pack0) n--;
+        const Job& j = q.job[n];
+        if (n != at_job) {
+            __syncthreads();
+            if (warp == 0) {
+                double s = 0.0;
+                for (int i = lane; i < (int)gridDim.x; i += 32) s += __ldcg(q.norms + (long)n * gridDim.x + i);
+                s = warp_sum_d(s);
+                if (lane == 0) s_norm = s;
+            }
+            __syncthreads();
+            at_job = n;
+        }
+        const Scale scale = scale_of(s_norm, j.p);
+        const int block = (t - j.pack0) / j.cb, row0 = block * 128, col0 = (t - j.pack0 - block * j.cb) * 64;
+        uint8_t* dst = j.x[0] + (long)(t - j.pack0) * kTileBytes;
+        if (!j.tall) {
+            // eight columns of a row per unit
+            for (int u = tid; u < 128 * 8; u += kTiledThreads) {
+                const int row = u >> 3, col = (u & 7) * 8;
+                float v[8];
+                const int left = row0 + row < j.r ? j.c - col0 - col : 0;
+                const long at = (row0 + row) * j.in_pitch + col0 + col;
+                const float4 d[2] = {load_direction4(q, j, at, left), load_direction4(q, j, at + 4, left - 4)};
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    v[4 * k] = scale(d[k].x), v[4 * k + 1] = scale(d[k].y), v[4 * k + 2] = scale(d[k].z),
+                              v[4 * k + 3] = scale(d[k].w);
+                uint4 hi, lo;
+                pack8(v, hi, lo);
+                uint8_t* p = dst + row * 128 + (((u & 7) ^ (row & 7)) << 4);
+                *reinterpret_cast<uint4*>(p) = hi;
+                if (SPLIT) *reinterpret_cast<uint4*>(p + j.x_bytes) = lo;
+            }
+        } else {
+            // four rows of eight columns per unit: eight lines of U, lanes along them
+            for (int u = tid; u < 32 * 8; u += kTiledThreads) {
+                const int row = (u & 31) * 4, chunk = u >> 5;
+                float v[4][8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int line = col0 + chunk * 8 + k;
+                    const float4 d = load_direction4(q, j, line * j.in_pitch + row0 + row,
+                                                     line < j.c ? j.r - row0 - row : 0);
+                    v[0][k] = scale(d.x), v[1][k] = scale(d.y), v[2][k] = scale(d.z), v[3][k] = scale(d.w);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint4 hi, lo;
+                    pack8(v[i], hi, lo);
+                    uint8_t* p = dst + (row + i) * 128 + ((chunk ^ ((row + i) & 7)) << 4);
+                    *reinterpret_cast<uint4*>(p) = hi;
+                    if (SPLIT) *reinterpret_cast<uint4*>(p + j.x_bytes) = lo;
+                }
+            }
+        }
+    }
+    ok = ok && grid_barrier(q.barrier, ++turn, q.status, &s_ok);
+
+    int n = 0, accs = 0;          // stages and accumulators that this warp's role has passed
+    bool bad = false;
+    for (int step = 0; ok && step < 4 * q.steps; step++) {
+        const int phase = step & 3, src = (step >> 2) & 1;
+        if (phase == 1) {
+            // the parts of X X^T
+            if (!q.sums) continue;
+            for (long u = (long)blockIdx.x * kTiledThreads + tid; u < q.sums; u += (long)gridDim.x * kTiledThreads) {
+                int k = q.count - 1;
+                while (k > 0 && u < q.job[k].sum0) k--;
+                const Job& j = q.job[k];
+                const int e = (int)(u - j.sum0), tile = e >> 11, row = (e >> 4) & 127, col = (e & 15) * 8;
+                const float* from = q.parts + (long)(j.part0 + tile * j.splits) * (kTile * kTile) + row * kTile + col;
+                float v[8] = {};
+                for (int s = 0; s < j.splits; s++) {
+                    const float4 f = __ldcg(reinterpret_cast<const float4*>(from + (long)s * kTile * kTile));
+                    const float4 g = __ldcg(reinterpret_cast<const float4*>(from + (long)s * kTile * kTile + 4));
+                    v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+                    v[4] += g.x, v[5] += g.y, v[6] += g.z, v[7] += g.w;
+                }
+                const float f = exp2f((float)(kGramExp - 2 * j.p));
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] *= f;
+                uint4 hi, lo;
+                pack8(v, hi, lo);
+                const int bj = tile / j.rb, bi = tile - bj * j.rb;
+                uint8_t* p = j.a + tile_offset(bi * kTile + row, bj * kTile + col, 2 * j.rb);
+                *reinterpret_cast<uint4*>(p) = hi;
+                if (SPLIT) *reinterpret_cast<uint4*>(p + j.a_bytes) = lo;
+            }
+            ok = grid_barrier(q.barrier, ++turn, q.status, &s_ok);
+            continue;
+        }
+        const int product = phase == 0 ? kGram : phase == 2 ? kSquare : kApply;
+        const bool last = product == kApply && (step >> 2) + 1 == q.steps;
+        const int tiles = product == kGram ? q.grams : product == kSquare ? q.squares : q.applies;
+        if (warp == 0) {
+            if (lane == 0) {
+                const int first = n;
+                for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+                    const TileAt at = tile_at<BN>(q, product, t);
+                    const Job& j = q.job[at.job];
+                    const uint8_t* left = product == kGram ? j.x[src] : product == kSquare ? j.a : j.b;
+                    const long left_lo = product == kGram ? j.x_bytes : j.a_bytes;
+                    const int lcb = product == kGram ? j.cb : 2 * j.rb;
+                    // of the BN columns, those whose operand exists: 64-column blocks of X, 128-row blocks
+                    const int pieces = product == kApply ? min(BN / 64, j.cb - at.j * (BN / 64))
+                                                         : min(BN / 128, j.rb - at.j * (BN / 128));
+                    const int piece = product == kApply ? kTileBytes / 2 : kTileBytes;
+                    for (int k = at.k0; k < at.k1; k++, n++) {
+                        const int s = n % S::kCount;
+                        if (!(ok = mbar_wait(&empty[s], ((n / S::kCount) & 1) ^ 1, q.status, kStatusWait))) break;
+                        uint8_t* st = smem + s * S::kBytes;
+                        mbar_arrive_expect_tx(&full[s], (kTileBytes + pieces * piece) * (SPLIT ? 2 : 1));
+                        const uint8_t* a = left + ((long)at.i * lcb + k) * kTileBytes;
+                        bulk_load(st, a, kTileBytes, &full[s]);
+                        if (SPLIT) bulk_load(st + S::kHalf, a + left_lo, kTileBytes, &full[s]);
+                        for (int h = 0; h < pieces; h++) {
+                            // B X: 64 rows of neighbouring column blocks of X; otherwise neighbouring row blocks
+                            const uint8_t* b =
+                                product == kApply
+                                    ? j.x[src] + ((long)(k >> 1) * j.cb + at.j * (BN / 64) + h) * kTileBytes +
+                                          (k & 1) * (kTileBytes / 2)
+                                    : left + ((long)(at.j * (BN / 128) + h) * lcb + k) * kTileBytes;
+                            bulk_load(st + kTileBytes + h * piece, b, piece, &full[s]);
+                            if (SPLIT)
+                                bulk_load(st + S::kHalf + kTileBytes + h * piece,
+                                          b + (product == kApply ? j.x_bytes : left_lo), piece, &full[s]);
+                        }
+                    }
+                }
+                // no copy is in flight when the CTA ends, even after a wait that gave up
+                for (int i = max(first, n - S::kCount); i < n; i++)
+                    ok &= mbar_wait(&full[i % S::kCount], (i / S::kCount) & 1, q.status, kStatusWait);
+                if (!ok) s_ok = 0;
+            }
+        } else if (warp == 2) {
+            // every wait of the MMA side; after one that gave up the hand-offs go on, so that every warp finishes
+            for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+                const TileAt at = tile_at<BN>(q, product, t);
+                for (int k = at.k0; k < at.k1; k++, n++) {
+                    if (k == at.k0 || (SPLIT && (k - at.k0) % kSegment == 0)) {
+                        if (ok) ok = mbar_wait(&tempty[accs & 1], ((accs >> 1) & 1) ^ 1, q.status, kStatusWait);
+                        accs++;
+                    }
+                    if (ok) ok = mbar_wait(&full[n % S::kCount], (n / S::kCount) & 1, q.status, kStatusWait);
+                    named_bar_sync(kTiledBar, 64);
+                }
+            }
+            if (!ok) s_ok = 0;
+        } else if (warp == 1) {
+            const uint32_t idesc = idesc_f16(BN, product == kApply);
+            // MN-major: 64-column blocks 8 KB apart, groups of 8 K rows 1 KB apart, 16 K rows per MMA
+            const uint32_t lbo = product == kApply ? kTileBytes / 2 : 0;
+            const uint32_t step_b = product == kApply ? 2048 / 16 : 2;
+            const uint32_t smem0 = smem_u32(smem);
+            for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+                const TileAt at = tile_at<BN>(q, product, t);
+                for (int k = at.k0; k < at.k1; k++, n++) {
+                    const int s = n % S::kCount, in_segment = SPLIT ? (k - at.k0) % kSegment : k - at.k0;
+                    const uint32_t d = tmem + (accs & 1) * BN;
+                    named_bar_sync(kTiledBar, 64);
+                    tc_fence_after();
+                    const uint64_t ah = smem_desc(smem0 + s * S::kBytes, 0, 1024, kLayoutSw128);
+                    const uint64_t bh = smem_desc(smem0 + s * S::kBytes + kTileBytes, lbo, 1024, kLayoutSw128);
+                    constexpr uint64_t kLo = S::kHalf / 16;
+#pragma unroll
+                    for (int kk = 0; kk < kChunk / 16; kk++) {
+                        mma_f16_elect(d, ah + 2 * kk, bh + step_b * kk, idesc, (in_segment | kk) != 0);
+                        if (SPLIT) {
+                            mma_f16_elect(d, ah + 2 * kk, bh + kLo + step_b * kk, idesc, 1);
+                            mma_f16_elect(d, ah + kLo + 2 * kk, bh + step_b * kk, idesc, 1);
+                        }
+                    }
+                    mma_commit_elect(&empty[s]);
+                    if (k + 1 == at.k1 || (SPLIT && in_segment + 1 == kSegment)) {
+                        mma_commit_elect(&tfull[accs & 1]);
+                        accs++;
+                    }
+                }
+            }
+        } else if (warp >= 4) {
+            const int r = (warp & 3) * 32 + lane;
+            constexpr int kCols = BN / 2;          // of this warp: four warps share the rows, two the columns
+            const int c_first = ((warp - 4) >> 2) * kCols;
+            for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+                const TileAt at = tile_at<BN>(q, product, t);
+                const Job& j = q.job[at.job];
+                // accumulator times: X X^T 2^2p -> A 2^14;  A A 2^28 -> 2^14;  B X 2^(14 + p) -> X 2^p
+                const float f = product == kGram ? exp2f((float)(kGramExp - 2 * j.p))
+                                                 : exp2f((float)-kGramExp) * (product == kSquare ? kNsC : 1.0f);
+                const float out_f = exp2f((float)-j.p);
+                // 32 columns from c on of this thread's row
+                auto emit = [&](int c, float* v) {
+                    if (product == kGram && j.splits > 1) {
+                        float4* part = reinterpret_cast<float4*>(
+                            q.parts + (long)(j.part0 + (at.j * j.rb + at.i) * j.splits + at.split) * (kTile * kTile) +
+                            r * kTile + c);
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            __stcg(part + k, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
+                        return;
+                    }
+                    const int bj = at.j * (BN / 128) + (c >> 7);      // 128-column block
+                    if (product == kApply ? 2 * bj >= j.cb : bj < at.i || bj >= j.rb) return;
+#pragma unroll
+                    for (int k = 0; k < 32; k++) v[k] *= f;
+                    const int cb = product == kApply ? j.cb : 2 * j.rb;
+                    const int cc = c & 127, chunk = (cc & 63) >> 3;
+                    const long off = ((long)at.i * cb + 2 * bj + (cc >> 6)) * kTileBytes + r * 128;
+                    if (product != kGram) {
+                        float x[32];
+                        read32<SPLIT>((product == kSquare ? j.a : j.x[src]) + off,
+                                      product == kSquare ? j.a_bytes : j.x_bytes, r, chunk, x);
+                        const float g = product == kSquare ? kNsB : kNsA;
+#pragma unroll
+                        for (int k = 0; k < 32; k++) v[k] += g * x[k];
+                    }
+                    if (last) {
+#pragma unroll
+                        for (int k = 0; k < 32; k++) v[k] *= out_f;
+                        finish<32>(q, j, at.i * kTile + r, bj * kTile + cc, v, bad);
+                        return;
+                    }
+                    uint8_t* dst = product == kGram ? j.a : product == kSquare ? j.b : j.x[src ^ 1];
+                    uint8_t* mirror = product != kApply && bj > at.i
+                                          ? dst + ((long)bj * cb + 2 * at.i + (r >> 6)) * kTileBytes
+                                          : nullptr;
+                    write32<SPLIT>(dst + off, product == kApply ? j.x_bytes : j.a_bytes, r, chunk, v, mirror, cc);
+                };
+                if (SPLIT) {
+                    float acc[kCols];
+                    const int segments = (at.k1 - at.k0 + kSegment - 1) / kSegment;
+                    for (int g = 0; g < segments; g++, accs++) {
+                        if (ok) ok = mbar_wait(&tfull[accs & 1], (accs >> 1) & 1, q.status, kStatusWait);
+                        tc_fence_after();
+                        const uint32_t d = tmem + (accs & 1) * BN + c_first + ((uint32_t)((warp & 3) * 32) << 16);
+#pragma unroll
+                        for (int c = 0; c < kCols; c += 16) {
+                            float v[16];
+                            tmem_ld16(d + c, v);
+#pragma unroll
+                            for (int k = 0; k < 16; k++) acc[c + k] = g ? acc[c + k] + v[k] : v[k];
+                        }
+                        tc_fence_before();
+                        mbar_arrive(&tempty[accs & 1]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 32) emit(c_first + c, acc + c);
+                } else {
+                    if (ok) ok = mbar_wait(&tfull[accs & 1], (accs >> 1) & 1, q.status, kStatusWait);
+                    tc_fence_after();
+                    const uint32_t d = tmem + (accs & 1) * BN + ((uint32_t)((warp & 3) * 32) << 16);
+#pragma unroll 1
+                    for (int c = c_first; c < c_first + kCols; c += 32) {
+                        float v[32];
+                        __syncwarp();
+                        tmem_ld32(d + c, v);
+                        emit(c, v);
+                    }
+                    tc_fence_before();
+                    mbar_arrive(&tempty[accs & 1]);
+                    accs++;
+                }
+            }
+            if (!ok) s_ok = 0;
+        }
+        __syncwarp();
+        if (last) break;
+        ok = grid_barrier(q.barrier, ++turn, q.status, &s_ok);
+    }
+    if (bad && q.status) atomicExch(q.status, kStatusNonFinite);
+    __syncthreads();
+    if (warp == 3) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 2 * BN);
+    }
+}
+
 // ------------------------------------------------------------------ host side
 
 struct Shape {
@@ -900,7 +1122,10 @@ struct Shape {
     long bytes(bool split) const { return (2 * x_bytes + 2 * a_bytes) * (split ? 2 : 1); }
 };
 
-constexpr long kNormBytes = (long)kMaxJobs * kMaxNormParts * sizeof(double);
+// Beside the operands: the barrier's counter, partial norms, and the parts of split X X^T (at most one per SM).
+constexpr int kMaxSms = 160;
+constexpr long kControlBytes = 1024, kNormBytes = (long)kMaxJobs * kMaxSms * sizeof(double),
+               kPartBytes = (long)kMaxSms * kTile * kTile * sizeof(float);
 
 long round_up(long v, long to) { return (v + to - 1) / to * to; }
 
@@ -908,54 +1133,77 @@ int scale_exponent(const Shape& s) {
     return std::min(15, (int)std::floor(0.5 * std::log2((double)s.r * s.c)));
 }
 
-void layout_job(Job& j, const Shape& s, bool split, uint8_t*& at, const double* norm, int index) {
-    j.rb = s.rb, j.cb = s.cb;
-    j.x_bytes = s.x_bytes, j.a_bytes = s.a_bytes;
-    const int halves = split ? 2 : 1;
-    j.x[0] = at;
-    j.x[1] = j.x[0] + halves * s.x_bytes;
-    j.a = j.x[1] + halves * s.x_bytes;
-    j.b = j.a + halves * s.a_bytes;
-    at = j.b + halves * s.a_bytes;
-    j.norm = norm + (long)index * kMaxNormParts;
-}
-
-template <int PHASE, bool SPLIT, bool LAST>
-void launch_ns(const Jobs& q, int src, cudaStream_t stream) {
-    using S = Stages<SPLIT>;
+template <bool SPLIT, int BN, int N>
+void launch_tiled(const Jobs<N>& q, cudaStream_t stream) {
+    using S = Stages<SPLIT, BN>;
     static PerDeviceOnce once;
-    once_per_device(once, [] { set_max_dynamic_smem(ns_kernel<PHASE, SPLIT, LAST>, S::kSmem, "ns_kernel"); });
-    const int tiles = PHASE == kApply ? q.full_tiles : q.tri_tiles;
-    ns_kernel<PHASE, SPLIT, LAST><<<std::min(tiles, device_sms()), kThreads, S::kSmem, stream>>>(q, src);
-    launch_check("ns_kernel");
+    once_per_device(once, [] { set_max_dynamic_smem(tiled_kernel<SPLIT, BN, N>, S::kSmem, "tiled_kernel"); });
+    const cudaError_t e = cudaMemsetAsync(q.barrier, 0, sizeof(uint32_t), stream);
+    if (e != cudaSuccess) throw std::runtime_error(std::string("cudaMemsetAsync: ") + cudaGetErrorString(e));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(std::min(device_sms(), kMaxSms));
+    cfg.blockDim = dim3(kTiledThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, tiled_kernel<SPLIT, BN, N>, q);
+    launch_check("tiled_kernel");
 }
 
-template <bool SPLIT>
-void run_jobs(Jobs& q, double* parts, cudaStream_t stream) {
-    long elems = 0, xtiles = 0;
-    q.tri_tiles = q.full_tiles = 0;
-    for (int i = 0; i < q.count; i++) {
-        Job& j = q.job[i];
-        j.tri0 = q.tri_tiles;
-        j.full0 = q.full_tiles;
-        q.tri_tiles += j.rb * (j.rb + 1) / 2;
-        q.full_tiles += j.rb * (j.cb / 2);
-        elems = std::max(elems, (long)j.r * j.c);
-        xtiles = std::max(xtiles, (long)j.rb * j.cb);
+template <bool SPLIT, int N>
+void run_tiled(const Settings& set, const std::vector<Source>& list, uint8_t* workspace, cudaStream_t stream) {
+    Jobs<N> q{};
+    static_cast<Settings&>(q) = set;
+    q.barrier = reinterpret_cast<uint32_t*>(workspace);
+    q.norms = reinterpret_cast<double*>(workspace + kControlBytes);
+    q.parts = reinterpret_cast<float*>(workspace + kControlBytes + kNormBytes);
+    uint8_t* at = workspace + kControlBytes + kNormBytes + kPartBytes;
+    int narrow = 0, full = 0;   // tiles of 128 x 128 of all X X^T: upper triangles, and all of them
+    for (const Source& s : list) {
+        const Shape shape(s.r, s.c);
+        narrow += shape.rb * (shape.rb + 1) / 2;
+        full += shape.rb * shape.rb;
     }
-    q.norm_parts = (int)std::min<long>(kMaxNormParts, (elems + 4095) / 4096);
-    norm_kernel<<<dim3(q.norm_parts, q.count), 256, 0, stream>>>(q, parts);
-    launch_check("norm_kernel");
-    pack_kernel<SPLIT><<<dim3((unsigned)std::min<long>(xtiles, 2048), q.count), 256, 0, stream>>>(q);
-    launch_check("pack_kernel");
-    for (int s = 0; s < q.steps; s++) {
-        launch_ns<kGram, SPLIT, false>(q, s & 1, stream);
-        launch_ns<kSquare, SPLIT, false>(q, s & 1, stream);
-        if (s + 1 < q.steps)
-            launch_ns<kApply, SPLIT, false>(q, s & 1, stream);
-        else
-            launch_ns<kApply, SPLIT, true>(q, s & 1, stream);
+    const int sms = std::min(device_sms(), kMaxSms);
+    // Single fp16 operands are bound by the copies into shared memory, which 128 x 256 tiles cut by a quarter; they
+    // pay once every SM has several of them.  Pairs do three products per copy and need 128 columns' registers.
+    const bool wide = !SPLIT && narrow >= 4 * sms;
+    const int bn = wide ? 256 : 128;
+    for (const Source& source : list) {
+        const Shape s(source.r, source.c);
+        Job& j = q.job[q.count++];
+        static_cast<Source&>(j) = source;
+        j.rb = s.rb, j.cb = s.cb;
+        j.x_bytes = s.x_bytes, j.a_bytes = s.a_bytes;
+        const int halves = SPLIT ? 2 : 1;
+        j.x[0] = at;
+        j.x[1] = j.x[0] + halves * s.x_bytes;
+        j.a = j.x[1] + halves * s.x_bytes;
+        j.b = j.a + halves * s.a_bytes;
+        at = j.b + halves * s.a_bytes;
+        // split X X^T while its tiles leave SMs idle, in parts of four stages at least
+        j.splits = std::max(1, std::min(sms / std::max(1, full), ((s.c + 63) / 64) / 4));
+        j.pack0 = q.packs, j.gram0 = q.grams, j.square0 = q.squares, j.apply0 = q.applies, j.sum0 = q.sums;
+        j.part0 = q.grams;      // read only where splits > 1, when every X X^T unit has a part
+        const int triangle = bn == 128 ? s.rb * (s.rb + 1) / 2 : [&] {
+            int n = 0;
+            for (int c = 0; 2 * c < s.rb; c++) n += std::min(2 * c + 2, s.rb);
+            return n;
+        }();
+        q.packs += s.rb * s.cb;
+        q.grams += j.splits > 1 ? s.rb * s.rb * j.splits : triangle;
+        q.squares += triangle;
+        q.applies += s.rb * ((s.cb * 64 + bn - 1) / bn);
+        if (j.splits > 1) q.sums += s.rb * s.rb * kTile * kTile / 8;
     }
+    if constexpr (!SPLIT) {
+        if (wide) return launch_tiled<false, 256, N>(q, stream);
+    }
+    launch_tiled<SPLIT, 128, N>(q, stream);
 }
 
 // CTAs a matrix takes on the cluster path (a power of two up to 8), 0 where it does not fit.  One per 64 columns,
@@ -1031,30 +1279,24 @@ void run_sources(const Settings& set, const std::vector<Source>& list, void* wor
         else
             launch_slabs<SPLIT, kMaxJobs>(set, part, stream);
     }
-    double* parts = reinterpret_cast<double*>(round_up(reinterpret_cast<intptr_t>(workspace), 1024));
-    Jobs q{};
-    static_cast<Settings&>(q) = set;
-    uint8_t* at = nullptr;
-    for (size_t i = 0; i < tiled.size(); i++) {
-        if (q.count == 0) at = reinterpret_cast<uint8_t*>(parts) + kNormBytes;
-        Job& j = q.job[q.count];
-        j = Job{};
-        static_cast<Source&>(j) = tiled[i];
-        layout_job(j, Shape(j.r, j.c), SPLIT, at, parts, q.count);
-        if (++q.count == kMaxJobs || i + 1 == tiled.size()) {
-            run_jobs<SPLIT>(q, parts, stream);
-            q.count = 0;
-        }
+    uint8_t* at = reinterpret_cast<uint8_t*>(round_up(reinterpret_cast<intptr_t>(workspace), 1024));
+    for (size_t first = 0; first < tiled.size(); first += kMaxJobs) {
+        const std::vector<Source> part(tiled.begin() + first,
+                                       tiled.begin() + std::min<size_t>(tiled.size(), first + kMaxJobs));
+        if (part.size() == 1)
+            run_tiled<SPLIT, 1>(set, part, at, stream);
+        else
+            run_tiled<SPLIT, kMaxJobs>(set, part, at, stream);
     }
 }
 
-// Bytes of the tiled path for these shapes; its chunks of kMaxJobs matrices run one after another in the same
-// memory.  A call whose matrices all take the cluster path needs none, but the size may not depend on which
-// matrices of a list are active, so every matrix counts.
-size_t tiled_bytes(const std::vector<Shape>& shapes, bool split) {
+// Workspace of a call.  Matrices on the cluster path need none; whether a shape takes it does not depend on the rest of
+// the list (slab_ranks tries clusters up to eight for any), so a call with part of a list's matrices needs no more.
+size_t workspace_bytes(const std::vector<Shape>& shapes, bool split) {
     long sum = 0;
-    for (const Shape& s : shapes) sum += s.bytes(split);
-    return (size_t)(kNormBytes + sum + 1024);
+    for (const Shape& s : shapes)
+        if (!slab_ranks(s, split, 1)) sum += s.bytes(split);
+    return (size_t)(1024 + (sum ? kControlBytes + kNormBytes + kPartBytes + sum : 0));
 }
 
 bool aligned16(const void* p, long pitch_bytes, int bytes) {
@@ -1067,7 +1309,7 @@ size_t muon_workspace_bytes(const MuonMatrix* m, int count, bool split) {
     std::vector<Shape> shapes;
     for (int i = 0; i < count; i++)
         if (m[i].rows && m[i].cols) shapes.emplace_back(m[i].rows, m[i].cols);
-    return tiled_bytes(shapes, split);
+    return workspace_bytes(shapes, split);
 }
 
 void muon_update(const MuonMatrix* m, int count, const MuonRule& rule, void* workspace, int* status,
@@ -1096,7 +1338,7 @@ void muon_update(const MuonMatrix* m, int count, const MuonRule& rule, void* wor
 
 size_t orthogonalize_workspace_bytes(int rows, int cols, int out_type) {
     if (rows == 0 || cols == 0) return 0;
-    return tiled_bytes({Shape(rows, cols)}, out_type == kTypeF32);
+    return workspace_bytes({Shape(rows, cols)}, out_type == kTypeF32);
 }
 
 void orthogonalize(const void* in, int in_type, long in_pitch, int rows, int cols, int steps, void* out, int out_type,

@@ -128,7 +128,7 @@ def test_layout_sizes(rows, cols):
 
 def test_workspaces_grow_with_the_matrix_and_with_the_precision():
     single = sy.orthogonalize_workspace(256, 512, sy.SY_TYPE_BF16)
-    assert 0 < single < sy.orthogonalize_workspace(256, 512, sy.SY_TYPE_F32)
+    assert 0 < sy.orthogonalize_workspace(64, 576, sy.SY_TYPE_BF16) < single < sy.orthogonalize_workspace(256, 512, sy.SY_TYPE_F32)
     assert single == sy.orthogonalize_workspace(512, 256, sy.SY_TYPE_BF16)
     one = sy.muon_tensors([(P, P, P, 256, 512)])
     two = sy.muon_tensors([(P, P, P, 256, 512)] * 2)

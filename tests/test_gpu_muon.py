@@ -25,7 +25,8 @@ def update(rows, cols, seed, dtype=torch.float32):
 
 
 SHAPES = [(1, 1), (1, 300), (300, 1), (2, 2), (17, 5), (64, 576), (80, 720), (127, 129), (128, 128), (129, 640),
-          (576, 64), (700, 333), (130, 2304), (512, 512)]
+          (576, 64), (700, 333), (130, 2304), (512, 512), (129, 129), (128, 3000), (4500, 140), (300, 9000), (1100, 1030),
+          (3500, 3400)]
 
 
 @pytest.mark.parametrize("rows, cols", SHAPES)
@@ -116,8 +117,9 @@ def test_muon_list(opts, precision, tol):
     check_muon(shapes, opts, sy.muon_options(precision=precision, **opts), tol)
 
 
-def test_muon_of_more_matrices_than_one_launch_takes():
-    shapes = [(8 + i, 200 - 2 * i) for i in range(70)]
+@pytest.mark.parametrize("shapes", [[(8 + i, 200 - 2 * i) for i in range(70)], [(130 + i, 140 + 3 * i) for i in range(37)],
+                                    [(130 + 40 * (i % 2), 60 + 37 * i) for i in range(40)], [(900, 1300), (1000, 2049), (2000, 300)]])
+def test_muon_of_longer_lists_and_larger_matrices(shapes):
     check_muon(shapes, dict(lr=0.02), sy.muon_options(0.02), SPLIT_TOL)
 
 
@@ -144,11 +146,12 @@ def test_muon_skips_empty_matrices_and_reports_values_that_are_not_finite():
     del keep
 
 
-def test_graphs_with_their_own_workspaces_replay_side_by_side():
+@pytest.mark.parametrize("shapes", [[(64, 200), (100, 60)], [(200, 300), (64, 200), (140, 131)]])
+def test_graphs_with_their_own_workspaces_replay_side_by_side(shapes):
     o = sy.muon_options(0.02, weight_decay=0.01)
     runs = []
     for seed in (1, 2):
-        w, m, d = ([x.cuda() for x in v] for v in lists([(64, 200), (100, 60)], seed))
+        w, m, d = ([x.cuda() for x in v] for v in lists(shapes, seed))
         t = sy.muon_tensors([(a.data_ptr(), b.data_ptr(), c.data_ptr(), *a.shape) for a, b, c in zip(w, m, d)])
         work = torch.empty(sy.muon_workspace(t, o), dtype=torch.uint8, device="cuda")
         s = torch.cuda.Stream()
