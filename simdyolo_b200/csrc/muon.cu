@@ -48,7 +48,7 @@ struct Source {
     int p;                      // X is held times 2^p
     int in_type, out_type;
     float rate;                 // Muon: factor of O in the update
-    int vec;                    // rows of every matrix start on 16 bytes (8 for 16-bit types)
+    int mode;                   // how U (and the momentum) is read
 };
 
 struct Settings {
@@ -68,30 +68,37 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
     lo = __float2half_rn(v - __half2float(hi));
 }
 
-// Up to four consecutive values (the first n; the rest are zero).  Read past L1: Muon's momentum may just have been
-// written by another SM.
-__device__ __forceinline__ float4 load_u4(const void* in, int type, long at, int n, bool vec) {
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (n <= 0) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (type == kTypeF32) {
-        const float* p = static_cast<const float*>(in) + at;
-        if (vec && n >= 4) return __ldcg(reinterpret_cast<const float4*>(p));
-        for (int i = 0; i < 4; i++)
-            if (i < n) v[i] = __ldcg(p + i);
+// How four consecutive values of a matrix are read: one access where its rows are aligned and a multiple of four long,
+// otherwise value by value.
+enum { kWide32, kWide16, kAny32, kAny16 };
+
+// Up to four consecutive values from `at` (the first n; the rest are zero; the wide modes see multiples of four only).
+// Without branches, so that a thread's loads overlap: a lane with nothing to read takes the first value.  Past L1:
+// Muon's momentum may just have been written by another SM.
+template <int MODE>
+__device__ __forceinline__ float4 load_u4(const void* in, int type, long at, int n) {
+    float v[4];
+    if (MODE == kWide32) {
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(in) + (n > 0 ? at : 0)));
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    } else if (MODE == kAny32) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = __ldcg(static_cast<const float*>(in) + (i < n ? at + i : 0));
     } else {
-        const uint16_t* p = static_cast<const uint16_t*>(in) + at;
-        uint16_t h[4] = {0, 0, 0, 0};
-        if (vec && n >= 4) {
-            const uint2 u = __ldcg(reinterpret_cast<const uint2*>(p));
-            h[0] = (uint16_t)u.x, h[1] = (uint16_t)(u.x >> 16), h[2] = (uint16_t)u.y, h[3] = (uint16_t)(u.y >> 16);
+        const uint16_t* p = static_cast<const uint16_t*>(in);
+        uint32_t h[4];
+        if (MODE == kWide16) {
+            const uint2 u = __ldcg(reinterpret_cast<const uint2*>(p + (n > 0 ? at : 0)));
+            h[0] = u.x & 0xffff, h[1] = u.x >> 16, h[2] = u.y & 0xffff, h[3] = u.y >> 16;
         } else {
-            for (int i = 0; i < 4; i++)
-                if (i < n) h[i] = __ldcg(p + i);
+#pragma unroll
+            for (int i = 0; i < 4; i++) h[i] = __ldcg(p + (i < n ? at + i : 0));
         }
+#pragma unroll
         for (int i = 0; i < 4; i++)
-            v[i] = type == kTypeBF16 ? __uint_as_float((uint32_t)h[i] << 16) : __half2float(__ushort_as_half(h[i]));
+            v[i] = type == kTypeBF16 ? __uint_as_float(h[i] << 16) : __half2float(__ushort_as_half((uint16_t)h[i]));
     }
-    return make_float4(v[0], v[1], v[2], v[3]);
+    return make_float4(n > 0 ? v[0] : 0.0f, n > 1 ? v[1] : 0.0f, n > 2 ? v[2] : 0.0f, n > 3 ? v[3] : 0.0f);
 }
 
 // Muon's direction from the (scaled) gradient g and the new momentum m
@@ -100,6 +107,7 @@ __device__ __forceinline__ float direction(const Settings& q, float g, float m) 
 }
 
 // The momentum step of up to four values at `at`; v: the gradient, then the direction.
+template <int MODE>
 __device__ __forceinline__ void update_momentum(const Settings& q, const Source& j, long at, int n, float* v,
                                                 const float4& old) {
     float w[4] = {old.x, old.y, old.z, old.w};
@@ -108,8 +116,8 @@ __device__ __forceinline__ void update_momentum(const Settings& q, const Source&
         w[k] = q.momentum * w[k] + q.grad_scale * v[k];
         v[k] = direction(q, v[k], w[k]);
     }
-    if (j.vec && n >= 4) {
-        *reinterpret_cast<float4*>(j.momentum + at) = make_float4(w[0], w[1], w[2], w[3]);
+    if (MODE == kWide32) {
+        if (n > 0) *reinterpret_cast<float4*>(j.momentum + at) = make_float4(w[0], w[1], w[2], w[3]);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; k++)
@@ -118,10 +126,11 @@ __device__ __forceinline__ void update_momentum(const Settings& q, const Source&
 }
 
 // U after the momentum step: up to four values
+template <int MODE>
 __device__ __forceinline__ float4 load_direction4(const Settings& q, const Source& j, long at, int n) {
-    float4 g = load_u4(j.in, j.in_type, at, n, j.vec);
-    if (j.weight) {
-        const float4 m = load_u4(j.momentum, kTypeF32, at, n, j.vec);
+    float4 g = load_u4<MODE>(j.in, j.in_type, at, n);
+    if ((MODE == kWide32 || MODE == kAny32) && j.weight) {
+        const float4 m = load_u4<MODE>(j.momentum, kTypeF32, at, n);
         g.x = direction(q, g.x, m.x), g.y = direction(q, g.y, m.y);
         g.z = direction(q, g.z, m.z), g.w = direction(q, g.w, m.w);
     }
@@ -157,33 +166,49 @@ __device__ __forceinline__ void pack8(const float* v, uint4& hi, uint4& lo) {
     lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// N consecutive values of a row of O (X's orientation) from `col` on: the output, or the weight update.  The old
-// weights are all loaded before the first is stored, so that the loads overlap.
-template <int N>
-__device__ __forceinline__ void finish(const Settings& q, const Source& j, int row, int col, const float* v, bool& bad) {
-    if (row >= j.r || col >= j.c) return;
-    const int n = min(N, j.c - col);
-    const long at = j.tall ? col * j.out_pitch + row : row * j.out_pitch + col, step = j.tall ? j.out_pitch : 1;
-    if (j.weight) {
-        float w[N];
-        const float keep = 1.0f - q.lr * q.decay;
-        if (!j.tall && j.vec && n == N) {
-            float4* p = reinterpret_cast<float4*>(j.weight + at);
+// Lanes 0-15 and 16-31 hold 16 rows of 16 values each; afterwards lane l holds value l % 16 of all 16 rows of its half.
+__device__ __forceinline__ void transpose16(float* v, int lane) {
 #pragma unroll
-            for (int k = 0; k < N / 4; k++) *reinterpret_cast<float4*>(w + 4 * k) = p[k];
+    for (int m = 8; m; m >>= 1) {
+        const bool up = lane & m;
 #pragma unroll
-            for (int k = 0; k < N; k++) {
-                w[k] = w[k] * keep - j.rate * v[k];
-                bad |= !(fabsf(w[k]) <= 3.402823466e38f);
-            }
-#pragma unroll
-            for (int k = 0; k < N / 4; k++) p[k] = *reinterpret_cast<const float4*>(w + 4 * k);
-            return;
+        for (int k = 0; k < 16; k++) {
+            if (k & m) continue;
+            const float got = __shfl_xor_sync(0xffffffffu, up ? v[k] : v[k + m], m);
+            if (up)
+                v[k] = got;
+            else
+                v[k + m] = got;
         }
+    }
+}
+
+// 16 consecutive values of O (X's orientation) per lane, from column `col` of row row0 + lane: the output, or the weight
+// update.  Called by a whole warp.  Where X is U the block is transposed between the lanes first, so that a warp's
+// accesses run along the rows of the output for any pitch and alignment; where X is U transposed they do already.
+// The old weights are all loaded before the first is stored, so that the loads overlap.
+__device__ __forceinline__ void finish16(const Settings& q, const Source& j, int row0, int col, float* v, bool& bad) {
+    const int lane = threadIdx.x & 31;
+    long at, step;
+    int n;                           // valid values of this lane
+    if (j.tall) {
+        const int row = row0 + lane;
+        at = (long)col * j.out_pitch + row, step = j.out_pitch;
+        n = row < j.r ? min(16, j.c - col) : 0;
+    } else {
+        transpose16(v, lane);
+        const int row = row0 + (lane & 16);
+        col += lane & 15;
+        at = (long)row * j.out_pitch + col, step = j.out_pitch;
+        n = col < j.c ? min(16, j.r - row) : 0;
+    }
+    if (j.weight) {
+        float w[16];
+        const float keep = 1.0f - q.lr * q.decay;
 #pragma unroll
-        for (int k = 0; k < N; k++) w[k] = k < n ? j.weight[at + k * step] : 0.0f;
+        for (int k = 0; k < 16; k++) w[k] = k < n ? j.weight[at + k * step] : 0.0f;
 #pragma unroll
-        for (int k = 0; k < N; k++) {
+        for (int k = 0; k < 16; k++) {
             w[k] = w[k] * keep - j.rate * v[k];
             if (k < n) {
                 bad |= !(fabsf(w[k]) <= 3.402823466e38f);
@@ -193,12 +218,12 @@ __device__ __forceinline__ void finish(const Settings& q, const Source& j, int r
     } else if (j.out_type == kTypeF32) {
         float* o = static_cast<float*>(j.out) + at;
 #pragma unroll
-        for (int k = 0; k < N; k++)
+        for (int k = 0; k < 16; k++)
             if (k < n) o[k * step] = v[k];
     } else {
         uint16_t* o = static_cast<uint16_t*>(j.out) + at;
 #pragma unroll
-        for (int k = 0; k < N; k++)
+        for (int k = 0; k < 16; k++)
             if (k < n)
                 o[k * step] = j.out_type == kTypeBF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v[k]))
                                                       : __half_as_ushort(__float2half_rn(v[k]));
@@ -233,10 +258,10 @@ struct SlabJobs : Settings {
 __host__ __device__ constexpr int slab_x_bytes(int rows, int width) { return width / 64 * rows * 128; }   // one half
 __host__ __device__ constexpr int slab_a_bytes(int rows) { return (rows + 63) / 64 * rows * 128; }
 __host__ __device__ constexpr int slab_part_bytes(int rows) { return rows * (rows + 4) * 4; }
-int slab_smem(int rows, int width, bool split) {
+int slab_smem(int rows, int width, int ranks, bool split) {
     const int tiles = (slab_x_bytes(rows, width) + slab_a_bytes(rows)) * (split ? 2 : 1);
     // the last operand tile may be read for 128 rows
-    return 1024 + std::max(tiles + slab_part_bytes(rows), tiles - rows * 128 + 128 * 128);
+    return 1024 + std::max(tiles + (ranks > 1 ? slab_part_bytes(rows) : 0), tiles - rows * 128 + 128 * 128);
 }
 
 __device__ __forceinline__ void slab_cluster_sync() {
@@ -318,6 +343,92 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t a_lo, 
     }
 }
 
+// The part of U that a CTA of the cluster path reads: units of four values along U's contiguous axis (X's columns, or
+// its rows when tall), zero outside the matrix.
+struct SlabUnits {
+    int col0, per, count, live_across, live_along, tall;
+    float per_inv;
+    __device__ SlabUnits(const SlabJob& j, int col0, int cols, int tiles) : col0(col0), tall(j.tall) {
+        per = (j.tall ? j.rows : tiles * 64) / 4;
+        count = (j.tall ? cols : j.rows) * per;
+        live_across = j.tall ? cols : j.r, live_along = j.tall ? j.r : cols;
+        per_inv = 1.0f / per;
+    }
+    // values of unit u that exist, and where they are; line and k: its place across and along
+    __device__ int locate(int u, long pitch, int& line, int& k, long& at) const {
+        line = fast_div(u, per_inv), k = (u - line * per) * 4;
+        at = (tall ? col0 + line : (long)line) * pitch + (tall ? k : col0 + k);
+        return u < count && line < live_across ? live_along - k : 0;
+    }
+};
+
+// Momentum and this thread's part of |U|^2 (double: no scale of the gradient overflows or loses terms).  d: the last
+// four units, which are all of this thread's where the slab is small.
+template <int MODE>
+__device__ __forceinline__ double slab_norm(const Settings& q, const SlabJob& j, const SlabUnits& units, float4* d) {
+    double s = 0.0;
+    for (int base = threadIdx.x; base < units.count; base += 4 * kSlabThreads) {
+        float4 g[4], m[4];
+        long at[4];
+        int n[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            int line, k;
+            n[i] = units.locate(base + i * kSlabThreads, j.in_pitch, line, k, at[i]);
+            g[i] = load_u4<MODE>(j.in, j.in_type, at[i], n[i]);
+            if ((MODE == kWide32 || MODE == kAny32) && j.weight) m[i] = load_u4<MODE>(j.momentum, kTypeF32, at[i], n[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float v[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+            if ((MODE == kWide32 || MODE == kAny32) && j.weight) update_momentum<MODE>(q, j, at[i], n[i], v, m[i]);
+#pragma unroll
+            for (int k = 0; k < 4; k++) s += (double)v[k] * v[k];
+            d[i] = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    }
+    return s;
+}
+
+// X0 = U / |U| times 2^p
+template <int MODE, bool SPLIT>
+__device__ __forceinline__ void slab_pack(const Settings& q, const SlabJob& j, const SlabUnits& units, const Scale& scale,
+                                          uint8_t* x, int x_lo, float4* d) {
+    const int rows = j.rows;
+    for (int base = threadIdx.x; base < units.count; base += 4 * kSlabThreads) {
+        if (units.count > 4 * kSlabThreads)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                int line, k;
+                long at;
+                const int n = units.locate(base + i * kSlabThreads, j.in_pitch, line, k, at);
+                d[i] = load_direction4<MODE>(q, j, at, n);
+            }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            int line, k0;
+            long at;
+            units.locate(base + i * kSlabThreads, j.in_pitch, line, k0, at);
+            if (base + i * kSlabThreads >= units.count) continue;
+            const float v[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+            __half hi[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) split_half(scale(v[k]), hi[k], lo[k]);
+            if (j.tall) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    *reinterpret_cast<__half*>(x + slab_offset(k0 + k, line, rows)) = hi[k];
+                    if (SPLIT) *reinterpret_cast<__half*>(x + x_lo + slab_offset(k0 + k, line, rows)) = lo[k];
+                }
+            } else {
+                uint8_t* p = x + slab_offset(line, k0, rows);
+                *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(hi);
+                if (SPLIT) *reinterpret_cast<uint2*>(p + x_lo) = *reinterpret_cast<const uint2*>(lo);
+            }
+        }
+    }
+}
+
 template <bool SPLIT, int N>
 __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_constant__ SlabJobs<N> q) {
     extern __shared__ uint8_t raw[];
@@ -356,31 +467,14 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         tmem_relinquish();
     }
 
-    // momentum and |U|^2: units of four values along U's contiguous axis (X's columns, or its rows when tall)
-    const int across = j.tall ? cols : rows, along = j.tall ? rows : tiles * 64;
-    const int live_across = j.tall ? cols : j.r, live_along = j.tall ? j.r : cols;
-    const int per = along / 4, units = across * per;
-    const float per_inv = 1.0f / per;
+    const SlabUnits units(j, col0, cols, tiles);
+    float4 d[4];
     double s = 0.0;
-    for (int base = tid; base < units; base += 4 * kSlabThreads) {
-        float4 g[4], m[4];
-        long at[4];
-        int n[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int u = base + i * kSlabThreads, line = fast_div(u, per_inv), k = (u - line * per) * 4;
-            n[i] = u < units && line < live_across ? live_along - k : 0;
-            at[i] = (j.tall ? col0 + line : (long)line) * j.in_pitch + (j.tall ? k : col0 + k);
-            g[i] = load_u4(j.in, j.in_type, at[i], n[i], j.vec);
-            if (j.weight) m[i] = load_u4(j.momentum, kTypeF32, at[i], n[i], j.vec);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float v[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
-            if (j.weight) update_momentum(q, j, at[i], n[i], v, m[i]);
-#pragma unroll
-            for (int k = 0; k < 4; k++) s += (double)v[k] * v[k];
-        }
+    switch (j.mode) {
+        case kWide32: s = slab_norm<kWide32>(q, j, units, d); break;
+        case kWide16: s = slab_norm<kWide16>(q, j, units, d); break;
+        case kAny32: s = slab_norm<kAny32>(q, j, units, d); break;
+        default: s = slab_norm<kAny16>(q, j, units, d); break;
     }
     s = warp_sum_d(s);
     if (lane == 0) red[warp] = s;
@@ -394,40 +488,17 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         norm = t;
     }
     slab_cluster_sync();
+    const double part_norm = lane < ranks ? peer_load_d(peer_addr(smem_u32(&norm), peer0 + lane)) : 0.0;
     s = 0.0;
-    for (int i = 0; i < ranks; i++) s += peer_load_d(peer_addr(smem_u32(&norm), peer0 + i));
+    for (int i = 0; i < ranks; i++) s += __shfl_sync(0xffffffffu, part_norm, i);
     const Scale scale = scale_of(s, j.p);
 
-    // X0 = U / |U| times 2^p; zero outside the matrix
-    for (int base = tid; base < units; base += 4 * kSlabThreads) {
-        float4 d[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int u = base + i * kSlabThreads, line = fast_div(u, per_inv), k = (u - line * per) * 4;
-            const int n = u < units && line < live_across ? live_along - k : 0;
-            d[i] = load_direction4(
-                q, j, (j.tall ? col0 + line : (long)line) * j.in_pitch + (j.tall ? k : col0 + k), n);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int u = base + i * kSlabThreads, line = fast_div(u, per_inv), k0 = (u - line * per) * 4;
-            if (u >= units) continue;
-            const float v[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
-            __half hi[4], lo[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) split_half(scale(v[k]), hi[k], lo[k]);
-            if (j.tall) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    *reinterpret_cast<__half*>(x + slab_offset(k0 + k, line, rows)) = hi[k];
-                    if (SPLIT) *reinterpret_cast<__half*>(x + x_lo + slab_offset(k0 + k, line, rows)) = lo[k];
-                }
-            } else {
-                uint8_t* p = x + slab_offset(line, k0, rows);
-                *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(hi);
-                if (SPLIT) *reinterpret_cast<uint2*>(p + x_lo) = *reinterpret_cast<const uint2*>(lo);
-            }
-        }
+    // X0, zero outside the matrix
+    switch (j.mode) {
+        case kWide32: slab_pack<kWide32, SPLIT>(q, j, units, scale, x, x_lo, d); break;
+        case kWide16: slab_pack<kWide16, SPLIT>(q, j, units, scale, x, x_lo, d); break;
+        case kAny32: slab_pack<kAny32, SPLIT>(q, j, units, scale, x, x_lo, d); break;
+        default: slab_pack<kAny16, SPLIT>(q, j, units, scale, x, x_lo, d); break;
     }
     if (j.tall)   // columns past the matrix in the last tile
         for (int i = tid; i < (tiles * 64 - cols) * rows; i += kSlabThreads) {
@@ -466,7 +537,11 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
             float v[16];
             __syncwarp();
             tmem_ld16(tmem + trow + c, v);
-            if (row < rows)
+            if (ranks == 1) {
+#pragma unroll
+                for (int k = 0; k < 16; k++) v[k] *= gram_f;
+                if (row < rows) slab_write16<SPLIT>(a, a_lo, row, c, rows, v);
+            } else if (row < rows)
 #pragma unroll
                 for (int k = 0; k < 4; k++)
                     *reinterpret_cast<float4*>(part + row * pp + c + 4 * k) =
@@ -474,16 +549,21 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
         tc_fence_before();
+        if (ranks == 1) {
+            fence_proxy_async();
+            __syncthreads();
+        }
         slab_cluster_sync();
-        // A = the sum over the cluster: this CTA's share of the rows, handed to everyone
+        // A = the sum over the cluster: this CTA's share of the rows, handed to everyone.  Each CTA begins with another
+        // peer, so the order of a sum depends on the row alone.
         const int share = rows / ranks, chunks = rows / 8;
-        for (int u = tid; u < share * chunks; u += kSlabThreads) {
+        for (int u = tid; ranks > 1 && u < share * chunks; u += kSlabThreads) {
             const int r = rank * share + u / chunks, c = u % chunks;
             float4 f[8], g[8];
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 if (i < ranks) {
-                    const uint32_t from = peer_addr(ps + (r * pp + c * 8) * 4, peer0 + i);
+                    const uint32_t from = peer_addr(ps + (r * pp + c * 8) * 4, peer0 + ((rank + i) & (ranks - 1)));
                     f[i] = peer_load4(from), g[i] = peer_load4(from + 16);
                 }
             float v[8] = {};
@@ -499,8 +579,9 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
             pack8(v, hi, lo);
             const uint32_t to = as + slab_offset(r, c * 8, rows);
             for (int i = 0; i < ranks; i++) {
-                peer_store4(peer_addr(to, peer0 + i), hi);
-                if (SPLIT) peer_store4(peer_addr(to + a_lo, peer0 + i), lo);
+                const uint32_t peer = peer0 + ((rank + i) & (ranks - 1));
+                peer_store4(peer_addr(to, peer), hi);
+                if (SPLIT) peer_store4(peer_addr(to + a_lo, peer), lo);
             }
         }
         asm volatile("fence.proxy.async;" ::: "memory");
@@ -555,16 +636,17 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
                 float v[16], old[16];
                 __syncwarp();
                 tmem_ld16(tmem + 128 + trow + c, v);
-                if (row >= rows) continue;
-                slab_read16<SPLIT>(x, x_lo, row, c0 + c, rows, old);
+                if (row < rows) {
+                    slab_read16<SPLIT>(x, x_lo, row, c0 + c, rows, old);
 #pragma unroll
-                for (int k = 0; k < 16; k++) v[k] = kNsA * old[k] + v[k] * back_f;
-                if (!last) {
-                    slab_write16<SPLIT>(x, x_lo, row, c0 + c, rows, v);
-                } else {
+                    for (int k = 0; k < 16; k++) v[k] = kNsA * old[k] + v[k] * back_f;
+                }
+                if (last) {
 #pragma unroll
                     for (int k = 0; k < 16; k++) v[k] *= out_f;
-                    finish<16>(q, j, row, col0 + c0 + c, v, bad);
+                    finish16(q, j, row & ~31, col0 + c0 + c, v, bad);
+                } else if (row < rows) {
+                    slab_write16<SPLIT>(x, x_lo, row, c0 + c, rows, v);
                 }
             }
             fence_proxy_async();
@@ -730,10 +812,10 @@ __device__ __forceinline__ void write32(uint8_t* hi, long lo, int row, int chunk
 // to plain loads and to bulk copies.  Gives up after a bounded number of polls, like every wait here.
 __device__ __forceinline__ bool grid_barrier(uint32_t* counter, uint32_t turn, int* status, int* s_ok) {
     asm volatile("fence.proxy.async;" ::: "memory");
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
         int ok = *s_ok;
+        __threadfence();
         atomicAdd(counter, 1);
         for (uint32_t polls = 0; ok; polls++) {
             uint32_t seen;
@@ -744,12 +826,87 @@ __device__ __forceinline__ bool grid_barrier(uint32_t* counter, uint32_t turn, i
                 if (status) atomicExch(status, kStatusWait);
             }
         }
+        __threadfence();
         *s_ok = ok;
     }
     __syncthreads();
-    __threadfence();
-    asm volatile("fence.proxy.async;" ::: "memory");
     return *s_ok;
+}
+
+// Momentum and this thread's part of |U|^2, units of four values dealt over the whole grid.
+template <int MODE>
+__device__ __forceinline__ double tiled_norm(const Settings& q, const Job& j) {
+    const int lines = j.tall ? j.c : j.r, length = j.tall ? j.r : j.c, per = (length + 3) / 4;
+    const long units = (long)lines * per, stride = (long)gridDim.x * kTiledThreads;
+    double s = 0.0;
+    for (long base = (long)blockIdx.x * kTiledThreads + threadIdx.x; base < units; base += 4 * stride) {
+        float4 g[4], m[4];
+        long at[4];
+        int n[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const long u = base + i * stride, line = u / per;
+            const int k = (int)(u - line * per) * 4;
+            n[i] = u < units ? length - k : 0;
+            at[i] = line * j.in_pitch + k;
+            g[i] = load_u4<MODE>(j.in, j.in_type, at[i], n[i]);
+            if ((MODE == kWide32 || MODE == kAny32) && j.weight) m[i] = load_u4<MODE>(j.momentum, kTypeF32, at[i], n[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float v[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+            if ((MODE == kWide32 || MODE == kAny32) && j.weight) update_momentum<MODE>(q, j, at[i], n[i], v, m[i]);
+#pragma unroll
+            for (int k = 0; k < 4; k++) s += (double)v[k] * v[k];
+        }
+    }
+    return s;
+}
+
+// One 128 x 64 tile of X0 = U / |U| times 2^p, zero outside the matrix.
+template <int MODE, bool SPLIT>
+__device__ __forceinline__ void tiled_pack(const Settings& q, const Job& j, const Scale& scale, int row0, int col0,
+                                           uint8_t* dst) {
+    if (!j.tall) {
+        // eight columns of a row per unit
+        for (int u = threadIdx.x; u < 128 * 8; u += kTiledThreads) {
+            const int row = u >> 3, col = (u & 7) * 8;
+            float v[8];
+            const int left = row0 + row < j.r ? j.c - col0 - col : 0;
+            const long at = (row0 + row) * j.in_pitch + col0 + col;
+            const float4 d[2] = {load_direction4<MODE>(q, j, at, left), load_direction4<MODE>(q, j, at + 4, left - 4)};
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                v[4 * k] = scale(d[k].x), v[4 * k + 1] = scale(d[k].y), v[4 * k + 2] = scale(d[k].z),
+                          v[4 * k + 3] = scale(d[k].w);
+            uint4 hi, lo;
+            pack8(v, hi, lo);
+            uint8_t* p = dst + row * 128 + (((u & 7) ^ (row & 7)) << 4);
+            *reinterpret_cast<uint4*>(p) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(p + j.x_bytes) = lo;
+        }
+    } else {
+        // four rows of eight columns per unit: eight lines of U, lanes along them
+        for (int u = threadIdx.x; u < 32 * 8; u += kTiledThreads) {
+            const int row = (u & 31) * 4, chunk = u >> 5;
+            float v[4][8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int line = col0 + chunk * 8 + k;
+                const float4 d = load_direction4<MODE>(q, j, line * j.in_pitch + row0 + row,
+                                                       line < j.c ? j.r - row0 - row : 0);
+                v[0][k] = scale(d.x), v[1][k] = scale(d.y), v[2][k] = scale(d.z), v[3][k] = scale(d.w);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint4 hi, lo;
+                pack8(v[i], hi, lo);
+                uint8_t* p = dst + (row + i) * 128 + ((chunk ^ ((row + i) & 7)) << 4);
+                *reinterpret_cast<uint4*>(p) = hi;
+                if (SPLIT) *reinterpret_cast<uint4*>(p + j.x_bytes) = lo;
+            }
+        }
+    }
 }
 
 template <bool SPLIT, int BN, int N>
@@ -789,29 +946,12 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
     // momentum and the partial sums of squares of U (double: no scale of the gradient overflows or loses terms)
     for (int n = 0; n < q.count; n++) {
         const Job& j = q.job[n];
-        const int lines = j.tall ? j.c : j.r, length = j.tall ? j.r : j.c, per = (length + 3) / 4;
-        const long units = (long)lines * per;
         double s = 0.0;
-        for (long base = (long)blockIdx.x * kTiledThreads + tid; base < units; base += 4L * gridDim.x * kTiledThreads) {
-            float4 g[4], m[4];
-            long at[4];
-            int left[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const long u = base + (long)i * gridDim.x * kTiledThreads, line = u / per;
-                const int k = (int)(u - line * per) * 4;
-                left[i] = u < units ? length - k : 0;
-                at[i] = line * j.in_pitch + k;
-                g[i] = load_u4(j.in, j.in_type, at[i], left[i], j.vec);
-                if (j.weight) m[i] = load_u4(j.momentum, kTypeF32, at[i], left[i], j.vec);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float v[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
-                if (j.weight) update_momentum(q, j, at[i], left[i], v, m[i]);
-#pragma unroll
-                for (int k = 0; k < 4; k++) s += (double)v[k] * v[k];
-            }
+        switch (j.mode) {
+            case kWide32: s = tiled_norm<kWide32>(q, j); break;
+            case kWide16: s = tiled_norm<kWide16>(q, j); break;
+            case kAny32: s = tiled_norm<kAny32>(q, j); break;
+            default: s = tiled_norm<kAny16>(q, j); break;
         }
         s = warp_sum_d(s);
         if (lane == 0) red[warp] = s;
@@ -844,45 +984,11 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
         const Scale scale = scale_of(s_norm, j.p);
         const int block = (t - j.pack0) / j.cb, row0 = block * 128, col0 = (t - j.pack0 - block * j.cb) * 64;
         uint8_t* dst = j.x[0] + (long)(t - j.pack0) * kTileBytes;
-        if (!j.tall) {
-            // eight columns of a row per unit
-            for (int u = tid; u < 128 * 8; u += kTiledThreads) {
-                const int row = u >> 3, col = (u & 7) * 8;
-                float v[8];
-                const int left = row0 + row < j.r ? j.c - col0 - col : 0;
-                const long at = (row0 + row) * j.in_pitch + col0 + col;
-                const float4 d[2] = {load_direction4(q, j, at, left), load_direction4(q, j, at + 4, left - 4)};
-#pragma unroll
-                for (int k = 0; k < 2; k++)
-                    v[4 * k] = scale(d[k].x), v[4 * k + 1] = scale(d[k].y), v[4 * k + 2] = scale(d[k].z),
-                              v[4 * k + 3] = scale(d[k].w);
-                uint4 hi, lo;
-                pack8(v, hi, lo);
-                uint8_t* p = dst + row * 128 + (((u & 7) ^ (row & 7)) << 4);
-                *reinterpret_cast<uint4*>(p) = hi;
-                if (SPLIT) *reinterpret_cast<uint4*>(p + j.x_bytes) = lo;
-            }
-        } else {
-            // four rows of eight columns per unit: eight lines of U, lanes along them
-            for (int u = tid; u < 32 * 8; u += kTiledThreads) {
-                const int row = (u & 31) * 4, chunk = u >> 5;
-                float v[4][8];
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const int line = col0 + chunk * 8 + k;
-                    const float4 d = load_direction4(q, j, line * j.in_pitch + row0 + row,
-                                                     line < j.c ? j.r - row0 - row : 0);
-                    v[0][k] = scale(d.x), v[1][k] = scale(d.y), v[2][k] = scale(d.z), v[3][k] = scale(d.w);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint4 hi, lo;
-                    pack8(v[i], hi, lo);
-                    uint8_t* p = dst + (row + i) * 128 + ((chunk ^ ((row + i) & 7)) << 4);
-                    *reinterpret_cast<uint4*>(p) = hi;
-                    if (SPLIT) *reinterpret_cast<uint4*>(p + j.x_bytes) = lo;
-                }
-            }
+        switch (j.mode) {
+            case kWide32: tiled_pack<kWide32, SPLIT>(q, j, scale, row0, col0, dst); break;
+            case kWide16: tiled_pack<kWide16, SPLIT>(q, j, scale, row0, col0, dst); break;
+            case kAny32: tiled_pack<kAny32, SPLIT>(q, j, scale, row0, col0, dst); break;
+            default: tiled_pack<kAny16, SPLIT>(q, j, scale, row0, col0, dst); break;
         }
     }
     ok = ok && grid_barrier(q.barrier, ++turn, q.status, &s_ok);
@@ -926,6 +1032,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
         if (warp == 0) {
             if (lane == 0) {
                 const int first = n;
+                asm volatile("fence.proxy.async;" ::: "memory");   // what the barrier made visible, to bulk copies too
                 for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
                     const TileAt at = tile_at<BN>(q, product, t);
                     const Job& j = q.job[at.job];
@@ -1048,7 +1155,8 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                     if (last) {
 #pragma unroll
                         for (int k = 0; k < 32; k++) v[k] *= out_f;
-                        finish<32>(q, j, at.i * kTile + r, bj * kTile + cc, v, bad);
+                        finish16(q, j, at.i * kTile + (r & ~31), bj * kTile + cc, v, bad);
+                        finish16(q, j, at.i * kTile + (r & ~31), bj * kTile + cc + 16, v + 16, bad);
                         return;
                     }
                     uint8_t* dst = product == kGram ? j.a : product == kSquare ? j.b : j.x[src ^ 1];
@@ -1214,7 +1322,7 @@ int slab_ranks(const Shape& s, bool split, size_t matrices) {
     const int rows = (s.r + 15) / 16 * 16;
     for (int ranks = 1; ranks <= 8; ranks *= 2) {
         const int width = (s.c + 64 * ranks - 1) / (64 * ranks) * 64;
-        if (slab_smem(rows, width, split) > kMaxSmem - 1024) continue;
+        if (slab_smem(rows, width, ranks, split) > kMaxSmem - 1024) continue;
         if (ranks == 8 || width == 64 || 2 * ranks * matrices > 128) return ranks;
     }
     return 0;
@@ -1232,7 +1340,7 @@ void launch_slabs(const Settings& set, const std::vector<SlabJob>& list, cudaStr
         SlabJob& j = q.job[q.count++] = s;
         j.first = ctas;
         ctas += j.ranks;
-        smem = std::max(smem, slab_smem(j.rows, j.width, SPLIT));
+        smem = std::max(smem, slab_smem(j.rows, j.width, j.ranks, SPLIT));
     }
     static PerDeviceOnce once;
     once_per_device(once, [] { set_max_dynamic_smem(slab_kernel<SPLIT, N>, kMaxSmem - 1024, "slab_kernel"); });
@@ -1299,7 +1407,7 @@ size_t workspace_bytes(const std::vector<Shape>& shapes, bool split) {
     return (size_t)(1024 + (sum ? kControlBytes + kNormBytes + kPartBytes + sum : 0));
 }
 
-bool aligned16(const void* p, long pitch_bytes, int bytes) {
+bool aligned(const void* p, long pitch_bytes, int bytes) {
     return reinterpret_cast<uintptr_t>(p) % bytes == 0 && pitch_bytes % bytes == 0;
 }
 
@@ -1326,8 +1434,7 @@ void muon_update(const MuonMatrix* m, int count, const MuonRule& rule, void* wor
         s.tall = m[i].rows > m[i].cols;
         s.p = scale_exponent(shape);
         s.rate = (float)((double)rule.lr * rule.rms * std::sqrt((double)shape.c));
-        s.vec = aligned16(s.in, s.in_pitch * 4, 16) && aligned16(s.momentum, s.in_pitch * 4, 16) &&
-                aligned16(s.weight, s.in_pitch * 4, 16);
+        s.mode = aligned(s.in, s.in_pitch * 4, 16) && aligned(s.momentum, s.in_pitch * 4, 16) ? kWide32 : kAny32;
         list.push_back(s);
     }
     if (rule.split)
@@ -1355,7 +1462,8 @@ void orthogonalize(const void* in, int in_type, long in_pitch, int rows, int col
     s.tall = rows > cols;
     s.p = scale_exponent(shape);
     const int bytes = in_type == kTypeF32 ? 4 : 2;
-    s.vec = aligned16(in, in_pitch * bytes, 4 * bytes);
+    const bool wide = aligned(in, in_pitch * bytes, 4 * bytes) && cols % 4 == 0;
+    s.mode = in_type == kTypeF32 ? (wide ? kWide32 : kAny32) : (wide ? kWide16 : kAny16);
     if (out_type == kTypeF32)
         run_sources<true>(set, {s}, workspace, stream);
     else
