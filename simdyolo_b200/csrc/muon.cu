@@ -678,14 +678,15 @@ struct Job : Source {
     long x_bytes, a_bytes;
     int rb, cb;                 // 128-row blocks of X; 64-column blocks (padded to an even number)
     int splits;                 // parts of X X^T's K
-    // first unit of this matrix in: packing (128 x 64 tiles), X X^T, A^2, B X, the sum of the split X X^T (16-byte
-    // pieces) and the parts' memory (128 x 128 tiles)
-    int pack0, gram0, square0, apply0, sum0, part0;
+    // first unit of this matrix in: packing (128 x 64 tiles), each product, and the sum of the split X X^T (16-byte
+    // pieces)
+    int pack0, tile0[3], sum0;
 };
 template <int N>
 struct Jobs : Settings {
     int count;
-    int packs, grams, squares, applies, sums;   // units of each phase
+    int packs, sums;                            // units of packing and of the sum of split products
+    int tiles[3], bn[3], upper[3];              // of each product: units, tile columns, upper triangle only
     double* norms;                              // [count][gridDim]
     float* parts;
     uint32_t* barrier;
@@ -699,73 +700,83 @@ constexpr int kTiledThreads = 32 * (4 + kEpilogueWarps);
 constexpr int kTiledBar = 1;                   // a stage is loaded: the waiting warp and the MMA warp
 constexpr int kSegment = 8;                    // stages (of 64 along K) per accumulator of pairs
 
-template <bool SPLIT, int BN>
+// Widest tile: single fp16 operands are bound by the copies into shared memory, which wider tiles cut; pairs do three
+// products per copy, and their sums in registers allow 128 columns.
+template <bool SPLIT>
 struct Stages {
-    static constexpr int kBytesB = BN / 128 * kTileBytes;
-    static constexpr int kHalf = kTileBytes + kBytesB;            // hi operands, then lo operands
+    static constexpr int kBn = SPLIT ? 128 : 256;
+    static constexpr int kHalf = kTileBytes + kBn / 128 * kTileBytes;   // hi operands, then lo operands
     static constexpr int kBytes = (SPLIT ? 2 : 1) * kHalf;
     static constexpr int kCount = 196608 / kBytes;
     static constexpr int kSmem = 1024 + kCount * kBytes + (2 * kCount + 4) * 8 + 16;
 };
 
 struct TileAt {
-    int job, i, j, k0, k1, split;   // 128-row block, BN-column block, stages along K
+    int job, i, j, k0, k1, split;   // 128-row block, column block of the product's width, stages along K
 };
 
-// unit t of a product phase: which matrix, which tile of it, which part of K
-template <int BN, int N>
-__device__ __forceinline__ TileAt tile_at(const Jobs<N>& q, int phase, int t) {
-    int n = q.count - 1;
-    while (n > 0 && t < (phase == kGram ? q.job[n].gram0 : phase == kSquare ? q.job[n].square0 : q.job[n].apply0)) n--;
+// unit t of a product: which matrix, which tile of it, which part of K
+template <int N>
+__device__ __forceinline__ TileAt tile_at(const Jobs<N>& q, int product, int t) {
+    int n = N == 1 ? 0 : q.count - 1;
+    while (N > 1 && n > 0 && t < q.job[n].tile0[product]) n--;
     const Job& j = q.job[n];
     TileAt a;
     a.job = n;
     a.split = 0;
     a.k0 = 0;
-    a.k1 = phase == kGram ? (j.c + 63) / 64 : (j.r + 63) / 64;
-    int u = t - (phase == kGram ? j.gram0 : phase == kSquare ? j.square0 : j.apply0);
-    if (phase == kApply) {
-        a.j = u / j.rb;
-        a.i = u - a.j * j.rb;
-    } else if (phase == kGram && j.splits > 1) {   // every tile, in parts
+    a.k1 = ((product == kGram ? j.c : j.r) + 63) / 64;
+    int u = t - j.tile0[product];
+    if (q.upper[product]) {   // the tiles that reach above the diagonal, by columns
+        const int w = q.bn[product] >> 7;          // column j holds row blocks 0 .. w (j + 1) - 1
+        int c = (int)((sqrtf(8.0f / w * u + 1.0f) - 1.0f) * 0.5f);
+        while (w * c * (c + 1) / 2 > u) c--;
+        while (w * (c + 1) * (c + 2) / 2 <= u) c++;
+        a.j = c;
+        a.i = u - w * c * (c + 1) / 2;
+        return a;
+    }
+    if (product == kGram && j.splits > 1) {
         const int all = a.k1;
         a.split = u % j.splits;
         u /= j.splits;
-        a.j = u / j.rb;
-        a.i = u - a.j * j.rb;
         a.k0 = (int)((long)all * a.split / j.splits);
         a.k1 = (int)((long)all * (a.split + 1) / j.splits);
-    } else {   // the tiles that reach above the diagonal, by columns
-        constexpr int kW = BN / 128;               // column j holds row blocks 0 .. kW (j + 1) - 1
-        int c = (int)((sqrtf(8.0f / kW * u + 1.0f) - 1.0f) * 0.5f);
-        while (kW * c * (c + 1) / 2 > u) c--;
-        while (kW * (c + 1) * (c + 2) / 2 <= u) c++;
-        a.j = c;
-        a.i = u - kW * c * (c + 1) / 2;
     }
+    a.j = u / j.rb;
+    a.i = u - a.j * j.rb;
     return a;
 }
 
+// 32 columns of a row of a tile as stored: fp16 values, hi and lo
 template <bool SPLIT>
-__device__ __forceinline__ void read32(const uint8_t* hi, long lo, int row, int chunk0, float* v) {
+struct OldBits {
+    uint4 hi[4], lo[SPLIT ? 4 : 1];
+    __device__ __forceinline__ void load(const uint8_t* row_hi, long lo_at, int row, int chunk0) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint8_t* p = row_hi + (((chunk0 + k) ^ (row & 7)) << 4);
+            hi[k] = __ldcg(reinterpret_cast<const uint4*>(p));
+            if (SPLIT) lo[k] = __ldcg(reinterpret_cast<const uint4*>(p + lo_at));
+        }
+    }
+};
+// v += g (hi + lo)
+template <bool SPLIT>
+__device__ __forceinline__ void add_old(float* v, float g, const OldBits<SPLIT>& x) {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const uint8_t* p = hi + (((chunk0 + k) ^ (row & 7)) << 4);
-        const uint4 h = __ldcg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+        const uint32_t h[4] = {x.hi[k].x, x.hi[k].y, x.hi[k].z, x.hi[k].w};
+        const uint4 low = x.lo[SPLIT ? k : 0];
+        const uint32_t l[4] = {low.x, low.y, low.z, low.w};
 #pragma unroll
-        for (int l = 0; l < 4; l++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[l]));
-            v[8 * k + 2 * l] = f.x, v[8 * k + 2 * l + 1] = f.y;
-        }
-        if (SPLIT) {
-            const uint4 g = __ldcg(reinterpret_cast<const uint4*>(p + lo));
-            const uint32_t x[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-            for (int l = 0; l < 4; l++) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[l]));
-                v[8 * k + 2 * l] += f.x, v[8 * k + 2 * l + 1] += f.y;
+        for (int m = 0; m < 4; m++) {
+            float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[m]));
+            if (SPLIT) {
+                const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&l[m]));
+                a.x += b.x, a.y += b.y;
             }
+            v[8 * k + 2 * m] += g * a.x, v[8 * k + 2 * m + 1] += g * a.y;
         }
     }
 }
@@ -826,7 +837,6 @@ __device__ __forceinline__ bool grid_barrier(uint32_t* counter, uint32_t turn, i
                 if (status) atomicExch(status, kStatusWait);
             }
         }
-        __threadfence();
         *s_ok = ok;
     }
     __syncthreads();
@@ -909,9 +919,9 @@ __device__ __forceinline__ void tiled_pack(const Settings& q, const Job& j, cons
     }
 }
 
-template <bool SPLIT, int BN, int N>
+template <bool SPLIT, int N>
 __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_constant__ Jobs<N> q) {
-    using S = Stages<SPLIT, BN>;
+    using S = Stages<SPLIT>;
     extern __shared__ uint8_t raw[];
     __shared__ double red[kTiledThreads / 32], s_norm;
     __shared__ int s_ok;
@@ -934,7 +944,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
         s_ok = 1;
     }
     if (warp == 3) {
-        tmem_alloc(tmem_slot, 2 * BN);
+        tmem_alloc(tmem_slot, 2 * S::kBn);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -1005,7 +1015,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                 while (k > 0 && u < q.job[k].sum0) k--;
                 const Job& j = q.job[k];
                 const int e = (int)(u - j.sum0), tile = e >> 11, row = (e >> 4) & 127, col = (e & 15) * 8;
-                const float* from = q.parts + (long)(j.part0 + tile * j.splits) * (kTile * kTile) + row * kTile + col;
+                const float* from = q.parts + (long)(j.tile0[kGram] + tile * j.splits) * (kTile * kTile) + row * kTile + col;
                 float v[8] = {};
                 for (int s = 0; s < j.splits; s++) {
                     const float4 f = __ldcg(reinterpret_cast<const float4*>(from + (long)s * kTile * kTile));
@@ -1028,40 +1038,48 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
         }
         const int product = phase == 0 ? kGram : phase == 2 ? kSquare : kApply;
         const bool last = product == kApply && (step >> 2) + 1 == q.steps;
-        const int tiles = product == kGram ? q.grams : product == kSquare ? q.squares : q.applies;
+        const int tiles = q.tiles[product], bn = q.bn[product];
         if (warp == 0) {
             if (lane == 0) {
                 const int first = n;
                 asm volatile("fence.proxy.async;" ::: "memory");   // what the barrier made visible, to bulk copies too
                 for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-                    const TileAt at = tile_at<BN>(q, product, t);
+                    const TileAt at = tile_at(q, product, t);
                     const Job& j = q.job[at.job];
                     const uint8_t* left = product == kGram ? j.x[src] : product == kSquare ? j.a : j.b;
                     const long left_lo = product == kGram ? j.x_bytes : j.a_bytes;
                     const int lcb = product == kGram ? j.cb : 2 * j.rb;
-                    // of the BN columns, those whose operand exists: 64-column blocks of X, 128-row blocks
-                    const int pieces = product == kApply ? min(BN / 64, j.cb - at.j * (BN / 64))
-                                                         : min(BN / 128, j.rb - at.j * (BN / 128));
-                    const int piece = product == kApply ? kTileBytes / 2 : kTileBytes;
+                    // the columns' operand in pieces of 64, those that exist: column blocks of X, halves of row blocks
+                    const int per = bn / 64, pieces = min(per, (product == kApply ? j.cb : 2 * j.rb) - at.j * per);
+                    constexpr int kPiece = kTileBytes / 2;
                     for (int k = at.k0; k < at.k1; k++, n++) {
                         const int s = n % S::kCount;
                         if (!(ok = mbar_wait(&empty[s], ((n / S::kCount) & 1) ^ 1, q.status, kStatusWait))) break;
                         uint8_t* st = smem + s * S::kBytes;
-                        mbar_arrive_expect_tx(&full[s], (kTileBytes + pieces * piece) * (SPLIT ? 2 : 1));
+                        mbar_arrive_expect_tx(&full[s], (kTileBytes + pieces * kPiece) * (SPLIT ? 2 : 1));
                         const uint8_t* a = left + ((long)at.i * lcb + k) * kTileBytes;
                         bulk_load(st, a, kTileBytes, &full[s]);
                         if (SPLIT) bulk_load(st + S::kHalf, a + left_lo, kTileBytes, &full[s]);
-                        for (int h = 0; h < pieces; h++) {
-                            // B X: 64 rows of neighbouring column blocks of X; otherwise neighbouring row blocks
+                        if (product == kApply) {
+                            // 64 rows of neighbouring column blocks of X
                             const uint8_t* b =
-                                product == kApply
-                                    ? j.x[src] + ((long)(k >> 1) * j.cb + at.j * (BN / 64) + h) * kTileBytes +
-                                          (k & 1) * (kTileBytes / 2)
-                                    : left + ((long)(at.j * (BN / 128) + h) * lcb + k) * kTileBytes;
-                            bulk_load(st + kTileBytes + h * piece, b, piece, &full[s]);
-                            if (SPLIT)
-                                bulk_load(st + S::kHalf + kTileBytes + h * piece,
-                                          b + (product == kApply ? j.x_bytes : left_lo), piece, &full[s]);
+                                j.x[src] + ((long)(k >> 1) * j.cb + at.j * per) * kTileBytes + (k & 1) * kPiece;
+                            for (int h = 0; h < pieces; h++) {
+                                bulk_load(st + kTileBytes + h * kPiece, b + h * kTileBytes, kPiece, &full[s]);
+                                if (SPLIT)
+                                    bulk_load(st + S::kHalf + kTileBytes + h * kPiece, b + h * kTileBytes + j.x_bytes,
+                                              kPiece, &full[s]);
+                            }
+                        } else {
+                            // neighbouring row blocks, or half of one
+                            for (int h = 0; h < pieces; h += 2) {
+                                const int at64 = at.j * per + h, bytes = min(2, pieces - h) * kPiece;
+                                const uint8_t* b =
+                                    left + ((long)(at64 >> 1) * lcb + k) * kTileBytes + (at64 & 1) * kPiece;
+                                bulk_load(st + kTileBytes + h * kPiece, b, bytes, &full[s]);
+                                if (SPLIT)
+                                    bulk_load(st + S::kHalf + kTileBytes + h * kPiece, b + left_lo, bytes, &full[s]);
+                            }
                         }
                     }
                 }
@@ -1073,7 +1091,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
         } else if (warp == 2) {
             // every wait of the MMA side; after one that gave up the hand-offs go on, so that every warp finishes
             for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-                const TileAt at = tile_at<BN>(q, product, t);
+                const TileAt at = tile_at(q, product, t);
                 for (int k = at.k0; k < at.k1; k++, n++) {
                     if (k == at.k0 || (SPLIT && (k - at.k0) % kSegment == 0)) {
                         if (ok) ok = mbar_wait(&tempty[accs & 1], ((accs >> 1) & 1) ^ 1, q.status, kStatusWait);
@@ -1085,16 +1103,16 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
             }
             if (!ok) s_ok = 0;
         } else if (warp == 1) {
-            const uint32_t idesc = idesc_f16(BN, product == kApply);
+            const uint32_t idesc = idesc_f16(bn, product == kApply);
             // MN-major: 64-column blocks 8 KB apart, groups of 8 K rows 1 KB apart, 16 K rows per MMA
             const uint32_t lbo = product == kApply ? kTileBytes / 2 : 0;
             const uint32_t step_b = product == kApply ? 2048 / 16 : 2;
             const uint32_t smem0 = smem_u32(smem);
             for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-                const TileAt at = tile_at<BN>(q, product, t);
+                const TileAt at = tile_at(q, product, t);
                 for (int k = at.k0; k < at.k1; k++, n++) {
                     const int s = n % S::kCount, in_segment = SPLIT ? (k - at.k0) % kSegment : k - at.k0;
-                    const uint32_t d = tmem + (accs & 1) * BN;
+                    const uint32_t d = tmem + (accs & 1) * S::kBn;
                     named_bar_sync(kTiledBar, 64);
                     tc_fence_after();
                     const uint64_t ah = smem_desc(smem0 + s * S::kBytes, 0, 1024, kLayoutSw128);
@@ -1117,83 +1135,106 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
             }
         } else if (warp >= 4) {
             const int r = (warp & 3) * 32 + lane;
-            constexpr int kCols = BN / 2;          // of this warp: four warps share the rows, two the columns
-            const int c_first = ((warp - 4) >> 2) * kCols;
+            // four warps share the rows, two the columns: `share` of them from c_first on, 32 at a time
+            const int share = bn / 2, c_first = ((warp - 4) >> 2) * share;
             for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-                const TileAt at = tile_at<BN>(q, product, t);
+                const TileAt at = tile_at(q, product, t);
                 const Job& j = q.job[at.job];
+                const bool part = product == kGram && j.splits > 1;
                 // accumulator times: X X^T 2^2p -> A 2^14;  A A 2^28 -> 2^14;  B X 2^(14 + p) -> X 2^p
-                const float f = product == kGram ? exp2f((float)(kGramExp - 2 * j.p))
-                                                 : exp2f((float)-kGramExp) * (product == kSquare ? kNsC : 1.0f);
-                const float out_f = exp2f((float)-j.p);
-                // 32 columns from c on of this thread's row
-                auto emit = [&](int c, float* v) {
-                    if (product == kGram && j.splits > 1) {
-                        float4* part = reinterpret_cast<float4*>(
-                            q.parts + (long)(j.part0 + (at.j * j.rb + at.i) * j.splits + at.split) * (kTile * kTile) +
-                            r * kTile + c);
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            __stcg(part + k, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
-                        return;
-                    }
-                    const int bj = at.j * (BN / 128) + (c >> 7);      // 128-column block
-                    if (product == kApply ? 2 * bj >= j.cb : bj < at.i || bj >= j.rb) return;
+                const float f = part ? 1.0f
+                                : product == kGram
+                                    ? exp2f((float)(kGramExp - 2 * j.p))
+                                    : exp2f((float)-kGramExp) * (product == kSquare ? kNsC : 1.0f);
+                const float g = product == kSquare ? kNsB : kNsA, out_f = exp2f((float)-j.p);
+                const int cb = product == kApply ? j.cb : 2 * j.rb;
+                const uint8_t* old = product == kSquare ? j.a : j.x[src];
+                const long lo = product == kApply ? j.x_bytes : j.a_bytes;
+                uint8_t* dst = product == kGram ? j.a : product == kSquare ? j.b : j.x[src ^ 1];
+                // whether the 32 columns from c on are wanted, and where they are in the tiles
+                auto wanted = [&](int c) {
+                    const int bj = (at.j * bn + c) >> 7;
+                    return bj < cb / 2 && !(q.upper[product] && bj < at.i);
+                };
+                auto offset = [&](int c) {
+                    return ((long)at.i * cb + ((at.j * bn + c) >> 6)) * kTileBytes + r * 128;
+                };
+                // v: 32 columns from c on of the accumulator; x: the old operand's
+                auto emit = [&](int c, float* v, const OldBits<SPLIT>& x) {
 #pragma unroll
                     for (int k = 0; k < 32; k++) v[k] *= f;
-                    const int cb = product == kApply ? j.cb : 2 * j.rb;
-                    const int cc = c & 127, chunk = (cc & 63) >> 3;
-                    const long off = ((long)at.i * cb + 2 * bj + (cc >> 6)) * kTileBytes + r * 128;
-                    if (product != kGram) {
-                        float x[32];
-                        read32<SPLIT>((product == kSquare ? j.a : j.x[src]) + off,
-                                      product == kSquare ? j.a_bytes : j.x_bytes, r, chunk, x);
-                        const float g = product == kSquare ? kNsB : kNsA;
+                    if (part) {
+                        const int tile = ((at.j * bn) >> 7) * j.rb + at.i;
+                        float4* to = reinterpret_cast<float4*>(
+                            q.parts + ((long)(j.tile0[kGram] + tile * j.splits + at.split) * kTile + r) * kTile +
+                            ((at.j * bn) & 127) + c);
 #pragma unroll
-                        for (int k = 0; k < 32; k++) v[k] += g * x[k];
+                        for (int k = 0; k < 8; k++)
+                            __stcg(to + k, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
+                        return;
                     }
+                    if (product != kGram) add_old<SPLIT>(v, g, x);
+                    const int col = at.j * bn + c;
                     if (last) {
 #pragma unroll
                         for (int k = 0; k < 32; k++) v[k] *= out_f;
-                        finish16(q, j, at.i * kTile + (r & ~31), bj * kTile + cc, v, bad);
-                        finish16(q, j, at.i * kTile + (r & ~31), bj * kTile + cc + 16, v + 16, bad);
+                        finish16(q, j, at.i * kTile + (r & ~31), col, v, bad);
+                        finish16(q, j, at.i * kTile + (r & ~31), col + 16, v + 16, bad);
                         return;
                     }
-                    uint8_t* dst = product == kGram ? j.a : product == kSquare ? j.b : j.x[src ^ 1];
-                    uint8_t* mirror = product != kApply && bj > at.i
+                    const int bj = col >> 7;
+                    uint8_t* mirror = q.upper[product] && bj > at.i
                                           ? dst + ((long)bj * cb + 2 * at.i + (r >> 6)) * kTileBytes
                                           : nullptr;
-                    write32<SPLIT>(dst + off, product == kApply ? j.x_bytes : j.a_bytes, r, chunk, v, mirror, cc);
+                    write32<SPLIT>(dst + offset(c), lo, r, (col & 63) >> 3, v, mirror, col & 127);
                 };
+                // the old operand's values are fetched while the accumulator is still being filled
+                OldBits<SPLIT> x[2];
+                if (product != kGram) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        if (32 * h < share && wanted(c_first + 32 * h))
+                            x[h].load(old + offset(c_first + 32 * h), lo, r, ((c_first + 32 * h) & 63) >> 3);
+                }
                 if (SPLIT) {
-                    float acc[kCols];
+                    float acc[S::kBn / 2];
                     const int segments = (at.k1 - at.k0 + kSegment - 1) / kSegment;
-                    for (int g = 0; g < segments; g++, accs++) {
+                    for (int m = 0; m < segments; m++, accs++) {
                         if (ok) ok = mbar_wait(&tfull[accs & 1], (accs >> 1) & 1, q.status, kStatusWait);
                         tc_fence_after();
-                        const uint32_t d = tmem + (accs & 1) * BN + c_first + ((uint32_t)((warp & 3) * 32) << 16);
+                        const uint32_t d = tmem + (accs & 1) * S::kBn + c_first + ((uint32_t)((warp & 3) * 32) << 16);
 #pragma unroll
-                        for (int c = 0; c < kCols; c += 16) {
-                            float v[16];
-                            tmem_ld16(d + c, v);
+                        for (int c = 0; c < S::kBn / 2; c += 32) {
+                            float v[32];
+                            if (c >= share) continue;
+                            tmem_ld32(d + c, v);
 #pragma unroll
-                            for (int k = 0; k < 16; k++) acc[c + k] = g ? acc[c + k] + v[k] : v[k];
+                            for (int k = 0; k < 32; k++) acc[c + k] = m ? acc[c + k] + v[k] : v[k];
                         }
                         tc_fence_before();
                         mbar_arrive(&tempty[accs & 1]);
                     }
 #pragma unroll
-                    for (int c = 0; c < kCols; c += 32) emit(c_first + c, acc + c);
+                    for (int h = 0; h < 2; h++)
+                        if (32 * h < share && wanted(c_first + 32 * h)) emit(c_first + 32 * h, acc + 32 * h, x[h]);
                 } else {
                     if (ok) ok = mbar_wait(&tfull[accs & 1], (accs >> 1) & 1, q.status, kStatusWait);
                     tc_fence_after();
-                    const uint32_t d = tmem + (accs & 1) * BN + ((uint32_t)((warp & 3) * 32) << 16);
+                    const uint32_t d = tmem + (accs & 1) * S::kBn + ((uint32_t)((warp & 3) * 32) << 16);
 #pragma unroll 1
-                    for (int c = c_first; c < c_first + kCols; c += 32) {
-                        float v[32];
-                        __syncwarp();
-                        tmem_ld32(d + c, v);
-                        emit(c, v);
+                    for (int c = c_first; c < c_first + share; c += 64) {
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int cc = c + 32 * h;
+                            if (cc >= c_first + share || !wanted(cc)) continue;
+                            float v[32];
+                            __syncwarp();
+                            tmem_ld32(d + cc, v);
+                            emit(cc, v, x[h]);
+                            // the same half of the next 64 columns
+                            if (product != kGram && cc + 64 < c_first + share && wanted(cc + 64))
+                                x[h].load(old + offset(cc + 64), lo, r, ((cc + 64) & 63) >> 3);
+                        }
                     }
                     tc_fence_before();
                     mbar_arrive(&tempty[accs & 1]);
@@ -1210,7 +1251,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
     __syncthreads();
     if (warp == 3) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * BN);
+        tmem_dealloc(tmem, 2 * S::kBn);
     }
 }
 
@@ -1241,11 +1282,11 @@ int scale_exponent(const Shape& s) {
     return std::min(15, (int)std::floor(0.5 * std::log2((double)s.r * s.c)));
 }
 
-template <bool SPLIT, int BN, int N>
+template <bool SPLIT, int N>
 void launch_tiled(const Jobs<N>& q, cudaStream_t stream) {
-    using S = Stages<SPLIT, BN>;
+    using S = Stages<SPLIT>;
     static PerDeviceOnce once;
-    once_per_device(once, [] { set_max_dynamic_smem(tiled_kernel<SPLIT, BN, N>, S::kSmem, "tiled_kernel"); });
+    once_per_device(once, [] { set_max_dynamic_smem(tiled_kernel<SPLIT, N>, S::kSmem, "tiled_kernel"); });
     const cudaError_t e = cudaMemsetAsync(q.barrier, 0, sizeof(uint32_t), stream);
     if (e != cudaSuccess) throw std::runtime_error(std::string("cudaMemsetAsync: ") + cudaGetErrorString(e));
     cudaLaunchConfig_t cfg{};
@@ -1258,8 +1299,16 @@ void launch_tiled(const Jobs<N>& q, cudaStream_t stream) {
     attr[0].val.cooperative = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, tiled_kernel<SPLIT, BN, N>, q);
+    cudaLaunchKernelEx(&cfg, tiled_kernel<SPLIT, N>, q);
     launch_check("tiled_kernel");
+}
+
+// Tiles of a product: all of them, or those that reach above the diagonal.
+int tile_count(const Shape& s, int product, int bn, bool upper) {
+    if (!upper) return s.rb * (((product == kApply ? s.cb : 2 * s.rb) * 64 + bn - 1) / bn);
+    int n = 0;
+    for (int c = 0; c * bn < s.rb * 128; c++) n += std::min(bn / 128 * (c + 1), s.rb);
+    return n;
 }
 
 template <bool SPLIT, int N>
@@ -1270,21 +1319,37 @@ void run_tiled(const Settings& set, const std::vector<Source>& list, uint8_t* wo
     q.norms = reinterpret_cast<double*>(workspace + kControlBytes);
     q.parts = reinterpret_cast<float*>(workspace + kControlBytes + kNormBytes);
     uint8_t* at = workspace + kControlBytes + kNormBytes + kPartBytes;
-    int narrow = 0, full = 0;   // tiles of 128 x 128 of all X X^T: upper triangles, and all of them
-    for (const Source& s : list) {
-        const Shape shape(s.r, s.c);
-        narrow += shape.rb * (shape.rb + 1) / 2;
-        full += shape.rb * shape.rb;
-    }
+    std::vector<Shape> shapes;
+    for (const Source& source : list) shapes.emplace_back(source.r, source.c);
     const int sms = std::min(device_sms(), kMaxSms);
-    // Single fp16 operands are bound by the copies into shared memory, which 128 x 256 tiles cut by a quarter; they
-    // pay once every SM has several of them.  Pairs do three products per copy and need 128 columns' registers.
-    const bool wide = !SPLIT && narrow >= 4 * sms;
-    const int bn = wide ? 256 : 128;
-    for (const Source& source : list) {
-        const Shape s(source.r, source.c);
+    int grams = 0;   // 128 x 128 tiles of all X X^T
+    for (const Shape& s : shapes) grams += s.rb * s.rb;
+    // Split X X^T while its tiles leave SMs idle, in parts of four stages at least.
+    std::vector<int> splits;
+    for (const Shape& s : shapes) splits.push_back(std::max(1, std::min(sms / grams, (s.c + 63) / 64 / 4)));
+    const bool any_split = *std::max_element(splits.begin(), splits.end()) > 1;
+    for (int p = 0; p < 3; p++) {
+        double least = 1e300;
+        for (int upper = 0; upper < (p == kApply ? 1 : 2); upper++)
+            for (int bn = upper ? 128 : 64; bn <= Stages<SPLIT>::kBn; bn *= 2) {
+                // split products use 128-column tiles and all of them
+                if (p == kGram && any_split && (upper || bn != 128)) continue;
+                // A stage is bound by its bytes at about 63 per cycle; a tile adds its start and its epilogue.
+                double work = 0, longest = 0;
+                for (const Shape& s : shapes) {
+                    const double stages = (p == kGram ? s.c : s.r) / 64.0;
+                    const double tile = stages * (kTileBytes + bn * 128) * (SPLIT ? 2 : 1) / 63 + 1500 + 10.0 * bn;
+                    work += tile * tile_count(s, p, bn, upper);
+                    longest = std::max(longest, tile);
+                }
+                const double t = std::max(work / sms + longest / 2, longest);
+                if (t < least) least = t, q.bn[p] = bn, q.upper[p] = upper;
+            }
+    }
+    for (size_t i = 0; i < list.size(); i++) {
+        const Shape& s = shapes[i];
         Job& j = q.job[q.count++];
-        static_cast<Source&>(j) = source;
+        static_cast<Source&>(j) = list[i];
         j.rb = s.rb, j.cb = s.cb;
         j.x_bytes = s.x_bytes, j.a_bytes = s.a_bytes;
         const int halves = SPLIT ? 2 : 1;
@@ -1293,39 +1358,52 @@ void run_tiled(const Settings& set, const std::vector<Source>& list, uint8_t* wo
         j.a = j.x[1] + halves * s.x_bytes;
         j.b = j.a + halves * s.a_bytes;
         at = j.b + halves * s.a_bytes;
-        // split X X^T while its tiles leave SMs idle, in parts of four stages at least
-        j.splits = std::max(1, std::min(sms / std::max(1, full), ((s.c + 63) / 64) / 4));
-        j.pack0 = q.packs, j.gram0 = q.grams, j.square0 = q.squares, j.apply0 = q.applies, j.sum0 = q.sums;
-        j.part0 = q.grams;      // read only where splits > 1, when every X X^T unit has a part
-        const int triangle = bn == 128 ? s.rb * (s.rb + 1) / 2 : [&] {
-            int n = 0;
-            for (int c = 0; 2 * c < s.rb; c++) n += std::min(2 * c + 2, s.rb);
-            return n;
-        }();
+        j.splits = splits[i];
+        j.pack0 = q.packs, j.sum0 = q.sums;
         q.packs += s.rb * s.cb;
-        q.grams += j.splits > 1 ? s.rb * s.rb * j.splits : triangle;
-        q.squares += triangle;
-        q.applies += s.rb * ((s.cb * 64 + bn - 1) / bn);
+        for (int p = 0; p < 3; p++) {
+            j.tile0[p] = q.tiles[p];
+            q.tiles[p] += tile_count(s, p, q.bn[p], q.upper[p]) * (p == kGram ? j.splits : 1);
+        }
         if (j.splits > 1) q.sums += s.rb * s.rb * kTile * kTile / 8;
     }
-    if constexpr (!SPLIT) {
-        if (wide) return launch_tiled<false, 256, N>(q, stream);
-    }
-    launch_tiled<SPLIT, 128, N>(q, stream);
+    launch_tiled<SPLIT, N>(q, stream);
 }
 
-// CTAs a matrix takes on the cluster path (a power of two up to 8), 0 where it does not fit.  One per 64 columns,
-// which shortens every pass over X, but no more than 128 / matrices where they fit: 128 CTAs is what clusters of eight
-// with one CTA per SM can hold at a time (two in each of the GPU's eight groups of SMs).
-int slab_ranks(const Shape& s, bool split, size_t matrices) {
+// Fewest CTAs (a power of two up to 8) whose shared memory holds a matrix, 0 where none does.
+int slab_ranks(const Shape& s, bool split) {
     if (s.r > 128) return 0;
     const int rows = (s.r + 15) / 16 * 16;
     for (int ranks = 1; ranks <= 8; ranks *= 2) {
         const int width = (s.c + 64 * ranks - 1) / (64 * ranks) * 64;
-        if (slab_smem(rows, width, ranks, split) > kMaxSmem - 1024) continue;
-        if (ranks == 8 || width == 64 || 2 * ranks * matrices > 128) return ranks;
+        if (slab_smem(rows, width, ranks, split) <= kMaxSmem - 1024) return ranks;
     }
     return 0;
+}
+
+void set_ranks(SlabJob& j, int ranks) {
+    j.ranks = ranks;
+    j.width = (j.c + 64 * ranks - 1) / (64 * ranks) * 64;
+}
+
+// Deals CTAs to the matrices of a launch.  Narrower slabs shorten every pass over X (64 x 576: 34 us on eight CTAs, 74 on
+// one), so the matrix with the most elements per CTA is given twice as many as long as all matrices fit 128 CTAs, which
+// is what clusters of eight with one CTA per SM can hold at a time (two in each of the GPU's eight groups of SMs).
+void deal_ranks(std::vector<SlabJob>& jobs) {
+    int total = 0;
+    for (const SlabJob& j : jobs) total += j.ranks;
+    for (;;) {
+        SlabJob* most = nullptr;
+        for (SlabJob& j : jobs) {
+            SlabJob more = j;
+            set_ranks(more, 2 * j.ranks);
+            if (j.ranks == 8 || total + j.ranks > 128 || more.width == j.width) continue;
+            if (!most || (long)j.rows * j.width > (long)most->rows * most->width) most = &j;
+        }
+        if (!most) return;
+        total += most->ranks;
+        set_ranks(*most, 2 * most->ranks);
+    }
 }
 
 template <bool SPLIT, int N>
@@ -1367,21 +1445,21 @@ void run_sources(const Settings& set, const std::vector<Source>& list, void* wor
     for (const Source& s : list) {
         SlabJob j{};
         static_cast<Source&>(j) = s;
-        j.ranks = slab_ranks(Shape(s.r, s.c), SPLIT, list.size());
-        if (!j.ranks) {
+        const int ranks = slab_ranks(Shape(s.r, s.c), SPLIT);
+        if (!ranks) {
             tiled.push_back(s);
             continue;
         }
         j.rows = (s.r + 15) / 16 * 16;
-        j.width = (s.c + 64 * j.ranks - 1) / (64 * j.ranks) * 64;
+        set_ranks(j, ranks);
         slabs.push_back(j);
     }
-    std::stable_sort(slabs.begin(), slabs.end(), [](const SlabJob& a, const SlabJob& b) {
-        return a.ranks != b.ranks ? a.ranks > b.ranks : (long)a.rows * a.width > (long)b.rows * b.width;
-    });
     for (size_t first = 0; first < slabs.size(); first += kMaxJobs) {
-        const std::vector<SlabJob> part(slabs.begin() + first,
-                                        slabs.begin() + std::min<size_t>(slabs.size(), first + kMaxJobs));
+        std::vector<SlabJob> part(slabs.begin() + first, slabs.begin() + std::min<size_t>(slabs.size(), first + kMaxJobs));
+        deal_ranks(part);
+        std::stable_sort(part.begin(), part.end(), [](const SlabJob& a, const SlabJob& b) {
+            return a.ranks != b.ranks ? a.ranks > b.ranks : (long)a.rows * a.width > (long)b.rows * b.width;
+        });
         if (part.size() == 1)
             launch_slabs<SPLIT, 1>(set, part, stream);
         else
@@ -1399,11 +1477,11 @@ void run_sources(const Settings& set, const std::vector<Source>& list, void* wor
 }
 
 // Workspace of a call.  Matrices on the cluster path need none; whether a shape takes it does not depend on the rest of
-// the list (slab_ranks tries clusters up to eight for any), so a call with part of a list's matrices needs no more.
+// the list, so a call with part of a list's matrices needs no more.
 size_t workspace_bytes(const std::vector<Shape>& shapes, bool split) {
     long sum = 0;
     for (const Shape& s : shapes)
-        if (!slab_ranks(s, split, 1)) sum += s.bytes(split);
+        if (!slab_ranks(s, split)) sum += s.bytes(split);
     return (size_t)(1024 + (sum ? kControlBytes + kNormBytes + kPartBytes + sum : 0));
 }
 
