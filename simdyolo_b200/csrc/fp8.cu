@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(256)
 
 constexpr int kTileRows = 128, kBlockK = 128;
 constexpr int kScaleSlots = 4;   // groups of four K blocks whose scale words are in flight
-constexpr int kThreads = 256;    // TMA, MMA, scales, MMA-side waits, then four epilogue warps
+// Warps: 0, 8 and 9 TMA, 1 MMA, 2 scales, 3 MMA-side waits, 4-7 epilogue.
+constexpr int kThreads = 320, kProducers = 3;
 constexpr int kStageBar = 1;     // named barrier: a stage is loaded (the waiting warp and the MMA warp)
 
 struct ProductParams {
@@ -310,14 +311,9 @@ struct ProductShape {
     static_assert(BN * 129 * 4 <= kStages * kStageBytes, "partial tile exceeds the stages");
 };
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
 __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-    uint32_t a;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_addr(addr, rank)) : "memory");
     return v;
 }
 
@@ -416,20 +412,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0) {
+    if (warp == 0 || warp >= 8) {
+        // The producers take turns.  A wait after a bulk copy holds a thread for ~1,000 cycles, whatever it waits for, more
+        // than a stage's copies or MMAs take.  The first stages are free and need no wait.
         if (lane == 0) {
-            int i = 0;
-            for (; i < k1 - k0; i++) {
+            const int mine = warp ? warp - 7 : 0;
+            int i = mine;
+            for (; i < k1 - k0; i += kProducers) {
                 const int s = i % S::kStages;
-                if (!mbar_wait(&empty[s], ((i / S::kStages) & 1) ^ 1, p.status, kStatusWait)) break;
+                if (i >= S::kStages && !mbar_wait(&empty[s], ((i / S::kStages) & 1) ^ 1, p.status, kStatusWait)) break;
                 uint8_t* st = smem + s * S::kStageBytes;
                 mbar_arrive_expect_tx(&full[s], S::kStageBytes);
                 tma_load_2d(st, &tm_a, &full[s], (k0 + i) * kBlockK, m0);
                 tma_load_2d(st + kTileRows * kBlockK, &tm_b, &full[s], (k0 + i) * kBlockK, n0);
             }
-            // no copy is in flight when the CTA ends, even after a wait that gave up
-            for (int j = max(0, i - S::kStages); j < i; j++)
-                mbar_wait(&full[j % S::kStages], (j / S::kStages) & 1, p.status, kStatusWait);
+            // No copy is in flight when the CTA ends, even after a wait that gave up.  Only the last use of a stage is
+            // waited for: the barrier of an earlier one may have moved on by two phases.
+            for (int j = mine; j < min(i, k1 - k0); j += kProducers)
+                if (j + S::kStages >= k1 - k0) mbar_wait(&full[j % S::kStages], (j / S::kStages) & 1, p.status, kStatusWait);
         }
     } else if (warp == 3) {
         // every wait of the MMA side; after one that gave up the hand-offs go on, so that every warp finishes
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncwarp();
-    if (warp >= 4) {
+    if (warp >= 4 && warp < 8) {
         const int q = warp & 3, r = q * 32 + lane, i = m0 + r;
         mbar_wait(done, 0, p.status, kStatusWait);
         tc_fence_after();
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
     }
     if (p.splits > 1) {
-        cluster_sync();
+        cluster_sync_all();
         const int share = kTileRows / p.splits, first = split * share;
         const uint32_t part = smem_u32(smem);
         for (int idx = threadIdx.x; idx < share * BN; idx += kThreads) {
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int s = 0; s < p.splits; s++) v += ld_cluster(part + (c * 129 + r) * 4, s);
             put(p, m0 + r, n0 + c, v);
         }
-        cluster_sync();   // a peer may still read this CTA's partial tile
+        cluster_sync_all();   // a peer may still read this CTA's partial tile
     } else {
         __syncthreads();
     }

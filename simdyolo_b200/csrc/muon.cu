@@ -264,14 +264,6 @@ int slab_smem(int rows, int width, int ranks, bool split) {
     return 1024 + std::max(tiles + (ranks > 1 ? slab_part_bytes(rows) : 0), tiles - rows * 128 + 128 * 128);
 }
 
-__device__ __forceinline__ void slab_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    return a;
-}
 __device__ __forceinline__ float4 peer_load4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -441,14 +433,12 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
     while (index < q.count && (int)blockIdx.x >= q.job[index].first + q.job[index].ranks) index++;
     if (index == q.count || (int)blockIdx.x < q.job[index].first) {
         // a cluster's CTA without a matrix takes part in its barriers
-        for (int i = 0; i < 2 + 2 * q.steps; i++) slab_cluster_sync();
+        for (int i = 0; i < 2 + 2 * q.steps; i++) cluster_sync_all();
         return;
     }
     const SlabJob& j = q.job[index];
     const int ranks = j.ranks, rank = blockIdx.x - j.first;
-    uint32_t peer0;                  // the matrix's first CTA within the cluster
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(peer0));
-    peer0 -= rank;
+    const uint32_t peer0 = cluster_rank() - rank;                  // the matrix's first CTA within the cluster
     const int rows = j.rows, col0 = rank * j.width;
     const int cols = min(j.width, max(0, j.c - col0));            // this CTA's columns, and as whole tiles
     const int tiles = (cols + 63) / 64;
@@ -487,7 +477,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         for (int w = 0; w < kSlabThreads / 32; w++) t += red[w];
         norm = t;
     }
-    slab_cluster_sync();
+    cluster_sync_all();
     const double part_norm = lane < ranks ? peer_load_d(peer_addr(smem_u32(&norm), peer0 + lane)) : 0.0;
     s = 0.0;
     for (int i = 0; i < ranks; i++) s += __shfl_sync(0xffffffffu, part_norm, i);
@@ -553,7 +543,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
             fence_proxy_async();
             __syncthreads();
         }
-        slab_cluster_sync();
+        cluster_sync_all();
         // A = the sum over the cluster: this CTA's share of the rows, handed to everyone.  Each CTA begins with another
         // peer, so the order of a sum depends on the row alone.
         const int share = rows / ranks, chunks = rows / 8;
@@ -585,7 +575,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
             }
         }
         asm volatile("fence.proxy.async;" ::: "memory");
-        slab_cluster_sync();
+        cluster_sync_all();
         // B = b A + c A^2, over A
         if (tid == 0) {
             asm volatile("fence.proxy.async;" ::: "memory");
@@ -655,7 +645,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         }
     }
     if (bad && q.status) atomicExch(q.status, kStatusNonFinite);
-    slab_cluster_sync();   // no CTA leaves while a peer may read its shared memory
+    cluster_sync_all();   // no CTA leaves while a peer may read its shared memory
     if (warp == 0) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -681,11 +671,12 @@ struct Job : Source {
     // first unit of this matrix in: packing (128 x 64 tiles), each product, and the sum of the split X X^T (16-byte
     // pieces)
     int pack0, tile0[3], sum0;
+    int part0;                  // and its first part (128 x 128 floats), splits per tile
 };
 template <int N>
 struct Jobs : Settings {
     int count;
-    int packs, sums;                            // units of packing and of the sum of split products
+    int packs, sums, parts_used;                // units of packing and of the sum of split products, parts
     int tiles[3], bn[3], upper[3];              // of each product: units, tile columns, upper triangle only
     double* norms;                              // [count][gridDim]
     float* parts;
@@ -700,12 +691,14 @@ constexpr int kTiledThreads = 32 * (4 + kEpilogueWarps);
 constexpr int kTiledBar = 1;                   // a stage is loaded: the waiting warp and the MMA warp
 constexpr int kSegment = 8;                    // stages (of 64 along K) per accumulator of pairs
 
-// Widest tile: single fp16 operands are bound by the copies into shared memory, which wider tiles cut; pairs do three
-// products per copy, and their sums in registers allow 128 columns.
+// A tile is 128 rows by up to kBn columns.  Pairs of fp16 keep two accumulators per tile: hi hi, and the cross products,
+// whose additions would otherwise truncate the hi hi sum twice as often; with their sums in registers that leaves
+// 128 columns.
 template <bool SPLIT>
 struct Stages {
     static constexpr int kBn = SPLIT ? 128 : 256;
-    static constexpr int kHalf = kTileBytes + kBn / 128 * kTileBytes;   // hi operands, then lo operands
+    static constexpr int kAccCols = 256;                             // TMEM columns of an accumulator (set)
+    static constexpr int kHalf = kTileBytes + kBn * 128;   // hi operands, then lo operands
     static constexpr int kBytes = (SPLIT ? 2 : 1) * kHalf;
     static constexpr int kCount = 196608 / kBytes;
     static constexpr int kSmem = 1024 + kCount * kBytes + (2 * kCount + 4) * 8 + 16;
@@ -727,24 +720,26 @@ __device__ __forceinline__ TileAt tile_at(const Jobs<N>& q, int product, int t) 
     a.k0 = 0;
     a.k1 = ((product == kGram ? j.c : j.r) + 63) / 64;
     int u = t - j.tile0[product];
-    if (q.upper[product]) {   // the tiles that reach above the diagonal, by columns
-        const int w = q.bn[product] >> 7;          // column j holds row blocks 0 .. w (j + 1) - 1
-        int c = (int)((sqrtf(8.0f / w * u + 1.0f) - 1.0f) * 0.5f);
-        while (w * c * (c + 1) / 2 > u) c--;
-        while (w * (c + 1) * (c + 2) / 2 <= u) c++;
+    if (q.upper[product]) {
+        // the tiles that reach above the diagonal, by columns: column c holds the first w (c + 1) row blocks
+        const int w = q.bn[product] >> 7;
+        auto before = [&](int c) { return w * c * (c + 1) / 2; };
+        int c = (int)sqrtf(2.0f * u / w);
+        while (before(c) > u) c--;
+        while (before(c + 1) <= u) c++;
         a.j = c;
-        a.i = u - w * c * (c + 1) / 2;
-        return a;
+        a.i = u - before(c);
+    } else {
+        if (product == kGram && j.splits > 1) {
+            const int all = a.k1;
+            a.split = u % j.splits;
+            u /= j.splits;
+            a.k0 = (int)((long)all * a.split / j.splits);
+            a.k1 = (int)((long)all * (a.split + 1) / j.splits);
+        }
+        a.j = u / j.rb;
+        a.i = u - a.j * j.rb;
     }
-    if (product == kGram && j.splits > 1) {
-        const int all = a.k1;
-        a.split = u % j.splits;
-        u /= j.splits;
-        a.k0 = (int)((long)all * a.split / j.splits);
-        a.k1 = (int)((long)all * (a.split + 1) / j.splits);
-    }
-    a.j = u / j.rb;
-    a.i = u - a.j * j.rb;
     return a;
 }
 
@@ -944,7 +939,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
         s_ok = 1;
     }
     if (warp == 3) {
-        tmem_alloc(tmem_slot, 2 * S::kBn);
+        tmem_alloc(tmem_slot, 2 * S::kAccCols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -1015,7 +1010,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                 while (k > 0 && u < q.job[k].sum0) k--;
                 const Job& j = q.job[k];
                 const int e = (int)(u - j.sum0), tile = e >> 11, row = (e >> 4) & 127, col = (e & 15) * 8;
-                const float* from = q.parts + (long)(j.tile0[kGram] + tile * j.splits) * (kTile * kTile) + row * kTile + col;
+                const float* from = q.parts + (long)(j.part0 + tile * j.splits) * (kTile * kTile) + row * kTile + col;
                 float v[8] = {};
                 for (int s = 0; s < j.splits; s++) {
                     const float4 f = __ldcg(reinterpret_cast<const float4*>(from + (long)s * kTile * kTile));
@@ -1039,7 +1034,10 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
         const int product = phase == 0 ? kGram : phase == 2 ? kSquare : kApply;
         const bool last = product == kApply && (step >> 2) + 1 == q.steps;
         const int tiles = q.tiles[product], bn = q.bn[product];
-        if (warp == 0) {
+        if (warp == 0 || warp == 3) {
+            // The two producers take turns.  A wait after a bulk copy holds a thread for ~1,000 cycles, whatever it waits
+            // for; alternating halves that per stage.  The first stages of a phase need no wait: the phase before has
+            // used up every stage.
             if (lane == 0) {
                 const int first = n;
                 asm volatile("fence.proxy.async;" ::: "memory");   // what the barrier made visible, to bulk copies too
@@ -1050,11 +1048,15 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                     const long left_lo = product == kGram ? j.x_bytes : j.a_bytes;
                     const int lcb = product == kGram ? j.cb : 2 * j.rb;
                     // the columns' operand in pieces of 64, those that exist: column blocks of X, halves of row blocks
-                    const int per = bn / 64, pieces = min(per, (product == kApply ? j.cb : 2 * j.rb) - at.j * per);
                     constexpr int kPiece = kTileBytes / 2;
+                    const int per = bn / 64, at64 = at.j * per;
+                    const int pieces = min(per, (product == kApply ? j.cb : 2 * j.rb) - at64);
                     for (int k = at.k0; k < at.k1; k++, n++) {
+                        if ((n & 1) != (warp == 3)) continue;
                         const int s = n % S::kCount;
-                        if (!(ok = mbar_wait(&empty[s], ((n / S::kCount) & 1) ^ 1, q.status, kStatusWait))) break;
+                        if (n - first >= S::kCount &&
+                            !(ok = mbar_wait(&empty[s], ((n / S::kCount) & 1) ^ 1, q.status, kStatusWait)))
+                            break;
                         uint8_t* st = smem + s * S::kBytes;
                         mbar_arrive_expect_tx(&full[s], (kTileBytes + pieces * kPiece) * (SPLIT ? 2 : 1));
                         const uint8_t* a = left + ((long)at.i * lcb + k) * kTileBytes;
@@ -1062,8 +1064,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                         if (SPLIT) bulk_load(st + S::kHalf, a + left_lo, kTileBytes, &full[s]);
                         if (product == kApply) {
                             // 64 rows of neighbouring column blocks of X
-                            const uint8_t* b =
-                                j.x[src] + ((long)(k >> 1) * j.cb + at.j * per) * kTileBytes + (k & 1) * kPiece;
+                            const uint8_t* b = j.x[src] + ((long)(k >> 1) * j.cb + at64) * kTileBytes + (k & 1) * kPiece;
                             for (int h = 0; h < pieces; h++) {
                                 bulk_load(st + kTileBytes + h * kPiece, b + h * kTileBytes, kPiece, &full[s]);
                                 if (SPLIT)
@@ -1073,9 +1074,9 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                         } else {
                             // neighbouring row blocks, or half of one
                             for (int h = 0; h < pieces; h += 2) {
-                                const int at64 = at.j * per + h, bytes = min(2, pieces - h) * kPiece;
-                                const uint8_t* b =
-                                    left + ((long)(at64 >> 1) * lcb + k) * kTileBytes + (at64 & 1) * kPiece;
+                                const int bytes = min(2, pieces - h) * kPiece;
+                                const uint8_t* b = left + ((long)((at64 + h) >> 1) * lcb + k) * kTileBytes +
+                                                   ((at64 + h) & 1) * kPiece;
                                 bulk_load(st + kTileBytes + h * kPiece, b, bytes, &full[s]);
                                 if (SPLIT)
                                     bulk_load(st + S::kHalf + kTileBytes + h * kPiece, b + left_lo, bytes, &full[s]);
@@ -1085,7 +1086,8 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                 }
                 // no copy is in flight when the CTA ends, even after a wait that gave up
                 for (int i = max(first, n - S::kCount); i < n; i++)
-                    ok &= mbar_wait(&full[i % S::kCount], (i / S::kCount) & 1, q.status, kStatusWait);
+                    if ((i & 1) == (warp == 3))
+                        ok &= mbar_wait(&full[i % S::kCount], (i / S::kCount) & 1, q.status, kStatusWait);
                 if (!ok) s_ok = 0;
             }
         } else if (warp == 2) {
@@ -1093,11 +1095,12 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
             for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
                 const TileAt at = tile_at(q, product, t);
                 for (int k = at.k0; k < at.k1; k++, n++) {
+                    const int s = n % S::kCount, parity = (n / S::kCount) & 1;
                     if (k == at.k0 || (SPLIT && (k - at.k0) % kSegment == 0)) {
                         if (ok) ok = mbar_wait(&tempty[accs & 1], ((accs >> 1) & 1) ^ 1, q.status, kStatusWait);
                         accs++;
                     }
-                    if (ok) ok = mbar_wait(&full[n % S::kCount], (n / S::kCount) & 1, q.status, kStatusWait);
+                    if (ok) ok = mbar_wait(&full[s], parity, q.status, kStatusWait);
                     named_bar_sync(kTiledBar, 64);
                 }
             }
@@ -1112,7 +1115,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                 const TileAt at = tile_at(q, product, t);
                 for (int k = at.k0; k < at.k1; k++, n++) {
                     const int s = n % S::kCount, in_segment = SPLIT ? (k - at.k0) % kSegment : k - at.k0;
-                    const uint32_t d = tmem + (accs & 1) * S::kBn;
+                    const uint32_t d = tmem + (accs & 1) * S::kAccCols;
                     named_bar_sync(kTiledBar, 64);
                     tc_fence_after();
                     const uint64_t ah = smem_desc(smem0 + s * S::kBytes, 0, 1024, kLayoutSw128);
@@ -1120,10 +1123,11 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                     constexpr uint64_t kLo = S::kHalf / 16;
 #pragma unroll
                     for (int kk = 0; kk < kChunk / 16; kk++) {
-                        mma_f16_elect(d, ah + 2 * kk, bh + step_b * kk, idesc, (in_segment | kk) != 0);
+                        const bool more = (in_segment | kk) != 0;
+                        mma_f16_elect(d, ah + 2 * kk, bh + step_b * kk, idesc, more);
                         if (SPLIT) {
-                            mma_f16_elect(d, ah + 2 * kk, bh + kLo + step_b * kk, idesc, 1);
-                            mma_f16_elect(d, ah + kLo + 2 * kk, bh + step_b * kk, idesc, 1);
+                            mma_f16_elect(d + S::kBn, ah + 2 * kk, bh + kLo + step_b * kk, idesc, more);
+                            mma_f16_elect(d + S::kBn, ah + kLo + 2 * kk, bh + step_b * kk, idesc, true);
                         }
                     }
                     mma_commit_elect(&empty[s]);
@@ -1156,6 +1160,11 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                     const int bj = (at.j * bn + c) >> 7;
                     return bj < cb / 2 && !(q.upper[product] && bj < at.i);
                 };
+                auto drained = [&] {   // this thread has read the accumulator
+                    tc_fence_before();
+                    mbar_arrive(&tempty[accs & 1]);
+                    accs++;
+                };
                 auto offset = [&](int c) {
                     return ((long)at.i * cb + ((at.j * bn + c) >> 6)) * kTileBytes + r * 128;
                 };
@@ -1166,7 +1175,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                     if (part) {
                         const int tile = ((at.j * bn) >> 7) * j.rb + at.i;
                         float4* to = reinterpret_cast<float4*>(
-                            q.parts + ((long)(j.tile0[kGram] + tile * j.splits + at.split) * kTile + r) * kTile +
+                            q.parts + ((long)(j.part0 + tile * j.splits + at.split) * kTile + r) * kTile +
                             ((at.j * bn) & 127) + c);
 #pragma unroll
                         for (int k = 0; k < 8; k++)
@@ -1199,20 +1208,23 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                 if (SPLIT) {
                     float acc[S::kBn / 2];
                     const int segments = (at.k1 - at.k0 + kSegment - 1) / kSegment;
-                    for (int m = 0; m < segments; m++, accs++) {
+                    for (int m = 0; m < segments; m++) {
                         if (ok) ok = mbar_wait(&tfull[accs & 1], (accs >> 1) & 1, q.status, kStatusWait);
                         tc_fence_after();
-                        const uint32_t d = tmem + (accs & 1) * S::kBn + c_first + ((uint32_t)((warp & 3) * 32) << 16);
+                        const uint32_t d = tmem + (accs & 1) * S::kAccCols + c_first + ((uint32_t)((warp & 3) * 32) << 16);
 #pragma unroll
-                        for (int c = 0; c < S::kBn / 2; c += 32) {
-                            float v[32];
+                        for (int c = 0; c < S::kBn / 2; c += 16) {
+                            float v[16], w[16];
                             if (c >= share) continue;
-                            tmem_ld32(d + c, v);
+                            tmem_ld16(d + c, v);
+                            tmem_ld16(d + S::kBn + c, w);
 #pragma unroll
-                            for (int k = 0; k < 32; k++) acc[c + k] = m ? acc[c + k] + v[k] : v[k];
+                            for (int k = 0; k < 16; k++) {
+                                v[k] += w[k];
+                                acc[c + k] = m ? acc[c + k] + v[k] : v[k];
+                            }
                         }
-                        tc_fence_before();
-                        mbar_arrive(&tempty[accs & 1]);
+                        drained();
                     }
 #pragma unroll
                     for (int h = 0; h < 2; h++)
@@ -1220,7 +1232,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                 } else {
                     if (ok) ok = mbar_wait(&tfull[accs & 1], (accs >> 1) & 1, q.status, kStatusWait);
                     tc_fence_after();
-                    const uint32_t d = tmem + (accs & 1) * S::kBn + ((uint32_t)((warp & 3) * 32) << 16);
+                    const uint32_t d = tmem + (accs & 1) * S::kAccCols + ((uint32_t)((warp & 3) * 32) << 16);
 #pragma unroll 1
                     for (int c = c_first; c < c_first + share; c += 64) {
 #pragma unroll
@@ -1236,9 +1248,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                                 x[h].load(old + offset(cc + 64), lo, r, ((cc + 64) & 63) >> 3);
                         }
                     }
-                    tc_fence_before();
-                    mbar_arrive(&tempty[accs & 1]);
-                    accs++;
+                    drained();
                 }
             }
             if (!ok) s_ok = 0;
@@ -1248,10 +1258,11 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
         ok = grid_barrier(q.barrier, ++turn, q.status, &s_ok);
     }
     if (bad && q.status) atomicExch(q.status, kStatusNonFinite);
+    tc_fence_before();
     __syncthreads();
     if (warp == 3) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * S::kBn);
+        tmem_dealloc(tmem, 2 * S::kAccCols);
     }
 }
 
@@ -1311,6 +1322,47 @@ int tile_count(const Shape& s, int product, int bn, bool upper) {
     return n;
 }
 
+// How the products of a call are tiled, by an estimate of the cycles they take.
+struct TilePlan {
+    int bn[3], upper[3];
+    std::vector<int> splits;
+};
+template <bool SPLIT>
+TilePlan plan_tiles(const std::vector<Shape>& shapes, int sms) {
+    TilePlan plan;
+    // A stage takes the longest of its producer's turn, its copies (about 90 bytes per cycle) and its MMAs (4,096
+    // multiply-adds per cycle); a tile adds its start and its epilogue.
+    auto stage = [&](int bn) {
+        return std::max({500.0, (SPLIT ? 2 : 1) * (kTileBytes + bn * 128) / 90.0, (SPLIT ? 3 : 1) * 2.0 * bn});
+    };
+    int grams = 0;
+    for (const Shape& s : shapes) grams += s.rb * s.rb;
+    for (const Shape& s : shapes) {
+        // X X^T is split while its tiles leave SMs idle, in parts of four stages at least, where the shorter K saves
+        // more than writing and adding the parts takes (about 9,000 cycles).
+        const int stages = (s.c + 63) / 64, most = std::max(1, std::min(sms / grams, stages / 4));
+        plan.splits.push_back((stages - (stages + most - 1) / most) * stage(128) > 9000 ? most : 1);
+    }
+    const bool any_split = *std::max_element(plan.splits.begin(), plan.splits.end()) > 1;
+    for (int p = 0; p < 3; p++) {
+        double least = 1e300;
+        for (int upper = 0; upper < (p == kApply ? 1 : 2); upper++)
+            for (int bn = upper ? 128 : 64; bn <= Stages<SPLIT>::kBn; bn *= 2) {
+                if (p == kGram && any_split && (upper || bn != 128)) continue;   // the parts are whole 128 x 128 tiles
+                double work = 0, longest = 0;
+                for (size_t i = 0; i < shapes.size(); i++) {
+                    const double stages = (p == kGram ? shapes[i].c / plan.splits[i] : shapes[i].r) / 64.0;
+                    const double tile = stages * stage(bn) + 1500 + 10.0 * bn;
+                    work += tile * tile_count(shapes[i], p, bn, upper) * (p == kGram ? plan.splits[i] : 1);
+                    longest = std::max(longest, tile);
+                }
+                const double t = std::max(work / sms + longest / 2, longest);
+                if (t < least) least = t, plan.bn[p] = bn, plan.upper[p] = upper;
+            }
+    }
+    return plan;
+}
+
 template <bool SPLIT, int N>
 void run_tiled(const Settings& set, const std::vector<Source>& list, uint8_t* workspace, cudaStream_t stream) {
     Jobs<N> q{};
@@ -1322,30 +1374,8 @@ void run_tiled(const Settings& set, const std::vector<Source>& list, uint8_t* wo
     std::vector<Shape> shapes;
     for (const Source& source : list) shapes.emplace_back(source.r, source.c);
     const int sms = std::min(device_sms(), kMaxSms);
-    int grams = 0;   // 128 x 128 tiles of all X X^T
-    for (const Shape& s : shapes) grams += s.rb * s.rb;
-    // Split X X^T while its tiles leave SMs idle, in parts of four stages at least.
-    std::vector<int> splits;
-    for (const Shape& s : shapes) splits.push_back(std::max(1, std::min(sms / grams, (s.c + 63) / 64 / 4)));
-    const bool any_split = *std::max_element(splits.begin(), splits.end()) > 1;
-    for (int p = 0; p < 3; p++) {
-        double least = 1e300;
-        for (int upper = 0; upper < (p == kApply ? 1 : 2); upper++)
-            for (int bn = upper ? 128 : 64; bn <= Stages<SPLIT>::kBn; bn *= 2) {
-                // split products use 128-column tiles and all of them
-                if (p == kGram && any_split && (upper || bn != 128)) continue;
-                // A stage is bound by its bytes at about 63 per cycle; a tile adds its start and its epilogue.
-                double work = 0, longest = 0;
-                for (const Shape& s : shapes) {
-                    const double stages = (p == kGram ? s.c : s.r) / 64.0;
-                    const double tile = stages * (kTileBytes + bn * 128) * (SPLIT ? 2 : 1) / 63 + 1500 + 10.0 * bn;
-                    work += tile * tile_count(s, p, bn, upper);
-                    longest = std::max(longest, tile);
-                }
-                const double t = std::max(work / sms + longest / 2, longest);
-                if (t < least) least = t, q.bn[p] = bn, q.upper[p] = upper;
-            }
-    }
+    const TilePlan plan = plan_tiles<SPLIT>(shapes, sms);
+    for (int p = 0; p < 3; p++) q.bn[p] = plan.bn[p], q.upper[p] = plan.upper[p];
     for (size_t i = 0; i < list.size(); i++) {
         const Shape& s = shapes[i];
         Job& j = q.job[q.count++];
@@ -1358,14 +1388,18 @@ void run_tiled(const Settings& set, const std::vector<Source>& list, uint8_t* wo
         j.a = j.x[1] + halves * s.x_bytes;
         j.b = j.a + halves * s.a_bytes;
         at = j.b + halves * s.a_bytes;
-        j.splits = splits[i];
+        j.splits = plan.splits[i];
         j.pack0 = q.packs, j.sum0 = q.sums;
         q.packs += s.rb * s.cb;
         for (int p = 0; p < 3; p++) {
             j.tile0[p] = q.tiles[p];
             q.tiles[p] += tile_count(s, p, q.bn[p], q.upper[p]) * (p == kGram ? j.splits : 1);
         }
-        if (j.splits > 1) q.sums += s.rb * s.rb * kTile * kTile / 8;
+        j.part0 = q.parts_used;
+        if (j.splits > 1) {
+            q.sums += s.rb * s.rb * kTile * kTile / 8;
+            q.parts_used += s.rb * s.rb * j.splits;
+        }
     }
     launch_tiled<SPLIT, N>(q, stream);
 }

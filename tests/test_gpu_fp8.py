@@ -112,7 +112,7 @@ def check(a, b, dtype, got, start=None):
 @pytest.mark.parametrize("m, n, k", [
     (1, 1, 1), (1, 16, 128), (1, 300, 1000), (2, 129, 127), (16, 128, 129), (17, 257, 513), (33, 1000, 2000),
     (65, 130, 4100), (127, 255, 640), (128, 128, 128), (129, 64, 200), (200, 33, 8000), (300, 1, 384), (513, 300, 256),
-    (1000, 1000, 700), (2300, 2500, 300)])
+    (1000, 1000, 700), (2300, 2500, 300), (1500, 5200, 2300), (2100, 4100, 640)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_product_sizes(m, n, k, dtype):
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
