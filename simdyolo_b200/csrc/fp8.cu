@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "kernels.h"
 
@@ -23,88 +24,99 @@ namespace {
 
 // ------------------------------------------------------------------ casts
 
-__device__ __forceinline__ float load_f(const float* p) { return *p; }
-__device__ __forceinline__ float load_f(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ float load_f(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ void store_f(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_f(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_f(__half* p, float v) { *p = __float2half_rn(v); }
 
-__device__ __forceinline__ void unpack(uint4 u, const __nv_bfloat16*, float* v) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void unpack(uint4 u, const __half*, float* v) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
-}
-__device__ __forceinline__ void unpack(uint4 u, const float*, float* v) {
-    v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
-}
-
-// 16 consecutive values of a row from column c; columns at and past `cols` read as zero.
+// 16 values of a row as they are stored, so that 16-bit types take 8 registers
 template <class T>
-__device__ __forceinline__ void load16(const T* row, int c, int cols, bool vec, float* v) {
-    if (vec && c + 16 <= cols) {
-        constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < 16 / kPer; i++)
-            unpack(__ldg(reinterpret_cast<const uint4*>(row + c) + i), row, v + i * kPer);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++) v[i] = c + i < cols ? load_f(row + c + i) : 0.0f;
-    }
-}
+struct Raw16 {
+    static constexpr int kWords = 4 * sizeof(T);
+    uint32_t w[kWords];
 
-// |v| of finite values, 0 for the others
-__device__ __forceinline__ float finite_size(float v) {
-    const float a = fabsf(v);
-    return a <= 3.402823466e38f ? a : 0.0f;
+    // from column c; columns at and past `cols` read as zero
+    __device__ __forceinline__ void load(const T* row, int c, int cols, bool vec) {
+        if (vec && c + 16 <= cols) {
+#pragma unroll
+            for (int i = 0; i < kWords / 4; i++) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+            }
+        } else if (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                w[i % kWords] = c + i < cols ? __ldg(reinterpret_cast<const uint32_t*>(row) + c + i) : 0u;
+        } else {
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t a = c + 2 * i < cols ? __ldg(p + c + 2 * i) : 0;
+                const uint32_t b = c + 2 * i + 1 < cols ? __ldg(p + c + 2 * i + 1) : 0;
+                w[i] = a | b << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) w[i] = 0;
+    }
+    __device__ __forceinline__ float get(int i) const;
+
+    // infinities become NaN, which maxima pass over
+    __device__ __forceinline__ void drop_infinities() {
+        constexpr uint32_t kInf = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+#pragma unroll
+        for (int i = 0; i < kWords; i++) {
+            if (sizeof(T) == 4) {
+                w[i] |= (w[i] & 0x7fffffffu) == kInf;
+            } else {
+                w[i] |= (w[i] & 0x7fffu) == kInf;
+                w[i] |= (uint32_t)((w[i] >> 16 & 0x7fffu) == kInf) << 16;
+            }
+        }
+    }
+};
+template <>
+__device__ __forceinline__ float Raw16<float>::get(int i) const {
+    return __uint_as_float(w[i]);
+}
+template <>
+__device__ __forceinline__ float Raw16<__nv_bfloat16>::get(int i) const {
+    return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+}
+template <>
+__device__ __forceinline__ float Raw16<__half>::get(int i) const {
+    return __half2float(__ushort_as_half((uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1])));
 }
 
 // Smallest e >= -126 with amax <= fmax 2^e.  fmax = 0.875 * 2^top (top 9 for e4m3, 16 for e5m2), so with
-// amax = f 2^x, f in [0.5, 1): e = x - top, plus one where f > 0.875.
+// amax = f 2^x, f in [0.5, 1): e = x - top, plus one where f > 0.875.  Read off the bits; a subnormal amax ends at -126.
 __device__ __forceinline__ int block_exponent(float amax, int top) {
-    if (amax == 0.0f) return 0;
-    int x;
-    const float f = frexpf(amax, &x);
-    return max(x - top + (f > 0.875f ? 1 : 0), -126);
+    const int bits = __float_as_int(amax);
+    return amax == 0.0f ? 0 : max((bits >> 23) - 126 - top + ((bits & 0x7fffff) > 0x600000), -126);
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 template <bool E5M2>
-__device__ __forceinline__ uint32_t cvt2(float lo, float hi) {
-    uint16_t r;
-    if (E5M2)
-        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-    else
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-    return r;
+__device__ __forceinline__ uint32_t cvt4(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    if (E5M2) {
+        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    } else {
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    }
+    return (uint32_t)lo | (uint32_t)hi << 16;
 }
-// The conversion saturates: an infinity, which no scale brings into range, becomes the format's infinity
-// (e5m2) or, as e4m3 has none, NaN.
-template <bool E5M2>
-__device__ __forceinline__ uint32_t cvt4(const float* v, float s) {
-    float x[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = v[i] * s;
-    uint32_t w = cvt2<E5M2>(x[0], x[1]) | cvt2<E5M2>(x[2], x[3]) << 16;
+// 16 values times s as 16 bytes
+template <bool E5M2, class T>
+__device__ __forceinline__ uint4 cvt16(const Raw16<T>& v, float s) {
+    uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (isinf(v[i])) {
-            const uint32_t b = (E5M2 ? 0x7cu : 0x7fu) | (v[i] < 0.0f ? 0x80u : 0u);
-            w = (w & ~(0xffu << (8 * i))) | b << (8 * i);
-        }
-    return w;
+        w[i] = cvt4<E5M2>(v.get(4 * i) * s, v.get(4 * i + 1) * s, v.get(4 * i + 2) * s, v.get(4 * i + 3) * s);
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 struct CastParams {
@@ -117,6 +129,17 @@ struct CastParams {
     int block_rows;      // 1 or 128
 };
 
+// An infinity, which no scale brings into range, becomes NaN in e4m3, which has no infinity, and stays one in e5m2: there
+// the blocks that held one get its bytes here, from a second look at 16 values of x.
+template <class T>
+__device__ __noinline__ void restore_infinities(const CastParams& p, int row, int c, uint8_t* q, int step) {
+    const T* x = static_cast<const T*>(p.x) + row * p.pitch;
+    for (int j = c; j < min(c + 16, p.cols); j++) {
+        const float v = (float)x[j];
+        if (isinf(v)) q[(j - c) * step] = v < 0.0f ? 0xfc : 0x7c;
+    }
+}
+
 // Blocks of 1 x 128 without the transposed copy: eight threads per block, 16 values each, the block's maximum
 // by three shuffles.  One read, one write, no shared memory.
 template <class T, bool E5M2>
@@ -126,23 +149,31 @@ __global__ void __launch_bounds__(256) cast_rows_kernel(CastParams p) {
     const uint32_t row = unit / kb, b = unit - row * kb;
     const bool live = row < (uint32_t)p.rows;
     const int c = b * 128 + (threadIdx.x & 7) * 16;
-    float v[16];
+    Raw16<T> v;
     if (live)
-        load16(static_cast<const T*>(p.x) + row * p.pitch, c, p.cols, p.vec, v);
+        v.load(static_cast<const T*>(p.x) + row * p.pitch, c, p.cols, p.vec);
     else
-        for (int i = 0; i < 16; i++) v[i] = 0.0f;
+        v.zero();
     float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; i++) amax = fmaxf(amax, finite_size(v[i]));
+    for (int i = 0; i < 16; i++) amax = fmaxf(amax, fabsf(v.get(i)));
 #pragma unroll
     for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const bool inf = isinf(amax);
+    if (__any_sync(0xffffffffu, inf)) {
+        v.drop_infinities();
+        amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) amax = fmaxf(amax, fabsf(v.get(i)));
+#pragma unroll
+        for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    }
     if (!live) return;
     const int e = block_exponent(amax, E5M2 ? 16 : 9);
-    const float s = pow2(-e);
     if (c < p.qp) {
-        uint4 w;
-        w.x = cvt4<E5M2>(v, s), w.y = cvt4<E5M2>(v + 4, s), w.z = cvt4<E5M2>(v + 8, s), w.w = cvt4<E5M2>(v + 12, s);
-        *reinterpret_cast<uint4*>(p.q + (long)row * p.qp + c) = w;
+        uint8_t* q = p.q + (long)row * p.qp + c;
+        *reinterpret_cast<uint4*>(q) = cvt16<E5M2>(v, pow2(-e));
+        if (E5M2 && inf) restore_infinities<T>(p, row, c, q, 1);
     }
     if ((threadIdx.x & 7) == 0) p.scale[(long)row * p.sp + b] = (uint8_t)(e + 127);
 }
@@ -153,41 +184,50 @@ __global__ void __launch_bounds__(256) cast_rows_kernel(CastParams p) {
 // word (column, row / 4) at column * 32 + (row / 4 ^ 4 (column / 16)), where the 32 lanes of a store and the
 // 16-byte groups of a read fall into different banks.
 template <class T, bool E5M2>
-__global__ void __launch_bounds__(256) cast_tile_kernel(CastParams p) {
-    __shared__ uint32_t smax[128];            // column maxima (bits of non-negative floats order as integers)
-    __shared__ uint32_t smax_tile;
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) cast_tile_kernel(CastParams p) {
+    __shared__ float cmax[8][128];            // column maxima of each warp's 16 rows; [0]: the columns' scales
+    __shared__ float tmax[8];
     __shared__ __align__(16) uint32_t tile[128 * 32];
-    const int t = threadIdx.x, seg = t & 7, rw = t >> 3;
-    const int b = blockIdx.x % ((p.cols + 127) / 128), rb = blockIdx.x / ((p.cols + 127) / 128);
+    const int t = threadIdx.x, seg = t & 7, rw = t >> 3, warp = t >> 5;
+    const int kb = (p.cols + 127) / 128, rb = blockIdx.x / kb, b = blockIdx.x - rb * kb;
     const int c = b * 128 + seg * 16, r0 = rb * 128 + rw * 4;
     constexpr int kTop = E5M2 ? 16 : 9;
-    if (t < 128) smax[t] = 0;
-    if (t == 0) smax_tile = 0;
-    float v[4][16];
+    Raw16<T> v[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if (r0 + i < p.rows)
-            load16(static_cast<const T*>(p.x) + (r0 + i) * p.pitch, c, p.cols, p.vec, v[i]);
+            v[i].load(static_cast<const T*>(p.x) + (r0 + i) * p.pitch, c, p.cols, p.vec);
         else
-#pragma unroll
-            for (int j = 0; j < 16; j++) v[i][j] = 0.0f;
+            v[i].zero();
     }
-    __syncthreads();
+    float size = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) size = fmaxf(size, fabsf(v[i].get(j)));
+    const bool inf = __syncthreads_or(isinf(size));
+    if (inf)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i].drop_infinities();
     float rmax[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         rmax[i] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 16; j++) rmax[i] = fmaxf(rmax[i], finite_size(v[i][j]));
+        for (int j = 0; j < 16; j++) rmax[i] = fmaxf(rmax[i], fabsf(v[i].get(j)));
 #pragma unroll
         for (int o = 4; o; o >>= 1) rmax[i] = fmaxf(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], o));
     }
     int e_tile = 0;
     if (p.block_rows == 128) {
-        if (seg == 0)
-            atomicMax(&smax_tile, __float_as_uint(fmaxf(fmaxf(rmax[0], rmax[1]), fmaxf(rmax[2], rmax[3]))));
+        float m = fmaxf(fmaxf(rmax[0], rmax[1]), fmaxf(rmax[2], rmax[3]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if ((t & 31) == 0) tmax[warp] = m;
         __syncthreads();
-        e_tile = block_exponent(__uint_as_float(smax_tile), kTop);
+#pragma unroll
+        for (int w = 0; w < 8; w++) m = fmaxf(m, tmax[w]);
+        e_tile = block_exponent(m, kTop);
         if (t == 0) {
             p.scale[(long)rb * p.sp + b] = (uint8_t)(e_tile + 127);
             if (p.qt) p.scale_t[(long)b * p.stp + rb] = (uint8_t)(e_tile + 127);
@@ -197,12 +237,10 @@ __global__ void __launch_bounds__(256) cast_tile_kernel(CastParams p) {
     for (int i = 0; i < 4; i++) {
         if (r0 + i >= p.rows) continue;
         const int e = p.block_rows == 128 ? e_tile : block_exponent(rmax[i], kTop);
-        const float s = pow2(-e);
         if (c < p.qp) {
-            uint4 w;
-            w.x = cvt4<E5M2>(v[i], s), w.y = cvt4<E5M2>(v[i] + 4, s), w.z = cvt4<E5M2>(v[i] + 8, s),
-            w.w = cvt4<E5M2>(v[i] + 12, s);
-            *reinterpret_cast<uint4*>(p.q + (long)(r0 + i) * p.qp + c) = w;
+            uint8_t* q = p.q + (long)(r0 + i) * p.qp + c;
+            *reinterpret_cast<uint4*>(q) = cvt16<E5M2>(v[i], pow2(-e));
+            if (E5M2 && inf) restore_infinities<T>(p, r0 + i, c, q, 1);
         }
         if (p.block_rows == 1 && seg == 0) p.scale[(long)(r0 + i) * p.sp + b] = (uint8_t)(e + 127);
     }
@@ -210,24 +248,33 @@ __global__ void __launch_bounds__(256) cast_tile_kernel(CastParams p) {
     if (p.block_rows == 1) {
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            float m = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) m = fmaxf(m, finite_size(v[i][j]));
+            float m = fmaxf(fmaxf(fabsf(v[0].get(j)), fabsf(v[1].get(j))), fmaxf(fabsf(v[2].get(j)), fabsf(v[3].get(j))));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            if ((t & 31) < 8) atomicMax(&smax[seg * 16 + j], __float_as_uint(m));
+            if ((t & 31) < 8) cmax[warp][seg * 16 + j] = m;
         }
         __syncthreads();
-        if (t < 128 && b * 128 + t < p.cols)
-            p.scale_t[(long)(b * 128 + t) * p.stp + rb] =
-                (uint8_t)(block_exponent(__uint_as_float(smax[t]), kTop) + 127);
+        if (t < 128) {
+            float m = cmax[0][t];
+#pragma unroll
+            for (int w = 1; w < 8; w++) m = fmaxf(m, cmax[w][t]);
+            const int e = block_exponent(m, kTop);
+            cmax[0][t] = pow2(-e);
+            if (b * 128 + t < p.cols) p.scale_t[(long)(b * 128 + t) * p.stp + rb] = (uint8_t)(e + 127);
+        }
+        __syncthreads();
     }
 #pragma unroll
     for (int j = 0; j < 16; j++) {
-        const int e = p.block_rows == 128 ? e_tile : block_exponent(__uint_as_float(smax[seg * 16 + j]), kTop);
-        const float col[4] = {v[0][j], v[1][j], v[2][j], v[3][j]};
-        tile[(seg * 16 + j) * 32 + (rw ^ (seg << 2))] = cvt4<E5M2>(col, pow2(-e));
+        const float s = p.block_rows == 128 ? pow2(-e_tile) : cmax[0][seg * 16 + j];
+        tile[(seg * 16 + j) * 32 + (rw ^ (seg << 2))] =
+            cvt4<E5M2>(v[0].get(j) * s, v[1].get(j) * s, v[2].get(j) * s, v[3].get(j) * s);
     }
+    if (E5M2 && inf)
+        for (int i = 0; i < 4; i++)
+            if (r0 + i < p.rows)
+                restore_infinities<T>(p, r0 + i, c,
+                                      reinterpret_cast<uint8_t*>(tile + seg * 16 * 32 + (rw ^ (seg << 2))) + i, 128);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -248,6 +295,20 @@ __global__ void __launch_bounds__(256)
     uncast_kernel(const uint8_t* q, const uint8_t* scale, int rows, int cols, int qp, int sp, int row_shift, T* out,
                   long pitch, int vec) {
     const uint32_t per = (cols + 15) / 16;
+    if (!vec) {
+        // rows of the output start anywhere: lanes take consecutive values, 512 columns of a row per warp
+        const uint32_t warps = (cols + 511) / 512, w = blockIdx.x * 8u + (threadIdx.x >> 5), row = w / warps;
+        if (row >= (uint32_t)rows) return;
+        const int c0 = (w - row * warps) * 512 + (threadIdx.x & 31);
+        const uint8_t* src = q + (long)row * qp;
+        const uint8_t* sc = scale + (long)(row >> row_shift) * sp;
+#pragma unroll 4
+        for (int c = c0; c < min(cols, c0 + 512); c += 32) {
+            const __half_raw h = __nv_cvt_fp8_to_halfraw(__ldg(src + c), E5M2 ? __NV_E5M2 : __NV_E4M3);
+            store_f(out + row * pitch + c, __half2float(__half(h)) * scale_value(__ldg(sc + (c >> 7))));
+        }
+        return;
+    }
     const uint32_t unit = blockIdx.x * 256u + threadIdx.x;
     const uint32_t row = unit / per;
     const int c = (unit - row * per) * 16;
@@ -264,7 +325,7 @@ __global__ void __launch_bounds__(256)
         store_f(&o[2 * i + 1], f.y * s);
     }
     T* dst = out + row * pitch + c;
-    if (vec && c + 16 <= cols) {
+    if (c + 16 <= cols) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T); i++)
             reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(o)[i];
@@ -300,20 +361,24 @@ template <int BN>
 struct ProductShape {
     static constexpr int kScaleRows = (BN + 127) / 128;              // N-side scale atoms of 128 rows
     static constexpr int kStageBytes = (kTileRows + BN) * kBlockK;
-    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int kStages = BN >= 128 ? 6 : 8;
     static constexpr int kScaleBytes = 512 * (1 + kScaleRows);
     static constexpr int kScaleCols = 4 * (1 + kScaleRows);
     static constexpr int kCols = BN + kScaleSlots * kScaleCols;
     static constexpr int kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
     static constexpr int kBarriers = 2 * kStages + 2 * kScaleSlots + 1;
     static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes + kBarriers * 8 + 16;
-    // the split sum's partial tile lies over the stages: BN columns of 129 floats
-    static_assert(BN * 129 * 4 <= kStages * kStageBytes, "partial tile exceeds the stages");
+    // the split sum's partial tile lies over the stages; its row pitch spreads eight rows over all banks
+    static constexpr int kPartPitch = BN + 4;
+    static_assert(kTileRows * kPartPitch * 4 <= kStages * kStageBytes, "partial tile exceeds the stages");
 };
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_addr(addr, rank)) : "memory");
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
 }
 
@@ -329,12 +394,13 @@ __device__ __forceinline__ void put(const ProductParams& p, int i, int j, float 
     }
 }
 
-// 32 consecutive columns of output row i in 16-byte pieces
-__device__ __forceinline__ void put_row32(const ProductParams& p, int i, int j, const float* v) {
+// N consecutive columns of output row i in 16-byte pieces (8 for N = 4 values of 16 bits)
+template <int N>
+__device__ __forceinline__ void put_row(const ProductParams& p, int i, int j, const float* v) {
     if (p.out_type == kTypeF32) {
         float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + i * p.pitch + j);
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
+        for (int k = 0; k < N / 4; k++) {
             float4 f = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
             if (p.accumulate) {
                 const float4 c = o[k];
@@ -344,23 +410,37 @@ __device__ __forceinline__ void put_row32(const ProductParams& p, int i, int j, 
         }
         return;
     }
-    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + i * p.pitch + j);
+    uint32_t w[N / 2];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        uint32_t w[4];
-#pragma unroll
-        for (int l = 0; l < 4; l++) {
-            const float a = v[8 * k + 2 * l], b = v[8 * k + 2 * l + 1];
-            if (p.out_type == kTypeBF16) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-                w[l] = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-                const __half2 h = __floats2half2_rn(a, b);
-                w[l] = *reinterpret_cast<const uint32_t*>(&h);
-            }
+    for (int k = 0; k < N / 2; k++) {
+        if (p.out_type == kTypeBF16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+            w[k] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+            w[k] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        o[k] = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    uint16_t* o = static_cast<uint16_t*>(p.out) + i * p.pitch + j;
+    if (N == 4)
+        *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+    else
+#pragma unroll
+        for (int k = 0; k < N / 8; k++)
+            reinterpret_cast<uint4*>(o)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+}
+
+// The scale words (four K blocks, group g) of rows r, r + 32, r + 64 and r + 96 of an operand: 16-byte row r % 32 of a
+// 512-byte atom.  Rows past the operand's end get the smallest scale; their products are zero.
+__device__ __forceinline__ uint4 scale_words(const ProductParams& p, int side, int r, int g) {
+    uint32_t x[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        x[j] = r + 32 * j < p.rows[side]
+                   ? __ldg(reinterpret_cast<const uint32_t*>(p.scale[side] +
+                                                             (long)((r + 32 * j) >> p.shift[side]) * p.sp[side]) + g)
+                   : 0u;
+    return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 // c = a b^T on 128 x BN tiles, one CTA per tile and K split.  Both operands stream through shared memory in
@@ -469,25 +549,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mma_commit_elect(done);
     } else if (warp == 2) {
-        // lane l gathers rows l, l + 32, l + 64, l + 96: the four words of 16-byte row l of the atom
         const int g0 = k0 >> 2, g1 = (k1 + 3) >> 2;
         for (int g = g0; g < g1; g++) {
             const int i = g - g0, slot = i % kScaleSlots;
             uint4 w[1 + S::kScaleRows];
 #pragma unroll
-            for (int a = 0; a < 1 + S::kScaleRows; a++) {
-                const int side = a > 0, first = side ? n0 + (a - 1) * 128 : m0;
-                uint32_t x[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int r = first + lane + 32 * j;
-                    x[j] = r < p.rows[side]
-                               ? __ldg(reinterpret_cast<const uint32_t*>(
-                                           p.scale[side] + (long)(r >> p.shift[side]) * p.sp[side]) + g)
-                               : 0u;
-                }
-                w[a] = make_uint4(x[0], x[1], x[2], x[3]);
-            }
+            for (int a = 0; a < 1 + S::kScaleRows; a++)
+                w[a] = scale_words(p, a > 0, (a > 0 ? n0 + (a - 1) * 128 : m0) + lane, g);
             if (!mbar_wait(&sempty[slot], ((i / kScaleSlots) & 1) ^ 1, p.status, kStatusWait)) break;
 #pragma unroll
             for (int a = 0; a < 1 + S::kScaleRows; a++)
@@ -513,11 +581,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr int kPer = BN % 32 == 0 ? 32 : 16;
             if (p.splits > 1) {
 #pragma unroll
-                for (int k = 0; k < kPer; k++) part[(c + k) * 129 + r] = v[k];
+                for (int k = 0; k < kPer; k += 4)
+                    *reinterpret_cast<float4*>(part + r * S::kPartPitch + c + k) =
+                        make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
             } else if (i < p.rows[0]) {
                 const int j = n0 + c;
                 if (kPer == 32 && p.vec && j + 32 <= p.rows[1]) {
-                    put_row32(p, i, j, v);
+                    put_row<32>(p, i, j, v);
                 } else {
 #pragma unroll
                     for (int k = 0; k < kPer; k++)
@@ -531,12 +601,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         cluster_sync_all();
         const int share = kTileRows / p.splits, first = split * share;
         const uint32_t part = smem_u32(smem);
-        for (int idx = threadIdx.x; idx < share * BN; idx += kThreads) {
-            const int r = first + (p.swap ? idx % share : idx / BN), c = p.swap ? idx / share : idx % BN;
+        for (int u = threadIdx.x; u < share * BN / 4; u += kThreads) {
+            // lanes along the output's rows
+            const int r = first + (p.swap ? u % share : u / (BN / 4)), c = (p.swap ? u / share : u % (BN / 4)) * 4;
             if (m0 + r >= p.rows[0] || n0 + c >= p.rows[1]) continue;
-            float v = 0.0f;
-            for (int s = 0; s < p.splits; s++) v += ld_cluster(part + (c * 129 + r) * 4, s);
-            put(p, m0 + r, n0 + c, v);
+            const uint32_t from = part + (r * S::kPartPitch + c) * 4;
+            float4 f[8];
+#pragma unroll
+            for (int s = 0; s < 8; s++)
+                if (s < p.splits) f[s] = ld_cluster4(peer_addr(from, s));
+            float v[4] = {f[0].x, f[0].y, f[0].z, f[0].w};
+#pragma unroll
+            for (int s = 1; s < 8; s++)
+                if (s < p.splits) v[0] += f[s].x, v[1] += f[s].y, v[2] += f[s].z, v[3] += f[s].w;
+            if (p.vec && n0 + c + 4 <= p.rows[1])
+                put_row<4>(p, m0 + r, n0 + c, v);
+            else
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (n0 + c + k < p.rows[1]) put(p, m0 + r, n0 + c + k, v[k]);
         }
         cluster_sync_all();   // a peer may still read this CTA's partial tile
     } else {
@@ -548,6 +631,219 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+// The same product for many tiles: persistent CTAs, two accumulators in TMEM, so that eight epilogue warps drain one
+// while the other fills (two of 256 columns and the scales exceed TMEM's 512).  The tensor core's FP32 accumulator
+// truncates, which shows in FP32 outputs over a long K; those add sums of kSegment blocks in registers.
+// Warps: 0 TMA, 1 MMA, 2 scales, 3 waits, 4-11 epilogue, and a second TMA warp where the registers for sums leave room.
+constexpr int wide_threads(bool f32) { return f32 ? 384 : 416; }
+constexpr int kSegment = 16;
+constexpr int kMaxSumColumns = 192;   // of FP32 outputs: 96 sums per thread
+
+template <int BN>
+struct WideShape {
+    static constexpr int kScaleRows = (BN + 127) / 128;
+    static constexpr int kStageBytes = (kTileRows + BN) * kBlockK;
+    static constexpr int kScaleBytes = 512 * (1 + kScaleRows), kScaleCols = 4 * (1 + kScaleRows);
+    static constexpr int kStages = (227 * 1024 - 2048 - kScaleSlots * kScaleBytes) / kStageBytes;
+    static constexpr int kCols = 2 * BN + kScaleSlots * kScaleCols;
+    static constexpr int kBarriers = 2 * kStages + 2 * kScaleSlots + 4;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes + kBarriers * 8 + 16;
+    static_assert(kCols <= 512 && kSmem <= 227 * 1024, "tile too wide");
+};
+
+template <int BN, bool F32>
+__global__ void __launch_bounds__(wide_threads(F32), 1)
+    product_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                        const ProductParams p) {
+    using S = WideShape<BN>;
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* ssm = smem + S::kStages * S::kStageBytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(ssm + kScaleSlots * S::kScaleBytes);
+    uint64_t *empty = full + S::kStages, *sfull = empty + S::kStages, *sempty = sfull + kScaleSlots;
+    uint64_t *tfull = sempty + kScaleSlots, *tempty = tfull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles = p.tiles_m * p.tiles_n, kb = p.kblocks;
+    const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;   // tiles of this CTA
+    auto place = [&](int t, int& m0, int& n0) {
+        const int tile = blockIdx.x + t * gridDim.x, band = 12 * p.tiles_n, in_band = tile % band;
+        const int first = tile / band * 12, band_m = min(12, p.tiles_m - first);
+        m0 = (first + in_band % band_m) * kTileRows, n0 = in_band / band_m * BN;
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < kScaleSlots; s++) {
+            mbar_init(&sfull[s], 32);
+            mbar_init(&sempty[s], 1);
+        }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(&tfull[s], 1);
+            mbar_init(&tempty[s], 256);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 3) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 || warp == 12) {
+        if (lane == 0) {
+            const int total = mine * kb;
+            bool ok = true;
+            for (int t = 0, n = 0; ok && t < mine; t++) {
+                int m0, n0;
+                place(t, m0, n0);
+                for (int k = 0; k < kb; k++, n++) {
+                    if (!F32 && (n & 1) != (warp == 12)) continue;
+                    const int s = n % S::kStages;
+                    if (n >= S::kStages &&
+                        !(ok = mbar_wait(&empty[s], ((n / S::kStages) & 1) ^ 1, p.status, kStatusWait)))
+                        break;
+                    uint8_t* st = smem + s * S::kStageBytes;
+                    mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+                    tma_load_2d(st, &tm_a, &full[s], k * kBlockK, m0);
+                    tma_load_2d(st + kTileRows * kBlockK, &tm_b, &full[s], k * kBlockK, n0);
+                    if (n + S::kStages >= total)   // no copy is in flight when the CTA ends
+                        mbar_wait(&full[s], (n / S::kStages) & 1, p.status, kStatusWait);
+                }
+            }
+        }
+    } else if (warp == 3) {
+        bool live = true;
+        for (int t = 0, n = 0, group = 0, acc = 0; t < mine; t++)
+            for (int k = 0; k < kb; k++, n++) {
+                if (k == 0 || (F32 && k % kSegment == 0)) {
+                    if (live) live = mbar_wait(&tempty[acc & 1], ((acc >> 1) & 1) ^ 1, p.status, kStatusWait);
+                    acc++;
+                }
+                if ((k & 3) == 0) {
+                    if (live) live = mbar_wait(&sfull[group % kScaleSlots], (group / kScaleSlots) & 1, p.status, kStatusWait);
+                    group++;
+                }
+                if (live) live = mbar_wait(&full[n % S::kStages], (n / S::kStages) & 1, p.status, kStatusWait);
+                named_bar_sync(kStageBar, 64);
+            }
+    } else if (warp == 1) {
+        const uint32_t st0 = smem_u32(smem), sc0 = smem_u32(ssm);
+        for (int t = 0, n = 0, group = 0, acc = 0; t < mine; t++)
+            for (int k = 0; k < kb; k++, n++) {
+                const int s = n % S::kStages, slot = group % kScaleSlots;
+                const uint32_t tsc = tmem + 2 * BN + slot * S::kScaleCols, d = tmem + (acc & 1) * BN;
+                named_bar_sync(kStageBar, 64);
+                tc_fence_after();
+                if ((k & 3) == 0)
+#pragma unroll
+                    for (int a = 0; a < 1 + S::kScaleRows; a++)
+                        tmem_cp_scales_elect(tsc + 4 * a,
+                                             smem_desc(sc0 + slot * S::kScaleBytes + a * 512, 0, 128, kLayoutNone));
+                const uint64_t da = smem_desc(st0 + s * S::kStageBytes, 0, 1024, kLayoutSw128);
+                const uint64_t db = smem_desc(st0 + s * S::kStageBytes + kTileRows * kBlockK, 0, 1024, kLayoutSw128);
+                const uint32_t idesc = p.idesc | (uint32_t)(k & 3) << 4 | (uint32_t)(k & 3) << 29;
+                const int in_segment = F32 ? k % kSegment : k;
+#pragma unroll
+                for (int i = 0; i < kBlockK / 32; i++)
+                    mma_mxf8_elect(d, da + 2 * i, db + 2 * i, idesc, tsc, tsc + 4, (in_segment | i) != 0);
+                mma_commit_elect(&empty[s]);
+                if ((k & 3) == 3 || k + 1 == kb) {
+                    mma_commit_elect(&sempty[slot]);
+                    group++;
+                }
+                if (k + 1 == kb || (F32 && in_segment + 1 == kSegment)) {
+                    mma_commit_elect(&tfull[acc & 1]);
+                    acc++;
+                }
+            }
+    } else if (warp == 2) {
+        bool ok = true;
+        for (int t = 0, group = 0; ok && t < mine; t++) {
+            int first[2];
+            place(t, first[0], first[1]);
+            for (int g = 0; g < (kb + 3) / 4; g++, group++) {
+                const int slot = group % kScaleSlots;
+                uint4 w[1 + S::kScaleRows];
+#pragma unroll
+                for (int a = 0; a < 1 + S::kScaleRows; a++)
+                    w[a] = scale_words(p, a > 0, first[a > 0] + (a > 0 ? a - 1 : 0) * 128 + lane, g);
+                if (!(ok = mbar_wait(&sempty[slot], ((group / kScaleSlots) & 1) ^ 1, p.status, kStatusWait))) break;
+#pragma unroll
+                for (int a = 0; a < 1 + S::kScaleRows; a++)
+                    *reinterpret_cast<uint4*>(ssm + slot * S::kScaleBytes + a * 512 + lane * 16) = w[a];
+                fence_proxy_async();
+                mbar_arrive(&sfull[slot]);
+            }
+        }
+    } else {
+        const int r = (warp & 3) * 32 + lane, c_first = ((warp - 4) >> 2) * (BN / 2);
+        const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
+        bool ok = true;
+        int acc = 0;
+        for (int t = 0; t < mine; t++) {
+            int m0, n0;
+            place(t, m0, n0);
+            const int i = m0 + r;
+            auto emit = [&](int c, const float* v) {
+                const int j = n0 + c;
+                if (i >= p.rows[0]) return;
+                if (p.vec && j + 16 <= p.rows[1]) {
+                    put_row<16>(p, i, j, v);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; k++)
+                        if (j + k < p.rows[1]) put(p, i, j + k, v[k]);
+                }
+            };
+            if (F32) {
+                float sum[BN / 2];
+                const int segments = (kb + kSegment - 1) / kSegment;
+                for (int g = 0; g < segments; g++, acc++) {
+                    if (ok) ok = mbar_wait(&tfull[acc & 1], (acc >> 1) & 1, p.status, kStatusWait);
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < BN / 2; c += 16) {
+                        float v[16];
+                        tmem_ld16(tmem + (acc & 1) * BN + quarter + c_first + c, v);
+#pragma unroll
+                        for (int k = 0; k < 16; k++) sum[c + k] = g ? sum[c + k] + v[k] : v[k];
+                    }
+                    tc_fence_before();
+                    mbar_arrive(&tempty[acc & 1]);
+                }
+#pragma unroll
+                for (int c = 0; c < BN / 2; c += 16) emit(c_first + c, sum + c);
+            } else {
+                if (ok) ok = mbar_wait(&tfull[acc & 1], (acc >> 1) & 1, p.status, kStatusWait);
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = c_first; c < c_first + BN / 2; c += 16) {
+                    float v[16];
+                    __syncwarp();
+                    tmem_ld16(tmem + (acc & 1) * BN + quarter + c, v);
+                    emit(c, v);
+                }
+                tc_fence_before();
+                mbar_arrive(&tempty[acc & 1]);
+                acc++;
+            }
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    if (warp == 3) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
 __global__ void fill_zero_kernel(ProductParams p) {
     const long n = (long)p.rows[0] * p.rows[1];
     for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x)
@@ -555,29 +851,33 @@ __global__ void fill_zero_kernel(ProductParams p) {
 }
 
 struct Plan {
-    int swap, bn, splits;
+    int swap, bn, splits, wide;
 };
 
-// Tile width, K splits and which operand takes the MMA's 128-row side, by an estimate of the time: a wave of
-// CTAs takes a fixed start and end plus, per K block, the longer of its MMAs and of its share of the copies.
-Plan plan_product(int m, int n, int kblocks, int sms) {
-    Plan best{0, 256, 1};
+// Tile width, K splits, the operand on the MMA's 128-row side and the kernel, by an estimate of the time in ns.
+Plan plan_product(int m, int n, int kblocks, bool f32, int sms) {
+    Plan best{0, 128, 1, 0};
     double least = 1e30;
+    auto offer = [&](double t, const Plan& p) {
+        if (t < least) least = t, best = p;
+    };
+    // of a block of K: a stage's copies at about 50 bytes per ns, or its MMAs
+    auto block = [](int bn) { return std::max((kTileRows + bn) * kBlockK / 160.0, bn * 1.2); };
     for (int swap = 0; swap < 2; swap++)
-        for (int bn : {16, 32, 64, 128, 256})
+        for (int bn : {16, 32, 64, 128})
             for (int splits : {1, 2, 4, 8}) {
                 if (splits > 1 && kblocks < 2 * splits) continue;
                 const long mt = ((swap ? n : m) + 127L) / 128, nt = ((swap ? m : n) + bn - 1L) / bn;
-                const long ctas = mt * nt * splits, waves = (ctas + sms - 1) / sms;
-                const double load = (kTileRows + bn) * kBlockK / 100.0 * std::min(1.0, (double)ctas / sms + 0.3);
-                const double block = std::max(load, bn * 0.55);   // ns
-                const double t = waves * (2500.0 + (splits > 1 ? 800.0 + 4.0 * bn : 6.0 * bn) +
-                                          block * ((kblocks + splits - 1) / splits));
-                if (t < least) {
-                    least = t;
-                    best = Plan{swap, bn, splits};
-                }
+                const long waves = (mt * nt * splits + sms - 1) / sms;
+                offer(waves * (4000.0 + (swap ? 20.0 : 8.0) * bn + (splits > 1 ? 1500.0 + 20.0 * bn : 0.0) +
+                               block(bn) * ((kblocks + splits - 1) / splits)),
+                      Plan{swap, bn, splits, 0});
             }
+    for (int bn : {128, 192, 224}) {
+        if (f32 && bn > kMaxSumColumns) continue;
+        const long tiles = ((m + 127L) / 128) * ((n + bn - 1L) / bn), waves = (tiles + sms - 1) / sms;
+        offer(4000.0 + 8.0 * bn + waves * std::max(block(bn) * kblocks, 8.0 * bn), Plan{0, bn, 1, 1});
+    }
     return best;
 }
 
@@ -616,6 +916,23 @@ void launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const ProductP
     launch_check("product_kernel");
 }
 
+template <int BN, bool F32>
+void launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const ProductParams& p, cudaStream_t stream) {
+    using S = WideShape<BN>;
+    static PerDeviceOnce once;
+    once_per_device(once, [] { set_max_dynamic_smem(product_wide_kernel<BN, F32>, S::kSmem, "product_wide_kernel"); });
+    const int grid = std::min(p.tiles_m * p.tiles_n, device_sms());
+    product_wide_kernel<BN, F32><<<grid, wide_threads(F32), S::kSmem, stream>>>(ta, tb, p);
+    launch_check("product_wide_kernel");
+}
+
+template <int BN>
+void launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const ProductParams& p, cudaStream_t stream) {
+    if constexpr (BN <= kMaxSumColumns)
+        if (p.out_type == kTypeF32) return launch_wide<BN, true>(ta, tb, p, stream);
+    launch_wide<BN, false>(ta, tb, p, stream);
+}
+
 template <class T>
 void launch_cast(const CastParams& p, bool e5m2, cudaStream_t stream) {
     const long kb = (p.cols + 127) / 128;
@@ -639,7 +956,8 @@ template <class T>
 void launch_uncast(const uint8_t* q, const uint8_t* scale, int rows, int cols, bool e5m2, int row_shift, T* out,
                    long pitch, cudaStream_t stream) {
     const int vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && pitch * sizeof(T) % 16 == 0;
-    const unsigned blocks = (unsigned)((rows * ((cols + 15L) / 16) + 255) / 256);
+    const unsigned blocks = vec ? (unsigned)((rows * ((cols + 15L) / 16) + 255) / 256)
+                                : (unsigned)((rows * ((cols + 511L) / 512) + 7) / 8);
     const int qp = (int)fp8_pitch(cols), sp = (int)fp8_scale_pitch(cols);
     if (e5m2)
         uncast_kernel<T, true><<<blocks, 256, 0, stream>>>(q, scale, rows, cols, qp, sp, row_shift, out, pitch, vec);
@@ -695,7 +1013,7 @@ void fp8_matmul(const Fp8Operand& a, const Fp8Operand& b, int k, void* out, int 
         launch_check("fill_zero_kernel");
         return;
     }
-    const Plan plan = plan_product(a.rows, b.rows, p.kblocks, device_sms());
+    const Plan plan = plan_product(a.rows, b.rows, p.kblocks, out_type == kTypeF32, device_sms());
     const Fp8Operand& left = plan.swap ? b : a;
     const Fp8Operand& right = plan.swap ? a : b;
     const Fp8Operand* side[2] = {&left, &right};
@@ -713,12 +1031,14 @@ void fp8_matmul(const Fp8Operand& a, const Fp8Operand& b, int k, void* out, int 
     p.vec = !plan.swap && reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch * elem % 16 == 0;
     const CUtensorMap ta = operand_map(left.q, left.rows, k, kTileRows);
     const CUtensorMap tb = operand_map(right.q, right.rows, k, plan.bn);
-    switch (plan.bn) {
+    switch (plan.wide ? 1000 + plan.bn : plan.bn) {
         case 16: launch_product<16>(ta, tb, p, stream); break;
         case 32: launch_product<32>(ta, tb, p, stream); break;
         case 64: launch_product<64>(ta, tb, p, stream); break;
         case 128: launch_product<128>(ta, tb, p, stream); break;
-        default: launch_product<256>(ta, tb, p, stream); break;
+        case 1128: launch_wide<128>(ta, tb, p, stream); break;
+        case 1192: launch_wide<192>(ta, tb, p, stream); break;
+        default: launch_wide<224>(ta, tb, p, stream); break;
     }
 }
 
