@@ -241,7 +241,10 @@ __device__ __forceinline__ void finish16(const Settings& q, const Source& j, int
 // accumulator rows that nothing reads.
 
 constexpr int kSlabThreads = 512;
-constexpr int kSlabRound = 384;      // columns of B X in TMEM at a time, beside 128 for the products of A
+// TMEM columns: the products of A and a round of columns of B X; for pairs each with as many for the cross products,
+// whose additions would otherwise truncate the hi hi sums twice as often.
+__host__ __device__ constexpr int slab_gram_cols(bool split) { return split ? 256 : 128; }
+__host__ __device__ constexpr int slab_round(bool split) { return split ? 128 : 384; }
 constexpr int kMaxSmem = 227 * 1024;
 
 struct SlabJob : Source {
@@ -324,14 +327,25 @@ __device__ __forceinline__ void slab_write16(uint8_t* hi, int lo, int row, int c
     }
 }
 
-// D += A B over 16 K elements of operands held as hi (+ lo at byte distance `a_lo`, `b_lo`)
+// D += A B over 16 K elements of operands held as hi (+ lo at byte distance `a_lo`, `b_lo`); the cross products go to the
+// accumulator 128 columns on.
 template <bool SPLIT>
 __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t a_lo, uint64_t b, uint64_t b_lo, uint32_t idesc,
                                          bool accumulate) {
     mma_f16(d, a, b, idesc, accumulate);
     if (SPLIT) {
-        mma_f16(d, a, b + b_lo, idesc, 1);
-        mma_f16(d, a + a_lo, b, idesc, 1);
+        mma_f16(d + 128, a, b + b_lo, idesc, accumulate);
+        mma_f16(d + 128, a + a_lo, b, idesc, 1);
+    }
+}
+template <bool SPLIT>
+__device__ __forceinline__ void load_pair16(uint32_t d, float* v) {
+    tmem_ld16(d, v);
+    if (SPLIT) {
+        float w[16];
+        tmem_ld16(d + 128, w);
+#pragma unroll
+        for (int k = 0; k < 16; k++) v[k] += w[k];
     }
 }
 
@@ -504,7 +518,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
     const uint64_t dx_mn = smem_desc(xs, rows * 128, 1024, kLayoutSw128);
     const uint64_t tile = rows * 128 / 16, dx_lo = x_lo / 16, da_lo = a_lo / 16;   // descriptor units
     const int row = (warp & 3) * 32 + lane, part_of = warp >> 2;   // accumulator row; warps share its columns
-    const uint32_t trow = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t trow = (uint32_t)((warp & 3) * 32) << 16, tmem_bx = tmem + slab_gram_cols(SPLIT);
     const float gram_f = exp2f((float)(kGramExp - 2 * j.p)), back_f = exp2f((float)-kGramExp), out_f = exp2f((float)-j.p);
     uint32_t phase = 0;
     bool bad = false;
@@ -526,7 +540,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         for (int c = part_of * 16; c < rows; c += kSlabThreads / 8) {
             float v[16];
             __syncwarp();
-            tmem_ld16(tmem + trow + c, v);
+            load_pair16<SPLIT>(tmem + trow + c, v);
             if (ranks == 1) {
 #pragma unroll
                 for (int k = 0; k < 16; k++) v[k] *= gram_f;
@@ -593,7 +607,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         for (int c = part_of * 16; c < rows; c += kSlabThreads / 8) {
             float v[16], old[16];
             __syncwarp();
-            tmem_ld16(tmem + trow + c, v);
+            load_pair16<SPLIT>(tmem + trow + c, v);
             if (row < rows) {
                 slab_read16<SPLIT>(a, a_lo, row, c, rows, old);
 #pragma unroll
@@ -606,14 +620,14 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         __syncthreads();
         // X <- a X + B X
         const bool last = step + 1 == q.steps;
-        for (int c0 = 0; c0 < tiles * 64; c0 += kSlabRound) {
-            const int n = min(kSlabRound, tiles * 64 - c0);
+        for (int c0 = 0; c0 < tiles * 64; c0 += slab_round(SPLIT)) {
+            const int n = min(slab_round(SPLIT), tiles * 64 - c0);
             if (tid == 0) {
                 tc_fence_after();
                 for (int n0 = 0; n0 < n; n0 += 256) {
                     const uint64_t b = dx_mn + (c0 + n0) / 64 * tile;
                     for (int kk = 0; kk < rows / 16; kk++)
-                        mma_pair<SPLIT>(tmem + 128 + n0, da + (kk >> 2) * tile + 2 * (kk & 3), da_lo, b + kk * (2048 / 16),
+                        mma_pair<SPLIT>(tmem_bx + n0, da + (kk >> 2) * tile + 2 * (kk & 3), da_lo, b + kk * (2048 / 16),
                                         dx_lo, idesc_f16(min(256, n - n0), 1), kk != 0);
                 }
                 mma_commit(&bar);
@@ -625,7 +639,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
             for (int c = part_of * 16; c < n; c += kSlabThreads / 8) {
                 float v[16], old[16];
                 __syncwarp();
-                tmem_ld16(tmem + 128 + trow + c, v);
+                load_pair16<SPLIT>(tmem_bx + trow + c, v);
                 if (row < rows) {
                     slab_read16<SPLIT>(x, x_lo, row, c0 + c, rows, old);
 #pragma unroll
@@ -660,8 +674,9 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
 // into one of two accumulators in TMEM, eight warps turn the other accumulator into the next operand.  The
 // symmetric products compute the upper triangle of tiles and write each tile twice; where X X^T has fewer tiles than
 // the GPU has SMs its K is split instead, and another phase adds the parts.
-// The tensor core's FP32 accumulator truncates, a bias that grows with the number of MMAs added into it; pairs of
-// fp16 therefore accumulate 512 elements along K at a time and add those sums in registers.
+// The tensor core's FP32 accumulator truncates: each MMA shrinks a sum by half an ulp on average, which the iteration
+// raises about fivefold (b A).  Pairs of fp16 therefore accumulate 128 elements along K (eight MMAs) at a time and add
+// those sums in registers; with 512 the error of a 1000 x 333 matrix was 6.6e-6, three times that of FP32 arithmetic.
 
 struct Job : Source {
     uint8_t *x[2], *a, *b;      // hi tiles; the lo tiles follow at x_bytes / a_bytes
@@ -689,7 +704,7 @@ enum { kGram = 0, kSquare = 1, kApply = 2 };   // A = X X^T;  B = b A + c A A;  
 constexpr int kEpilogueWarps = 8;
 constexpr int kTiledThreads = 32 * (4 + kEpilogueWarps);
 constexpr int kTiledBar = 1;                   // a stage is loaded: the waiting warp and the MMA warp
-constexpr int kSegment = 8;                    // stages (of 64 along K) per accumulator of pairs
+constexpr int kSegment = 2;                    // stages (of 64 along K) per accumulator of pairs
 
 // A tile is 128 rows by up to kBn columns.  Pairs of fp16 keep two accumulators per tile: hi hi, and the cross products,
 // whose additions would otherwise truncate the hi hi sum twice as often; with their sums in registers that leaves
