@@ -758,14 +758,44 @@ __device__ __forceinline__ TileAt tile_at(const Jobs<N>& q, int product, int t) 
     return a;
 }
 
-// 32 columns of a row of a tile as stored: fp16 values, hi and lo
+// Four lanes' 4 x 4 pieces of 16 bytes, transposed: piece i of lane q becomes piece q of lane i.  A lane of the accumulator
+// holds four pieces of its own row; afterwards an access of piece i by all lanes covers 64 consecutive bytes of each of
+// eight rows instead of 16 bytes of 32 rows, a quarter of the cache lines.
+__device__ __forceinline__ void transpose_pieces(uint4* c) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int m = 1; m <= 2; m <<= 1) {
+        const bool up = lane & m;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (k & m) continue;
+            const uint4 give = up ? c[k] : c[k + m];
+            uint4 got;
+            got.x = __shfl_xor_sync(0xffffffffu, give.x, m);
+            got.y = __shfl_xor_sync(0xffffffffu, give.y, m);
+            got.z = __shfl_xor_sync(0xffffffffu, give.z, m);
+            got.w = __shfl_xor_sync(0xffffffffu, give.w, m);
+            if (up)
+                c[k] = got;
+            else
+                c[k + m] = got;
+        }
+    }
+}
+// where piece i of lane `row` % 32 goes after transpose_pieces: byte offset from the lane's own row
+__device__ __forceinline__ int piece_offset(int row, int chunk0, int i) {
+    const int r = (row & ~3) + i;
+    return (r - row) * 128 + (((chunk0 + (row & 3)) ^ (r & 7)) << 4);
+}
+
+// 32 columns of a row of a tile as stored: fp16 values, hi and lo; fetched in transposed pieces
 template <bool SPLIT>
 struct OldBits {
     uint4 hi[4], lo[SPLIT ? 4 : 1];
     __device__ __forceinline__ void load(const uint8_t* row_hi, long lo_at, int row, int chunk0) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const uint8_t* p = row_hi + (((chunk0 + k) ^ (row & 7)) << 4);
+            const uint8_t* p = row_hi + piece_offset(row, chunk0, k);
             hi[k] = __ldcg(reinterpret_cast<const uint4*>(p));
             if (SPLIT) lo[k] = __ldcg(reinterpret_cast<const uint4*>(p + lo_at));
         }
@@ -773,7 +803,9 @@ struct OldBits {
 };
 // v += g (hi + lo)
 template <bool SPLIT>
-__device__ __forceinline__ void add_old(float* v, float g, const OldBits<SPLIT>& x) {
+__device__ __forceinline__ void add_old(float* v, float g, OldBits<SPLIT>& x) {
+    transpose_pieces(x.hi);
+    if (SPLIT) transpose_pieces(x.lo);
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         const uint32_t h[4] = {x.hi[k].x, x.hi[k].y, x.hi[k].z, x.hi[k].w};
@@ -805,11 +837,18 @@ __device__ __forceinline__ void write32(uint8_t* hi, long lo, int row, int chunk
         h[m] = *reinterpret_cast<const uint32_t*>(&a);
         l[m] = *reinterpret_cast<const uint32_t*>(&b);
     }
+    uint4 c[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        uint8_t* p = hi + (((chunk0 + k) ^ (row & 7)) << 4);
-        *reinterpret_cast<uint4*>(p) = make_uint4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
-        if (SPLIT) *reinterpret_cast<uint4*>(p + lo) = make_uint4(l[4 * k], l[4 * k + 1], l[4 * k + 2], l[4 * k + 3]);
+    for (int k = 0; k < 4; k++) c[k] = make_uint4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
+    transpose_pieces(c);
+#pragma unroll
+    for (int k = 0; k < 4; k++) *reinterpret_cast<uint4*>(hi + piece_offset(row, chunk0, k)) = c[k];
+    if (SPLIT) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) c[k] = make_uint4(l[4 * k], l[4 * k + 1], l[4 * k + 2], l[4 * k + 3]);
+        transpose_pieces(c);
+#pragma unroll
+        for (int k = 0; k < 4; k++) *reinterpret_cast<uint4*>(hi + lo + piece_offset(row, chunk0, k)) = c[k];
     }
     if (!mirror) return;
     const bool odd = row & 1;
@@ -1184,7 +1223,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                     return ((long)at.i * cb + ((at.j * bn + c) >> 6)) * kTileBytes + r * 128;
                 };
                 // v: 32 columns from c on of the accumulator; x: the old operand's
-                auto emit = [&](int c, float* v, const OldBits<SPLIT>& x) {
+                auto emit = [&](int c, float* v, OldBits<SPLIT>& x) {
 #pragma unroll
                     for (int k = 0; k < 32; k++) v[k] *= f;
                     if (part) {
@@ -1193,8 +1232,19 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                             q.parts + ((long)(j.part0 + tile * j.splits + at.split) * kTile + r) * kTile +
                             ((at.j * bn) & 127) + c);
 #pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            __stcg(to + k, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
+                        for (int h = 0; h < 2; h++) {
+                            uint4 p[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const float* w = v + 16 * h + 4 * k;
+                                p[k] = make_uint4(__float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]),
+                                                  __float_as_uint(w[3]));
+                            }
+                            transpose_pieces(p);
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                __stcg(reinterpret_cast<uint4*>(to) + ((r & ~3) + k - r) * (kTile / 4) + 4 * h + (r & 3), p[k]);
+                        }
                         return;
                     }
                     if (product != kGram) add_old<SPLIT>(v, g, x);
