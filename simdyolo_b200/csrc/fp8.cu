@@ -861,8 +861,9 @@ Plan plan_product(int m, int n, int kblocks, bool f32, int sms) {
     auto offer = [&](double t, const Plan& p) {
         if (t < least) least = t, best = p;
     };
-    // of a block of K: a stage's copies at about 50 bytes per ns, or its MMAs
-    auto block = [](int bn) { return std::max((kTileRows + bn) * kBlockK / 160.0, bn * 1.2); };
+    // A block of K is bound by shared memory, which every operand byte passes once in and once out, 128 bytes per cycle
+    // (measured at 8192^3: 281 ns for 128 columns, 357 for 192, 372 for 224; its MMAs take 135, 202 and 236).
+    auto block = [](int bn) { return (kTileRows + bn) * kBlockK * 2 / 240.0; };
     for (int swap = 0; swap < 2; swap++)
         for (int bn : {16, 32, 64, 128})
             for (int splits : {1, 2, 4, 8}) {
