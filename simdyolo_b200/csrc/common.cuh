@@ -400,6 +400,47 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
 
+// Lanes 0-15 and 16-31 hold 16 rows of 16 values each; afterwards lane l holds value l % 16 of all 16 rows of its half.
+__device__ __forceinline__ void transpose16(float* v, int lane) {
+#pragma unroll
+    for (int m = 8; m; m >>= 1) {
+        const bool up = lane & m;
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            if (k & m) continue;
+            const float got = __shfl_xor_sync(0xffffffffu, up ? v[k] : v[k + m], m);
+            if (up)
+                v[k] = got;
+            else
+                v[k + m] = got;
+        }
+    }
+}
+
+// Four lanes' 4 x 4 pieces of 16 bytes, transposed: piece i of lane q becomes piece q of lane i.  A lane of the accumulator
+// holds four pieces of its own row; afterwards an access of piece i by all lanes covers 64 consecutive bytes of each of
+// eight rows instead of 16 bytes of 32 rows, a quarter of the cache lines.
+__device__ __forceinline__ void transpose_pieces(uint4* c) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int m = 1; m <= 2; m <<= 1) {
+        const bool up = lane & m;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (k & m) continue;
+            const uint4 give = up ? c[k] : c[k + m];
+            uint4 got;
+            got.x = __shfl_xor_sync(0xffffffffu, give.x, m);
+            got.y = __shfl_xor_sync(0xffffffffu, give.y, m);
+            got.z = __shfl_xor_sync(0xffffffffu, give.z, m);
+            got.w = __shfl_xor_sync(0xffffffffu, give.w, m);
+            if (up)
+                c[k] = got;
+            else
+                c[k + m] = got;
+        }
+    }
+}
 // Shared-memory matrix descriptors (sm_100 version bits).
 //   K-major, SWIZZLE_128B (layout type 2): rows of 128 B (32 fp32 along K), 16 B chunks XOR-ed
 //     with (row % 8), 8-row groups 1024 B apart (SBO); LBO unused.  Matches TMA SWIZZLE_128B.

@@ -394,6 +394,16 @@ __device__ __forceinline__ void put(const ProductParams& p, int i, int j, float 
     }
 }
 
+// two values in the output's 16-bit type
+__device__ __forceinline__ uint32_t pack2(const ProductParams& p, float a, float b) {
+    if (p.out_type == kTypeBF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // N consecutive columns of output row i in 16-byte pieces (8 for N = 4 values of 16 bits)
 template <int N>
 __device__ __forceinline__ void put_row(const ProductParams& p, int i, int j, const float* v) {
@@ -412,15 +422,7 @@ __device__ __forceinline__ void put_row(const ProductParams& p, int i, int j, co
     }
     uint32_t w[N / 2];
 #pragma unroll
-    for (int k = 0; k < N / 2; k++) {
-        if (p.out_type == kTypeBF16) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-            w[k] = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-            const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-            w[k] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-    }
+    for (int k = 0; k < N / 2; k++) w[k] = pack2(p, v[2 * k], v[2 * k + 1]);
     uint16_t* o = static_cast<uint16_t*>(p.out) + i * p.pitch + j;
     if (N == 4)
         *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
@@ -428,6 +430,30 @@ __device__ __forceinline__ void put_row(const ProductParams& p, int i, int j, co
 #pragma unroll
         for (int k = 0; k < N / 8; k++)
             reinterpret_cast<uint4*>(o)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+}
+
+// 16 columns from j on of rows row0 + lane, any alignment: transposed between the lanes, so that a warp's accesses run
+// along the output's rows.  Called by a whole warp.
+__device__ __forceinline__ void put_rows16(const ProductParams& p, int row0, int j, float* v) {
+    const int lane = threadIdx.x & 31, first = row0 + (lane & 16), col = j + (lane & 15);
+    transpose16(v, lane);
+    if (col >= p.rows[1]) return;
+    const int n = min(16, p.rows[0] - first);
+    const long at = first * p.pitch + col;
+    if (p.out_type == kTypeF32) {
+        float* o = static_cast<float*>(p.out) + at;
+        float old[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++) old[k] = p.accumulate && k < n ? o[k * p.pitch] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; k++)
+            if (k < n) o[k * p.pitch] = old[k] + v[k];
+    } else {
+        uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+#pragma unroll
+        for (int k = 0; k < 16; k++)
+            if (k < n) o[k * p.pitch] = (uint16_t)pack2(p, v[k], 0.0f);
+    }
 }
 
 // The scale words (four K blocks, group g) of rows r, r + 32, r + 64 and r + 96 of an operand: 16-byte row r % 32 of a
@@ -584,14 +610,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int k = 0; k < kPer; k += 4)
                     *reinterpret_cast<float4*>(part + r * S::kPartPitch + c + k) =
                         make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-            } else if (i < p.rows[0]) {
+            } else {
                 const int j = n0 + c;
-                if (kPer == 32 && p.vec && j + 32 <= p.rows[1]) {
-                    put_row<32>(p, i, j, v);
-                } else {
+                if (p.swap) {   // lanes run along the output's rows already
 #pragma unroll
                     for (int k = 0; k < kPer; k++)
-                        if (j + k < p.rows[1]) put(p, i, j + k, v[k]);
+                        if (i < p.rows[0] && j + k < p.rows[1]) put(p, i, j + k, v[k]);
+                } else if (kPer == 32 && p.vec && j + 32 <= p.rows[1]) {
+                    if (i < p.rows[0]) put_row<32>(p, i, j, v);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kPer; k += 16) put_rows16(p, m0 + q * 32, j + k, v + k);
                 }
             }
         }
@@ -791,15 +820,30 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
             int m0, n0;
             place(t, m0, n0);
             const int i = m0 + r;
-            auto emit = [&](int c, const float* v) {
-                const int j = n0 + c;
-                if (i >= p.rows[0]) return;
-                if (p.vec && j + 16 <= p.rows[1]) {
-                    put_row<16>(p, i, j, v);
-                } else {
+            // Four pieces of 16 bytes from column c on: transposed between the lanes, so that a store covers 64 bytes of
+            // eight rows.
+            auto emit_pieces = [&](int c, uint4* q) {
+                constexpr int kPer = F32 ? 4 : 8;      // values per piece
+                const int row0 = i & ~3, j = n0 + c + kPer * (lane & 3);
+                transpose_pieces(q);
+                if (F32) {
+                    float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row0 * p.pitch + j);
+                    float4 old[4];
 #pragma unroll
-                    for (int k = 0; k < 16; k++)
-                        if (j + k < p.rows[1]) put(p, i, j + k, v[k]);
+                    for (int k = 0; k < 4; k++)
+                        old[k] = p.accumulate && row0 + k < p.rows[0] ? o[k * p.pitch / 4] : make_float4(0, 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float4 f = *reinterpret_cast<const float4*>(&q[k]);
+                        if (row0 + k < p.rows[0])
+                            o[k * p.pitch / 4] =
+                                make_float4(f.x + old[k].x, f.y + old[k].y, f.z + old[k].z, f.w + old[k].w);
+                    }
+                } else {
+                    uint16_t* o = static_cast<uint16_t*>(p.out) + row0 * p.pitch + j;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (row0 + k < p.rows[0]) *reinterpret_cast<uint4*>(o + k * p.pitch) = q[k];
                 }
             };
             if (F32) {
@@ -819,16 +863,36 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                     mbar_arrive(&tempty[acc & 1]);
                 }
 #pragma unroll
-                for (int c = 0; c < BN / 2; c += 16) emit(c_first + c, sum + c);
+                for (int c = 0; c < BN / 2; c += 16) {
+                    if (p.vec && n0 + c_first + c + 16 <= p.rows[1])
+                        emit_pieces(c_first + c, reinterpret_cast<uint4*>(sum + c));
+                    else
+                        put_rows16(p, i & ~31, n0 + c_first + c, sum + c);
+                }
             } else {
                 if (ok) ok = mbar_wait(&tfull[acc & 1], (acc >> 1) & 1, p.status, kStatusWait);
                 tc_fence_after();
+                int c = c_first;
 #pragma unroll 1
-                for (int c = c_first; c < c_first + BN / 2; c += 16) {
+                for (; c + 32 <= c_first + BN / 2 && p.vec && n0 + c + 32 <= p.rows[1]; c += 32) {
+                    float v[32];
+                    uint4 q[4];
+                    tmem_ld32(tmem + (acc & 1) * BN + quarter + c, v);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int l = 0; l < 4; l++) w[l] = pack2(p, v[8 * k + 2 * l], v[8 * k + 2 * l + 1]);
+                        q[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    emit_pieces(c, q);
+                }
+#pragma unroll 1
+                for (; c < c_first + BN / 2; c += 16) {
                     float v[16];
                     __syncwarp();
                     tmem_ld16(tmem + (acc & 1) * BN + quarter + c, v);
-                    emit(c, v);
+                    put_rows16(p, i & ~31, n0 + c, v);
                 }
                 tc_fence_before();
                 mbar_arrive(&tempty[acc & 1]);

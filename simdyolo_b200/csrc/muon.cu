@@ -166,23 +166,6 @@ __device__ __forceinline__ void pack8(const float* v, uint4& hi, uint4& lo) {
     lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// Lanes 0-15 and 16-31 hold 16 rows of 16 values each; afterwards lane l holds value l % 16 of all 16 rows of its half.
-__device__ __forceinline__ void transpose16(float* v, int lane) {
-#pragma unroll
-    for (int m = 8; m; m >>= 1) {
-        const bool up = lane & m;
-#pragma unroll
-        for (int k = 0; k < 16; k++) {
-            if (k & m) continue;
-            const float got = __shfl_xor_sync(0xffffffffu, up ? v[k] : v[k + m], m);
-            if (up)
-                v[k] = got;
-            else
-                v[k + m] = got;
-        }
-    }
-}
-
 // 16 consecutive values of O (X's orientation) per lane, from column `col` of row row0 + lane: the output, or the weight
 // update.  Called by a whole warp.  Where X is U the block is transposed between the lanes first, so that a warp's
 // accesses run along the rows of the output for any pitch and alignment; where X is U transposed they do already.
@@ -758,30 +741,6 @@ __device__ __forceinline__ TileAt tile_at(const Jobs<N>& q, int product, int t) 
     return a;
 }
 
-// Four lanes' 4 x 4 pieces of 16 bytes, transposed: piece i of lane q becomes piece q of lane i.  A lane of the accumulator
-// holds four pieces of its own row; afterwards an access of piece i by all lanes covers 64 consecutive bytes of each of
-// eight rows instead of 16 bytes of 32 rows, a quarter of the cache lines.
-__device__ __forceinline__ void transpose_pieces(uint4* c) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int m = 1; m <= 2; m <<= 1) {
-        const bool up = lane & m;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (k & m) continue;
-            const uint4 give = up ? c[k] : c[k + m];
-            uint4 got;
-            got.x = __shfl_xor_sync(0xffffffffu, give.x, m);
-            got.y = __shfl_xor_sync(0xffffffffu, give.y, m);
-            got.z = __shfl_xor_sync(0xffffffffu, give.z, m);
-            got.w = __shfl_xor_sync(0xffffffffu, give.w, m);
-            if (up)
-                c[k] = got;
-            else
-                c[k + m] = got;
-        }
-    }
-}
 // where piece i of lane `row` % 32 goes after transpose_pieces: byte offset from the lane's own row
 __device__ __forceinline__ int piece_offset(int row, int chunk0, int i) {
     const int r = (row & ~3) + i;
