@@ -432,28 +432,58 @@ __device__ __forceinline__ void put_row(const ProductParams& p, int i, int j, co
             reinterpret_cast<uint4*>(o)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
 }
 
-// 16 columns from j on of rows row0 + lane, any alignment: transposed between the lanes, so that a warp's accesses run
-// along the output's rows.  Called by a whole warp.
-__device__ __forceinline__ void put_rows16(const ProductParams& p, int row0, int j, float* v) {
-    const int lane = threadIdx.x & 31, first = row0 + (lane & 16), col = j + (lane & 15);
-    transpose16(v, lane);
-    if (col >= p.rows[1]) return;
-    const int n = min(16, p.rows[0] - first);
-    const long at = first * p.pitch + col;
-    if (p.out_type == kTypeF32) {
-        float* o = static_cast<float*>(p.out) + at;
-        float old[16];
+// Output rows of any alignment: a warp leaves 32 rows x 128 bytes (64 columns of 16 bits, 32 of FP32) in shared memory, a
+// row per lane, and writes them with its lanes along the rows.  (Lanes along the columns write a 3000 x 3001 output in
+// 103 us; rows 8 us.)
+constexpr int kRaggedPitch = 144;    // bytes; 16-byte accesses of eight rows fall into different banks
+constexpr int kRaggedBytes = 32 * kRaggedPitch;
+
+// 16 columns of this lane's row, the `at`-th 16 of the buffer
+template <bool F32>
+__device__ __forceinline__ void ragged_put(const ProductParams& p, uint8_t* buf, int at, const float* v) {
+    uint4* to = reinterpret_cast<uint4*>(buf + (threadIdx.x & 31) * kRaggedPitch + at * (F32 ? 64 : 32));
+    if (F32) {
 #pragma unroll
-        for (int k = 0; k < 16; k++) old[k] = p.accumulate && k < n ? o[k * p.pitch] : 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; k++)
-            if (k < n) o[k * p.pitch] = old[k] + v[k];
+        for (int k = 0; k < 4; k++)
+            to[k] = make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
+                               __float_as_uint(v[4 * k + 3]));
     } else {
-        uint16_t* o = static_cast<uint16_t*>(p.out) + at;
 #pragma unroll
-        for (int k = 0; k < 16; k++)
-            if (k < n) o[k * p.pitch] = (uint16_t)pack2(p, v[k], 0.0f);
+        for (int k = 0; k < 2; k++)
+            to[k] = make_uint4(pack2(p, v[8 * k], v[8 * k + 1]), pack2(p, v[8 * k + 2], v[8 * k + 3]),
+                               pack2(p, v[8 * k + 4], v[8 * k + 5]), pack2(p, v[8 * k + 6], v[8 * k + 7]));
     }
+}
+
+// the buffer's first `cols` columns to rows row0 .. row0 + 31, columns from j on
+template <bool F32>
+__device__ __forceinline__ void ragged_flush(const ProductParams& p, const uint8_t* buf, int row0, int j, int cols) {
+    const int lane = threadIdx.x & 31, n = min(32, p.rows[0] - row0);
+    cols = min(cols, p.rows[1] - j);
+    __syncwarp();
+    if (F32) {
+        float* o = static_cast<float*>(p.out) + row0 * p.pitch + j + lane;
+        if (lane < cols)
+            for (int k0 = 0; k0 < n; k0 += 8) {
+                float old[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) old[k] = p.accumulate && k0 + k < n ? o[(k0 + k) * p.pitch] : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (k0 + k < n)
+                        o[(k0 + k) * p.pitch] =
+                            old[k] + *reinterpret_cast<const float*>(buf + (k0 + k) * kRaggedPitch + 4 * lane);
+            }
+    } else {
+        uint16_t* o = static_cast<uint16_t*>(p.out) + row0 * p.pitch + j + lane;
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(buf) + lane;
+#pragma unroll 4
+        for (int k = 0; k < n; k++) {
+            if (lane < cols) o[k * p.pitch] = from[k * (kRaggedPitch / 2)];
+            if (lane + 32 < cols) o[k * p.pitch + 32] = from[k * (kRaggedPitch / 2) + 32];
+        }
+    }
+    __syncwarp();
 }
 
 // The scale words (four K blocks, group g) of rows r, r + 32, r + 64 and r + 96 of an operand: 16-byte row r % 32 of a
@@ -619,8 +649,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 } else if (kPer == 32 && p.vec && j + 32 <= p.rows[1]) {
                     if (i < p.rows[0]) put_row<32>(p, i, j, v);
                 } else {
-#pragma unroll
-                    for (int k = 0; k < kPer; k += 16) put_rows16(p, m0 + q * 32, j + k, v + k);
+                    // the stages are used up: their memory serves for the rows
+                    uint8_t* buf = smem + q * kRaggedBytes;
+                    if (p.out_type == kTypeF32) {
+                        for (int k = 0; k < kPer; k += 16) ragged_put<true>(p, buf, k >> 4, v + k);
+                        ragged_flush<true>(p, buf, m0 + q * 32, j, kPer);
+                    } else {
+                        for (int k = 0; k < kPer; k += 16) ragged_put<false>(p, buf, k >> 4, v + k);
+                        ragged_flush<false>(p, buf, m0 + q * 32, j, kPer);
+                    }
                 }
             }
         }
@@ -668,27 +705,29 @@ constexpr int wide_threads(bool f32) { return f32 ? 384 : 416; }
 constexpr int kSegment = 16;
 constexpr int kMaxSumColumns = 192;   // of FP32 outputs: 96 sums per thread
 
-template <int BN>
+template <int BN, bool RAGGED>
 struct WideShape {
     static constexpr int kScaleRows = (BN + 127) / 128;
     static constexpr int kStageBytes = (kTileRows + BN) * kBlockK;
     static constexpr int kScaleBytes = 512 * (1 + kScaleRows), kScaleCols = 4 * (1 + kScaleRows);
-    static constexpr int kStages = (227 * 1024 - 2048 - kScaleSlots * kScaleBytes) / kStageBytes;
+    static constexpr int kRagged = RAGGED ? 8 * kRaggedBytes : 0;   // of the eight epilogue warps
+    static constexpr int kStages = (227 * 1024 - 2048 - kScaleSlots * kScaleBytes - kRagged) / kStageBytes;
     static constexpr int kCols = 2 * BN + kScaleSlots * kScaleCols;
     static constexpr int kBarriers = 2 * kStages + 2 * kScaleSlots + 4;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes + kBarriers * 8 + 16;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes + kBarriers * 8 + 16 + kRagged;
     static_assert(kCols <= 512 && kSmem <= 227 * 1024, "tile too wide");
 };
 
-template <int BN, bool F32>
+template <int BN, bool F32, bool RAGGED>
 __global__ void __launch_bounds__(wide_threads(F32), 1)
     product_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                         const ProductParams p) {
-    using S = WideShape<BN>;
+    using S = WideShape<BN, RAGGED>;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint8_t* ssm = smem + S::kStages * S::kStageBytes;
-    uint64_t* full = reinterpret_cast<uint64_t*>(ssm + kScaleSlots * S::kScaleBytes);
+    uint8_t* ragged = ssm + kScaleSlots * S::kScaleBytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(ragged + S::kRagged);
     uint64_t *empty = full + S::kStages, *sfull = empty + S::kStages, *sempty = sfull + kScaleSlots;
     uint64_t *tfull = sempty + kScaleSlots, *tempty = tfull + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
@@ -820,12 +859,14 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
             int m0, n0;
             place(t, m0, n0);
             const int i = m0 + r;
-            // Four pieces of 16 bytes from column c on: transposed between the lanes, so that a store covers 64 bytes of
-            // eight rows.
+            uint8_t* buf = ragged + (warp - 4) * kRaggedBytes;
+            // Four pieces of 16 bytes from column c on, those inside the tile's half and the output: transposed between the
+            // lanes, so that a store covers 64 bytes of eight rows.  Columns come in whole pieces.
             auto emit_pieces = [&](int c, uint4* q) {
                 constexpr int kPer = F32 ? 4 : 8;      // values per piece
                 const int row0 = i & ~3, j = n0 + c + kPer * (lane & 3);
                 transpose_pieces(q);
+                if (j >= p.rows[1] || j - n0 >= c_first + BN / 2) return;
                 if (F32) {
                     float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row0 * p.pitch + j);
                     float4 old[4];
@@ -864,35 +905,47 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                 }
 #pragma unroll
                 for (int c = 0; c < BN / 2; c += 16) {
-                    if (p.vec && n0 + c_first + c + 16 <= p.rows[1])
-                        emit_pieces(c_first + c, reinterpret_cast<uint4*>(sum + c));
-                    else
-                        put_rows16(p, i & ~31, n0 + c_first + c, sum + c);
+                    if (!RAGGED) {
+                        if (n0 + c_first + c < p.rows[1]) emit_pieces(c_first + c, reinterpret_cast<uint4*>(sum + c));
+                    } else {
+                        ragged_put<true>(p, buf, (c >> 4) & 1, sum + c);
+                        if (c & 16) ragged_flush<true>(p, buf, i & ~31, n0 + c_first + c - 16, 32);
+                    }
                 }
             } else {
                 if (ok) ok = mbar_wait(&tfull[acc & 1], (acc >> 1) & 1, p.status, kStatusWait);
                 tc_fence_after();
-                int c = c_first;
+                const uint32_t d = tmem + (acc & 1) * BN + quarter + c_first;
+                if (!RAGGED) {
 #pragma unroll 1
-                for (; c + 32 <= c_first + BN / 2 && p.vec && n0 + c + 32 <= p.rows[1]; c += 32) {
-                    float v[32];
-                    uint4 q[4];
-                    tmem_ld32(tmem + (acc & 1) * BN + quarter + c, v);
+                    for (int c = 0; c < BN / 2 && n0 + c_first + c < p.rows[1]; c += 32) {
+                        float v[32];
+                        uint4 q[4];
+                        __syncwarp();
+                        tmem_ld16(d + c, v);
+                        if (c + 16 < BN / 2) tmem_ld16(d + c + 16, v + 16);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        uint32_t w[4];
+                        for (int k = 0; k < 4; k++) {
+                            uint32_t w[4];
 #pragma unroll
-                        for (int l = 0; l < 4; l++) w[l] = pack2(p, v[8 * k + 2 * l], v[8 * k + 2 * l + 1]);
-                        q[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (int l = 0; l < 4; l++) w[l] = pack2(p, v[8 * k + 2 * l], v[8 * k + 2 * l + 1]);
+                            q[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                        emit_pieces(c_first + c, q);
                     }
-                    emit_pieces(c, q);
-                }
+                } else {
 #pragma unroll 1
-                for (; c < c_first + BN / 2; c += 16) {
-                    float v[16];
-                    __syncwarp();
-                    tmem_ld16(tmem + (acc & 1) * BN + quarter + c, v);
-                    put_rows16(p, i & ~31, n0 + c, v);
+                    for (int c = 0; c < BN / 2 && n0 + c_first + c < p.rows[1]; c += 64) {
+                        const int some = min(64, BN / 2 - c);
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (16 * k < some) {
+                                float v[16];
+                                tmem_ld16(d + c + 16 * k, v);
+                                ragged_put<false>(p, buf, k, v);
+                            }
+                        ragged_flush<false>(p, buf, i & ~31, n0 + c_first + c, some);
+                    }
                 }
                 tc_fence_before();
                 mbar_arrive(&tempty[acc & 1]);
@@ -981,21 +1034,26 @@ void launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const ProductP
     launch_check("product_kernel");
 }
 
-template <int BN, bool F32>
+template <int BN, bool F32, bool RAGGED>
 void launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const ProductParams& p, cudaStream_t stream) {
-    using S = WideShape<BN>;
+    using S = WideShape<BN, RAGGED>;
     static PerDeviceOnce once;
-    once_per_device(once, [] { set_max_dynamic_smem(product_wide_kernel<BN, F32>, S::kSmem, "product_wide_kernel"); });
+    once_per_device(
+        once, [] { set_max_dynamic_smem(product_wide_kernel<BN, F32, RAGGED>, S::kSmem, "product_wide_kernel"); });
     const int grid = std::min(p.tiles_m * p.tiles_n, device_sms());
-    product_wide_kernel<BN, F32><<<grid, wide_threads(F32), S::kSmem, stream>>>(ta, tb, p);
+    product_wide_kernel<BN, F32, RAGGED><<<grid, wide_threads(F32), S::kSmem, stream>>>(ta, tb, p);
     launch_check("product_wide_kernel");
 }
 
 template <int BN>
 void launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const ProductParams& p, cudaStream_t stream) {
     if constexpr (BN <= kMaxSumColumns)
-        if (p.out_type == kTypeF32) return launch_wide<BN, true>(ta, tb, p, stream);
-    launch_wide<BN, false>(ta, tb, p, stream);
+        if (p.out_type == kTypeF32)
+            return p.vec ? launch_wide<BN, true, false>(ta, tb, p, stream) : launch_wide<BN, true, true>(ta, tb, p, stream);
+    if (p.vec)
+        launch_wide<BN, false, false>(ta, tb, p, stream);
+    else
+        launch_wide<BN, false, true>(ta, tb, p, stream);
 }
 
 template <class T>
@@ -1093,7 +1151,9 @@ void fp8_matmul(const Fp8Operand& a, const Fp8Operand& b, int k, void* out, int 
     p.tiles_m = (left.rows + kTileRows - 1) / kTileRows;
     p.tiles_n = (right.rows + plan.bn - 1) / plan.bn;
     p.idesc = idesc_mxf8(plan.bn, left.e5m2, right.e5m2);
-    p.vec = !plan.swap && reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch * elem % 16 == 0;
+    // whole 16-byte pieces of the output's rows
+    p.vec = !plan.swap && reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch * elem % 16 == 0 &&
+            (long)b.rows * elem % 16 == 0;
     const CUtensorMap ta = operand_map(left.q, left.rows, k, kTileRows);
     const CUtensorMap tb = operand_map(right.q, right.rows, k, plan.bn);
     switch (plan.wide ? 1000 + plan.bn : plan.bn) {
