@@ -213,6 +213,17 @@ __device__ __forceinline__ void finish16(const Settings& q, const Source& j, int
     }
 }
 
+// The same out of line, for the tiled kernel: it runs in the last iteration only, and inlined it crowds the instruction
+// cache of the others.  Returns whether a new weight is not finite.
+struct Values16 {
+    float v[16];
+};
+__device__ __noinline__ bool finish16_far(const Settings& q, const Source& j, int row0, int col, Values16 values) {
+    bool bad = false;
+    finish16(q, j, row0, col, values.v, bad);
+    return bad;
+}
+
 // ------------------------------------------------------------------ short matrices: one cluster each
 //
 // A matrix of at most 128 rows (of X) stays on chip for the whole call.  The CTAs of a cluster hold a slab of
@@ -1210,9 +1221,12 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                     const int col = at.j * bn + c;
                     if (last) {
 #pragma unroll
-                        for (int k = 0; k < 32; k++) v[k] *= out_f;
-                        finish16(q, j, at.i * kTile + (r & ~31), col, v, bad);
-                        finish16(q, j, at.i * kTile + (r & ~31), col + 16, v + 16, bad);
+                        for (int h = 0; h < 2; h++) {
+                            Values16 o;
+#pragma unroll
+                            for (int k = 0; k < 16; k++) o.v[k] = v[16 * h + k] * out_f;
+                            bad |= finish16_far(q, j, at.i * kTile + (r & ~31), col + 16 * h, o);
+                        }
                         return;
                     }
                     const int bj = col >> 7;
@@ -1221,17 +1235,16 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                                           : nullptr;
                     write32<SPLIT>(dst + offset(c), lo, r, (col & 63) >> 3, v, mirror, col & 127);
                 };
-                // the old operand's values are fetched while the accumulator is still being filled
-                OldBits<SPLIT> x[2];
-                if (product != kGram) {
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        if (32 * h < share && wanted(c_first + 32 * h))
-                            x[h].load(old + offset(c_first + 32 * h), lo, r, ((c_first + 32 * h) & 63) >> 3);
-                }
+                // The old operand's values are fetched while the accumulator is still being filled, 32 columns ahead.
+                OldBits<SPLIT> x;
+                auto fetch = [&](int c) {
+                    if (product != kGram && c < c_first + share && wanted(c)) x.load(old + offset(c), lo, r, (c & 63) >> 3);
+                };
+                fetch(c_first);
                 if (SPLIT) {
                     float acc[S::kBn / 2];
                     const int segments = (at.k1 - at.k0 + kSegment - 1) / kSegment;
+#pragma unroll 1
                     for (int m = 0; m < segments; m++) {
                         if (ok) ok = mbar_wait(&tfull[accs & 1], (accs >> 1) & 1, q.status, kStatusWait);
                         tc_fence_after();
@@ -1250,27 +1263,26 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                         }
                         drained();
                     }
+#pragma unroll 1
+                    for (int c = c_first; c < c_first + share; c += 32) {
+                        if (wanted(c)) emit(c, acc, x);
+                        fetch(c + 32);
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        if (32 * h < share && wanted(c_first + 32 * h)) emit(c_first + 32 * h, acc + 32 * h, x[h]);
+                        for (int k = 0; k < S::kBn / 2 - 32; k++) acc[k] = acc[k + 32];
+                    }
                 } else {
                     if (ok) ok = mbar_wait(&tfull[accs & 1], (accs >> 1) & 1, q.status, kStatusWait);
                     tc_fence_after();
                     const uint32_t d = tmem + (accs & 1) * S::kAccCols + ((uint32_t)((warp & 3) * 32) << 16);
 #pragma unroll 1
-                    for (int c = c_first; c < c_first + share; c += 64) {
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int cc = c + 32 * h;
-                            if (cc >= c_first + share || !wanted(cc)) continue;
+                    for (int c = c_first; c < c_first + share; c += 32) {
+                        if (wanted(c)) {
                             float v[32];
                             __syncwarp();
-                            tmem_ld32(d + cc, v);
-                            emit(cc, v, x[h]);
-                            // the same half of the next 64 columns
-                            if (product != kGram && cc + 64 < c_first + share && wanted(cc + 64))
-                                x[h].load(old + offset(cc + 64), lo, r, ((cc + 64) & 63) >> 3);
+                            tmem_ld32(d + c, v);
+                            emit(c, v, x);
                         }
+                        fetch(c + 32);
                     }
                     drained();
                 }
