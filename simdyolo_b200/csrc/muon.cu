@@ -1591,9 +1591,17 @@ void muon_update(const MuonMatrix* m, int count, const MuonRule& rule, void* wor
         run_sources<false>(set, list, workspace, stream);
 }
 
+// Whether an orthogonalisation runs on pairs.  Against 64 bits single fp16 operands leave 1.3e-3 to 1.7e-3 (relative
+// norm), about bf16's own rounding of 1.7e-3 and eight times fp16's; pairs leave 1e-6.  So only bf16 results take single
+// operands, and of those only matrices of more than 64 rows (of X): with fewer, single operands at times cost half as much
+// again as the rounding (a 4 x 2 matrix 3.2e-3 in all, some 2 x 2 ones 2e-2), and pairs cost little (64 x 576: 43 us
+// instead of 35).
+static bool takes_pairs(const Shape& s, int out_type) { return out_type != kTypeBF16 || s.r <= 64; }
+
 size_t orthogonalize_workspace_bytes(int rows, int cols, int out_type) {
     if (rows == 0 || cols == 0) return 0;
-    return workspace_bytes({Shape(rows, cols)}, out_type == kTypeF32);
+    const Shape shape(rows, cols);
+    return workspace_bytes({shape}, takes_pairs(shape, out_type));
 }
 
 void orthogonalize(const void* in, int in_type, long in_pitch, int rows, int cols, int steps, void* out, int out_type,
@@ -1612,7 +1620,7 @@ void orthogonalize(const void* in, int in_type, long in_pitch, int rows, int col
     const int bytes = in_type == kTypeF32 ? 4 : 2;
     const bool wide = aligned(in, in_pitch * bytes, 4 * bytes) && cols % 4 == 0;
     s.mode = in_type == kTypeF32 ? (wide ? kWide32 : kAny32) : (wide ? kWide16 : kAny16);
-    if (out_type == kTypeF32)
+    if (takes_pairs(shape, out_type))
         run_sources<true>(set, {s}, workspace, stream);
     else
         run_sources<false>(set, {s}, workspace, stream);

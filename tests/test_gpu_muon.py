@@ -40,6 +40,16 @@ def test_orthogonalize_shapes(rows, cols, out):
     assert status.item() == 0
 
 
+# Where the products run on pairs a 16-bit result is the FP32 one rounded: SPLIT_TOL plus half a step.
+@pytest.mark.parametrize("rows, cols, out", [(r, c, t) for r, c in ((2, 2), (4, 2), (9, 9), (33, 2000), (64, 64), (576, 64))
+                                             for t in (torch.bfloat16, torch.float16)] +
+                         [(r, c, torch.float16) for r, c in ((65, 65), (128, 300), (700, 333))])
+def test_orthogonalize_rounds_once(rows, cols, out):
+    for seed in range(4):
+        u = update(rows, cols, seed)
+        assert D.rel(D.orthogonalize(u.cuda(), out), D.orthogonal_reference(u)) <= SPLIT_TOL + D.HALF_STEP[out]
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
 @pytest.mark.parametrize("rows, cols", [(64, 200), (200, 64)])
 def test_orthogonalize_reads_types_and_strides_and_leaves_padding(dtype, rows, cols):
