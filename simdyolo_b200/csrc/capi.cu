@@ -1,5 +1,6 @@
 // extern "C" entry points declared in include/simdyolo_cuda.h.  Every call catches C++ exceptions
 // and returns a status code; the message is kept for sy_cuda_last_error.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <memory>
@@ -117,6 +118,12 @@ void check_format(int format, const char* what) {
     if (format != SY_FP8_E4M3 && format != SY_FP8_E5M2) fail(what, "unknown 8-bit format");
 }
 
+// The 8-bit kernels count rows and 16-value pieces of a matrix in 32 bits.
+void check_fp8_size(int rows, int cols, const char* what) {
+    if (std::max(rows, cols) > (1 << 30) || (int64_t)rows * sy::fp8_pitch(cols) > ((int64_t)1 << 35))
+        throw sy::SyError(SY_ERR_UNSUPPORTED_SHAPE, std::string(what) + ": matrix too large");
+}
+
 void check_block_rows(int block_rows, const char* what) {
     if (block_rows != 1 && block_rows != 128) fail(what, "block_rows must be 1 or 128");
 }
@@ -183,6 +190,31 @@ std::vector<sy::MuonMatrix> muon_matrices(const sy_muon_tensor* t, int count, co
         m.push_back({t[i].weight, t[i].momentum, t[i].grad, t[i].rows, t[i].cols});
     }
     return m;
+}
+
+// What one tensor's step writes, no tensor's step may read or write as well: they run at the same time.
+void check_apart(const std::vector<sy::MuonMatrix>& list, const char* what) {
+    struct Range {
+        uintptr_t first, end;
+        bool written;
+    };
+    std::vector<Range> ranges;
+    for (const auto& t : list) {
+        const size_t bytes = (size_t)t.rows * t.cols * sizeof(float);
+        if (!bytes) continue;
+        const auto add = [&](const float* p, bool written) {
+            const uintptr_t first = reinterpret_cast<uintptr_t>(p);
+            ranges.push_back({first, first + bytes, written});
+        };
+        add(t.weight, true), add(t.momentum, true), add(t.grad, false);
+    }
+    std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.first < b.first; });
+    uintptr_t written = 0, any = 0;          // ends of the ranges passed
+    for (const Range& r : ranges) {
+        if (r.first < (r.written ? any : written)) fail(what, "tensors share memory");
+        any = std::max(any, r.end);
+        if (r.written) written = std::max(written, r.end);
+    }
 }
 
 }  // namespace
@@ -818,6 +850,8 @@ sy_status sy_cuda_matmul_fp8(int32_t device, const float* a, const float* b, flo
         if (!a || !b || !c || m < 1 || n < 1 || k < 1)
             throw sy::SyError(SY_ERR_INVALID_ARGUMENT, "matmul_fp8: bad arguments");
         check_format(format, "matmul_fp8");
+        for (auto [rows, cols] : {std::pair(m, k), std::pair(k, n), std::pair(n, k)})
+            check_fp8_size(rows, cols, "matmul_fp8");
         check_device(device);
         Scratch s;
         const size_t na = (size_t)m * k, nb = (size_t)k * n, nc = (size_t)m * n;
@@ -850,6 +884,7 @@ sy_status sy_cuda_muon_update(int32_t device, float* weight, float* momentum, co
     return guarded(nullptr, [&] {
         if (!weight || !momentum || !grad || rows < 1 || cols < 1)
             throw sy::SyError(SY_ERR_INVALID_ARGUMENT, "muon_update: bad arguments");
+        check_ns_size(rows, cols, "muon_update");
         const sy::MuonRule rule = muon_rule(options, "muon_update");
         check_device(device);
         Scratch s;
@@ -891,6 +926,8 @@ sy_status sy_cuda_quantize_fp8_device(int32_t device, const void* x, int32_t x_t
     return guarded(nullptr, [&] {
         const char* what = "quantize_fp8_device";
         check_matrix(x_type, rows, cols, x_pitch, what);
+        check_fp8_size(rows, cols, what);
+        if (qt) check_fp8_size(cols, rows, what);
         check_format(format, what);
         check_block_rows(block_rows, what);
         if (!qt != !scale_t) fail(what, "qt and scale_t come together");
@@ -917,6 +954,7 @@ sy_status sy_cuda_dequantize_fp8_device(int32_t device, const uint8_t* q, const 
     return guarded(nullptr, [&] {
         const char* what = "dequantize_fp8_device";
         check_matrix(out_type, rows, cols, out_pitch, what);
+        check_fp8_size(rows, cols, what);
         check_format(format, what);
         check_block_rows(block_rows, what);
         if (rows == 0 || cols == 0) return SY_OK;
@@ -943,6 +981,8 @@ sy_status sy_cuda_matmul_fp8_device(int32_t device, const uint8_t* a, const uint
         check_block_rows(a_block_rows, what);
         check_block_rows(b_block_rows, what);
         if (k < 0) fail(what, "negative size");
+        check_fp8_size(m, k, what);
+        check_fp8_size(n, k, what);
         if (accumulate && out_type != SY_TYPE_F32) fail(what, "accumulate needs an SY_TYPE_F32 output");
         if (m == 0 || n == 0) return SY_OK;
         check_aligned(out, element_bytes(out_type), what, "out");
@@ -1024,6 +1064,7 @@ sy_status sy_cuda_muon_update_device(int32_t device, const sy_muon_tensor* tenso
         if (workspace_bytes < (int64_t)sy::muon_workspace_bytes(m.data(), count, rule.split))
             fail(what, "workspace too small");
         if (status) check_aligned(status, 4, what, "status");
+        check_apart(m, what);
         DeviceScope scope(device);
         for (const auto& t : m)
             if (t.rows && t.cols)

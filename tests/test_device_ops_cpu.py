@@ -99,6 +99,38 @@ def test_matrices_past_the_tile_counts_are_unsupported():
         orthogonalize(rows=1 << 21, cols=1 << 21, x_pitch=1 << 21, out_pitch=1 << 21, workspace_bytes=1 << 62)
 
 
+@pytest.mark.parametrize("call, kw", [
+    (quantize, dict(rows=(1 << 30) + 1, cols=1)),
+    (quantize, dict(rows=1 << 28, cols=129)),
+    (quantize, dict(rows=1, cols=(1 << 31) - 1, x_pitch=1 << 31)),
+    (quantize, dict(rows=33, cols=3 << 28, x_pitch=3 << 28, block_rows=128, qt=P, scale_t=P)),
+    (dequantize, dict(rows=(1 << 31) - 1)),
+    (dequantize, dict(rows=1 << 28, cols=256)),
+    (matmul, dict(k=(1 << 31) - 1)),
+    (matmul, dict(m=(1 << 30) + 1, n=1)),
+    (matmul, dict(m=1 << 20, k=1 << 16)),
+    (matmul, dict(n=1 << 20, k=1 << 16, out_pitch=1 << 20)),
+])
+def test_8_bit_matrices_past_32_bit_counts_are_unsupported(call, kw):
+    with pytest.raises(sy.UnsupportedShape, match="too large"):
+        call(**kw)
+
+
+def test_muon_tensors_that_share_memory_are_refused():
+    n = 32 * 64 * 4
+
+    def step(*entries):
+        t = sy.muon_tensors([(w, m, g, 32, 64) for w, m, g in entries])
+        sy.muon_update_device(t, sy.muon_options(0.02), P, 1 << 30)
+
+    for entries in ([(P, P + n, P + 2 * n)] * 2,
+                    [(P, P + n, P + 2 * n), (P + 3 * n, P + 4 * n, P + n - 4)],
+                    [(P, P + n, P)], [(P, P, P + n)], [(P, P + n - 4, P + 4 * n)],
+                    [(P + 9 * n, P + 8 * n, P + 7 * n), (P, P + n, P + 9 * n + 4)]):
+        with pytest.raises(sy.InvalidArgument, match="share memory"):
+            step(*entries)
+
+
 def test_empty_calls_need_no_memory():
     quantize(rows=0, x=0, q=0, scale=0)
     dequantize(cols=0, q=0, scale=0, out=0)
