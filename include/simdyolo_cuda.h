@@ -6,7 +6,7 @@
  * IComputeBackend.MatMul (src/SimdYolo/Compute.cs:11-25).  This library moves the whole inner
  * batch loop behind one call: frozen backbone forward, Detect-head forward/backward with
  * per-image training BatchNorm, DFL + CIoU + BCE loss with the task-aligned assigner, the
- * optional NCCL gradient all-reduce and the SGD-momentum / AdamW update.
+ * optional NCCL gradient all-reduce and the SGD-momentum / AdamW / Muon update.
  *
  * Conventions: plain C types; host pointers unless a name says "device"; the caller owns every
  * buffer it passes and may reuse it as soon as a call returns (calls are synchronous, except the operators on
@@ -88,7 +88,9 @@ typedef struct sy_config {
     sy_block box_blocks[3][8];  /* cv2.{0,1,2} (and one2one_cv2.{0,1,2} with end_to_end) */
     sy_block cls_blocks[3][8];  /* cv3.{0,1,2} (and one2one_cv3.{0,1,2} with end_to_end) */
     float bn_eps, bn_momentum;  /* DetectionHead.cs:71 (PT defaults 1e-3 / 0.03) */
-    int32_t optimizer;          /* SY_OPT_* */
+    int32_t optimizer;          /* SY_OPT_*.  Muon: nesterov, 5 iterations, rms 0.2 (sy_muon_options), `momentum` and
+                                 * `weight_decay` of the matrices; beta1, beta2, adam_eps of the other parameters;
+                                 * the products' precision follows `precision` */
     float lr, momentum, weight_decay;
     float beta1, beta2, adam_eps;
     int32_t precision;          /* SY_PRECISION_TF32, or SY_PRECISION_3XTF32 for the FP32 parity mode */
@@ -216,8 +218,8 @@ SY_API sy_status sy_cuda_eval_loss_features(sy_session *session, const float *co
 /* The completed-epoch counter YoloTrainer passes to DetectionHead.Loss (YoloTrainer.cs:192); it only
  * matters for progressive end-to-end heads.  Evaluation always uses epoch 0 (YoloTrainer.cs:243). */
 SY_API sy_status sy_cuda_set_epoch(sy_session *session, int32_t epoch);
-/* AdamW steps taken per optimizer group: [0] class branches, [1] cv2, [2] one2one_cv2 (a box group steps only
- * when an image connected it).  AdamW is not in the reference; with sy_cuda_get/set_optimizer_state these
+/* AdamW steps (also of SY_OPT_MUON's other parameters) taken per optimizer group: [0] class branches, [1] cv2,
+ * [2] one2one_cv2 (a box group steps only when an image connected it).  AdamW is not in the reference; with sy_cuda_get/set_optimizer_state these
  * counts complete the state a resumed AdamW run needs. */
 SY_API sy_status sy_cuda_get_optimizer_steps(const sy_session *session, int32_t steps[3]);
 SY_API sy_status sy_cuda_set_optimizer_steps(sy_session *session, const int32_t steps[3]);
@@ -402,8 +404,9 @@ SY_API sy_status sy_cuda_matmul_fp8_device(int32_t device, const uint8_t *a, con
 
 /* Orthogonalises x [rows][cols] by `steps` (1 .. 16; Muon uses 5) Newton-Schulz iterations: X = x / |x|_F
  * (transposed while it has more rows than columns), then X <- a X + (b A + c A^2) X with A = X X^T and
- * (a, b, c) = (3.4445, -4.7750, 2.0315).  A zero matrix gives zeros, one whose norm is not finite NaN.  With an
- * SY_TYPE_F32 output the products carry 22 significant bits per operand, with 16-bit outputs 11 (as TF32 does).
+ * (a, b, c) = (3.4445, -4.7750, 2.0315).  A zero matrix gives zeros, one whose norm is not finite NaN.  The products
+ * carry 22 significant bits per operand; 11 (as TF32 does) where the output is SY_TYPE_BF16 and both dimensions are
+ * above 64.
  * The workspace (sy_cuda_orthogonalize_workspace bytes, any alignment, no initial contents) is overwritten. */
 SY_API int64_t sy_cuda_orthogonalize_workspace(int32_t rows, int32_t cols, int32_t out_type);
 SY_API sy_status sy_cuda_orthogonalize_device(int32_t device, const void *x, int32_t x_type, int64_t x_pitch, int32_t rows,
@@ -426,7 +429,7 @@ typedef struct sy_muon_options {
     int32_t nesterov, steps, precision;
 } sy_muon_options;
 /* The Muon step of `count` matrices in one set of launches (tensors is host memory, read before the call
- * returns; no two tensors share memory).  *status receives SY_ERR_NONFINITE when a new weight is not finite. */
+ * returns).  No tensor's weight or momentum may share memory with anything else in the list.  *status receives SY_ERR_NONFINITE when a new weight is not finite. */
 SY_API int64_t sy_cuda_muon_workspace(const sy_muon_tensor *tensors, int32_t count, const sy_muon_options *options);
 SY_API sy_status sy_cuda_muon_update_device(int32_t device, const sy_muon_tensor *tensors, int32_t count,
                                             const sy_muon_options *options, void *workspace, int64_t workspace_bytes,

@@ -2,7 +2,8 @@
 
 The CUDA library (libsimdyolo_cuda.so, built from csrc/ for sm_100a) implements the hot path of
 SimdYolo.Training (YoloTrainer's batch loop: frozen backbone forward, Detect head forward/backward,
-DFL + CIoU + BCE loss with the task-aligned assigner, SGD-momentum / AdamW, NCCL all-reduce).
+DFL + CIoU + BCE loss with the task-aligned assigner, SGD-momentum / AdamW / Muon, NCCL all-reduce), and
+operators on device memory for 8-bit products and Muon updates.
 This module is the Python mirror of the reference's host API over that ABI (ctypes), used by the
 tests and bench.py.  There is no CPU fallback: every compute call goes to the CUDA library.
 """
@@ -663,7 +664,7 @@ class Session:
         _check(lib().sy_cuda_set_epoch(self._h, epoch), self._h)
 
     def optimizer_steps(self) -> list:
-        """AdamW steps taken per optimizer group (class branches, cv2, one2one_cv2)."""
+        """AdamW steps taken per optimizer group (class branches, cv2, one2one_cv2), also of a Muon session."""
         out = np.zeros(3, np.int32)
         _check(lib().sy_cuda_get_optimizer_steps(self._h, _ip(out)), self._h)
         return [int(v) for v in out]
