@@ -513,7 +513,14 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
     const uint64_t tile = rows * 128 / 16, dx_lo = x_lo / 16, da_lo = a_lo / 16;   // descriptor units
     const int row = (warp & 3) * 32 + lane, part_of = warp >> 2;   // accumulator row; warps share its columns
     const uint32_t trow = (uint32_t)((warp & 3) * 32) << 16, tmem_bx = tmem + slab_gram_cols(SPLIT);
-    const float gram_f = exp2f((float)(kGramExp - 2 * j.p)), back_f = exp2f((float)-kGramExp), out_f = exp2f((float)-j.p);
+    // The tensor core cuts off what an addition (of 16 products) has below the accumulator's last place, on average half a
+    // place.  Sums of like sign, the diagonals of X X^T and A^2, come out low by that much per addition, which the next
+    // iterations raise; raised by 2^-24 each they are right on average (five iterations, error against 64 bits: 80 x 720
+    // 2.4e-6 -> 1.4e-6, positive 128 x 1024 3.8e-6 -> 1.9e-6; FP32 products 1.1e-6 and 1.6e-6).
+    const float lost = SPLIT ? 0x1p-24f : 0.0f;
+    const float gram_f = exp2f((float)(kGramExp - 2 * j.p)) * (1.0f + lost * ((min(j.width, j.c) + 15) / 16));
+    const float back_f = exp2f((float)-kGramExp), square_f = back_f * (1.0f + lost * (rows / 16));
+    const float out_f = exp2f((float)-j.p);
     uint32_t phase = 0;
     bool bad = false;
     for (int step = 0; step < q.steps; step++) {
@@ -605,7 +612,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
             if (row < rows) {
                 slab_read16<SPLIT>(a, a_lo, row, c, rows, old);
 #pragma unroll
-                for (int k = 0; k < 16; k++) v[k] = kNsB * old[k] + kNsC * (v[k] * back_f);
+                for (int k = 0; k < 16; k++) v[k] = kNsB * old[k] + kNsC * (v[k] * square_f);
                 slab_write16<SPLIT>(a, a_lo, row, c, rows, v);
             }
         }
