@@ -697,24 +697,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// The same product for many tiles: persistent CTAs, two accumulators in TMEM, so that eight epilogue warps drain one
+// The same product for many tiles: persistent CTAs, two accumulators in TMEM, so that the epilogue warps drain one
 // while the other fills (two of 256 columns and the scales exceed TMEM's 512).  The tensor core's FP32 accumulator
-// truncates, which shows in FP32 outputs over a long K; those add sums of kSegment blocks in registers.
-// Warps: 0 TMA, 1 MMA, 2 scales, 3 waits, 4-11 epilogue, and a second TMA warp where the registers for sums leave room.
-constexpr int wide_threads(bool f32) { return f32 ? 384 : 416; }
+// truncates, which shows in FP32 outputs over a long K; those add sums of kSegment blocks in registers, at most 80 per
+// thread of three groups of epilogue warps (two groups end at 192 columns: 8192^3 512 us, three 438; a weight
+// gradient of 4096 x 1000 over 16,384, whose 240-column tiles make one wave, 82 us and 66).
+// Warps: 0 TMA, 1 MMA, 2 scales, 3 waits, from 4 on epilogue, the last a second TMA warp for 16-bit outputs.
+__host__ __device__ constexpr int epilogue_groups(bool f32) { return f32 ? 3 : 2; }
+constexpr int wide_threads(bool f32) { return f32 ? 512 : 416; }
 constexpr int kSegment = 16;
-constexpr int kMaxSumColumns = 192;   // of FP32 outputs: 96 sums per thread
 
 template <int BN, bool RAGGED>
 struct WideShape {
     static constexpr int kScaleRows = (BN + 127) / 128;
     static constexpr int kStageBytes = (kTileRows + BN) * kBlockK;
     static constexpr int kScaleBytes = 512 * (1 + kScaleRows), kScaleCols = 4 * (1 + kScaleRows);
+    static constexpr int kSlots = BN > 224 ? 2 : kScaleSlots;
     static constexpr int kRagged = RAGGED ? 8 * kRaggedBytes : 0;   // of the eight epilogue warps
-    static constexpr int kStages = (227 * 1024 - 2048 - kScaleSlots * kScaleBytes - kRagged) / kStageBytes;
-    static constexpr int kCols = 2 * BN + kScaleSlots * kScaleCols;
-    static constexpr int kBarriers = 2 * kStages + 2 * kScaleSlots + 4;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes + kBarriers * 8 + 16 + kRagged;
+    static constexpr int kStages = (227 * 1024 - 2048 - kSlots * kScaleBytes - kRagged) / kStageBytes;
+    static constexpr int kCols = 2 * BN + kSlots * kScaleCols;
+    static constexpr int kBarriers = 2 * kStages + 2 * kSlots + 4;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kSlots * kScaleBytes + kBarriers * 8 + 16 + kRagged;
     static_assert(kCols <= 512 && kSmem <= 227 * 1024, "tile too wide");
 };
 
@@ -726,10 +729,10 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint8_t* ssm = smem + S::kStages * S::kStageBytes;
-    uint8_t* ragged = ssm + kScaleSlots * S::kScaleBytes;
+    uint8_t* ragged = ssm + S::kSlots * S::kScaleBytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(ragged + S::kRagged);
-    uint64_t *empty = full + S::kStages, *sfull = empty + S::kStages, *sempty = sfull + kScaleSlots;
-    uint64_t *tfull = sempty + kScaleSlots, *tempty = tfull + 2;
+    uint64_t *empty = full + S::kStages, *sfull = empty + S::kStages, *sempty = sfull + S::kSlots;
+    uint64_t *tfull = sempty + S::kSlots, *tempty = tfull + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tiles = p.tiles_m * p.tiles_n, kb = p.kblocks;
@@ -745,13 +748,13 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int s = 0; s < kScaleSlots; s++) {
+        for (int s = 0; s < S::kSlots; s++) {
             mbar_init(&sfull[s], 32);
             mbar_init(&sempty[s], 1);
         }
         for (int s = 0; s < 2; s++) {
             mbar_init(&tfull[s], 1);
-            mbar_init(&tempty[s], 256);
+            mbar_init(&tempty[s], epilogue_groups(F32) * 128);
         }
         fence_barrier_init();
     }
@@ -764,7 +767,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 || warp == 12) {
+    if (warp == 0 || (!F32 && warp == 12)) {
         if (lane == 0) {
             const int total = mine * kb;
             bool ok = true;
@@ -795,7 +798,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                     acc++;
                 }
                 if ((k & 3) == 0) {
-                    if (live) live = mbar_wait(&sfull[group % kScaleSlots], (group / kScaleSlots) & 1, p.status, kStatusWait);
+                    if (live) live = mbar_wait(&sfull[group % S::kSlots], (group / S::kSlots) & 1, p.status, kStatusWait);
                     group++;
                 }
                 if (live) live = mbar_wait(&full[n % S::kStages], (n / S::kStages) & 1, p.status, kStatusWait);
@@ -805,7 +808,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
         const uint32_t st0 = smem_u32(smem), sc0 = smem_u32(ssm);
         for (int t = 0, n = 0, group = 0, acc = 0; t < mine; t++)
             for (int k = 0; k < kb; k++, n++) {
-                const int s = n % S::kStages, slot = group % kScaleSlots;
+                const int s = n % S::kStages, slot = group % S::kSlots;
                 const uint32_t tsc = tmem + 2 * BN + slot * S::kScaleCols, d = tmem + (acc & 1) * BN;
                 named_bar_sync(kStageBar, 64);
                 tc_fence_after();
@@ -837,12 +840,12 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
             int first[2];
             place(t, first[0], first[1]);
             for (int g = 0; g < (kb + 3) / 4; g++, group++) {
-                const int slot = group % kScaleSlots;
+                const int slot = group % S::kSlots;
                 uint4 w[1 + S::kScaleRows];
 #pragma unroll
                 for (int a = 0; a < 1 + S::kScaleRows; a++)
                     w[a] = scale_words(p, a > 0, first[a > 0] + (a > 0 ? a - 1 : 0) * 128 + lane, g);
-                if (!(ok = mbar_wait(&sempty[slot], ((group / kScaleSlots) & 1) ^ 1, p.status, kStatusWait))) break;
+                if (!(ok = mbar_wait(&sempty[slot], ((group / S::kSlots) & 1) ^ 1, p.status, kStatusWait))) break;
 #pragma unroll
                 for (int a = 0; a < 1 + S::kScaleRows; a++)
                     *reinterpret_cast<uint4*>(ssm + slot * S::kScaleBytes + a * 512 + lane * 16) = w[a];
@@ -851,7 +854,8 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
             }
         }
     } else {
-        const int r = (warp & 3) * 32 + lane, c_first = ((warp - 4) >> 2) * (BN / 2);
+        constexpr int kPart = (BN / epilogue_groups(F32) + 15) / 16 * 16;   // columns of a warp, the last group's fewer
+        const int r = (warp & 3) * 32 + lane, c_first = ((warp - 4) >> 2) * kPart, c_end = min(BN, c_first + kPart);
         const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
         bool ok = true;
         int acc = 0;
@@ -860,13 +864,13 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
             place(t, m0, n0);
             const int i = m0 + r;
             uint8_t* buf = ragged + (warp - 4) * kRaggedBytes;
-            // Four pieces of 16 bytes from column c on, those inside the tile's half and the output: transposed between the
+            // Four pieces of 16 bytes from column c on, those inside the warp's part and the output: transposed between the
             // lanes, so that a store covers 64 bytes of eight rows.  Columns come in whole pieces.
             auto emit_pieces = [&](int c, uint4* q) {
                 constexpr int kPer = F32 ? 4 : 8;      // values per piece
                 const int row0 = i & ~3, j = n0 + c + kPer * (lane & 3);
                 transpose_pieces(q);
-                if (j >= p.rows[1] || j - n0 >= c_first + BN / 2) return;
+                if (j >= p.rows[1] || j - n0 >= c_end) return;
                 if (F32) {
                     float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row0 * p.pitch + j);
                     float4 old[4];
@@ -888,28 +892,46 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                 }
             };
             if (F32) {
-                float sum[BN / 2];
+                float sum[kPart] = {};
                 const int segments = (kb + kSegment - 1) / kSegment;
                 for (int g = 0; g < segments; g++, acc++) {
                     if (ok) ok = mbar_wait(&tfull[acc & 1], (acc >> 1) & 1, p.status, kStatusWait);
+                    __syncwarp();
                     tc_fence_after();
 #pragma unroll
-                    for (int c = 0; c < BN / 2; c += 16) {
+                    for (int c = 0; c < kPart; c += 16) {
+                        if (c_first + c >= c_end) break;
                         float v[16];
                         tmem_ld16(tmem + (acc & 1) * BN + quarter + c_first + c, v);
 #pragma unroll
-                        for (int k = 0; k < 16; k++) sum[c + k] = g ? sum[c + k] + v[k] : v[k];
+                        for (int k = 0; k < 16; k++) {
+                            sum[c + k] += v[k];
+                            asm volatile("" : "+f"(sum[c + k]));   // before the next load: registers are short
+                        }
                     }
                     tc_fence_before();
                     mbar_arrive(&tempty[acc & 1]);
                 }
 #pragma unroll
-                for (int c = 0; c < BN / 2; c += 16) {
-                    if (!RAGGED) {
-                        if (n0 + c_first + c < p.rows[1]) emit_pieces(c_first + c, reinterpret_cast<uint4*>(sum + c));
-                    } else {
-                        ragged_put<true>(p, buf, (c >> 4) & 1, sum + c);
-                        if (c & 16) ragged_flush<true>(p, buf, i & ~31, n0 + c_first + c - 16, 32);
+                for (int c = 0; c < kPart; c += 16) {
+                    const int j = n0 + c_first + c;
+                    if (c_first + c >= c_end || j >= p.rows[1]) break;
+                    if (!p.swap) {
+                        emit_pieces(c_first + c, reinterpret_cast<uint4*>(sum + c));
+                    } else if (i < p.rows[0]) {   // lanes run along the output's rows, which may start anywhere
+                        float* o = static_cast<float*>(p.out) + j * p.pitch + i;
+#pragma unroll
+                        for (int h = 0; h < 16; h += 8) {
+                            float old[8];
+                            asm volatile("" : "+l"(o));   // addresses as they are needed: the sums fill the registers
+                            const float* from = o;
+#pragma unroll
+                            for (int k = 0; k < 8; k++, from += p.pitch)
+                                old[k] = p.accumulate && j + h + k < p.rows[1] ? *from : 0.0f;
+#pragma unroll
+                            for (int k = 0; k < 8; k++, o += p.pitch)
+                                if (j + h + k < p.rows[1]) *o = sum[c + h + k] + old[k];
+                        }
                     }
                 }
             } else {
@@ -972,7 +994,7 @@ struct Plan {
 };
 
 // Tile width, K splits, the operand on the MMA's 128-row side and the kernel, by an estimate of the time in ns.
-Plan plan_product(int m, int n, int kblocks, bool f32, int sms) {
+Plan plan_product(int m, int n, int kblocks, bool f32, bool vec, int sms) {
     Plan best{0, 128, 1, 0};
     double least = 1e30;
     auto offer = [&](double t, const Plan& p) {
@@ -991,11 +1013,14 @@ Plan plan_product(int m, int n, int kblocks, bool f32, int sms) {
                                block(bn) * ((kblocks + splits - 1) / splits)),
                       Plan{swap, bn, splits, 0});
             }
-    for (int bn : {128, 192, 224}) {
-        if (f32 && bn > kMaxSumColumns) continue;
-        const long tiles = ((m + 127L) / 128) * ((n + bn - 1L) / bn), waves = (tiles + sms - 1) / sms;
-        offer(4000.0 + 8.0 * bn + waves * std::max(block(bn) * kblocks, 8.0 * bn), Plan{0, bn, 1, 1});
-    }
+    // FP32 outputs whose rows are not whole 16-byte pieces leave with the lanes along them, as the M side.
+    for (int swap = f32 && !vec; swap <= (int)f32; swap++)
+        for (int bn : {128, 192, 224, 240}) {
+            if (!f32 && bn > 224) continue;
+            const long tiles = ((swap ? n : m) + 127L) / 128 * (((swap ? m : n) + bn - 1L) / bn);
+            const long waves = (tiles + sms - 1) / sms;
+            offer(4000.0 + 8.0 * bn + waves * std::max(block(bn) * kblocks, 8.0 * bn), Plan{swap, bn, 1, 1});
+        }
     return best;
 }
 
@@ -1047,13 +1072,13 @@ void launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const ProductPara
 
 template <int BN>
 void launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const ProductParams& p, cudaStream_t stream) {
-    if constexpr (BN <= kMaxSumColumns)
-        if (p.out_type == kTypeF32)
-            return p.vec ? launch_wide<BN, true, false>(ta, tb, p, stream) : launch_wide<BN, true, true>(ta, tb, p, stream);
-    if (p.vec)
-        launch_wide<BN, false, false>(ta, tb, p, stream);
-    else
-        launch_wide<BN, false, true>(ta, tb, p, stream);
+    if (p.out_type == kTypeF32) return launch_wide<BN, true, false>(ta, tb, p, stream);
+    if constexpr (BN <= 224) {
+        if (p.vec)
+            launch_wide<BN, false, false>(ta, tb, p, stream);
+        else
+            launch_wide<BN, false, true>(ta, tb, p, stream);
+    }
 }
 
 template <class T>
@@ -1136,7 +1161,9 @@ void fp8_matmul(const Fp8Operand& a, const Fp8Operand& b, int k, void* out, int 
         launch_check("fill_zero_kernel");
         return;
     }
-    const Plan plan = plan_product(a.rows, b.rows, p.kblocks, out_type == kTypeF32, device_sms());
+    // whole 16-byte pieces of the output's rows
+    const bool vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch * elem % 16 == 0 && (long)b.rows * elem % 16 == 0;
+    const Plan plan = plan_product(a.rows, b.rows, p.kblocks, out_type == kTypeF32, vec, device_sms());
     const Fp8Operand& left = plan.swap ? b : a;
     const Fp8Operand& right = plan.swap ? a : b;
     const Fp8Operand* side[2] = {&left, &right};
@@ -1151,9 +1178,7 @@ void fp8_matmul(const Fp8Operand& a, const Fp8Operand& b, int k, void* out, int 
     p.tiles_m = (left.rows + kTileRows - 1) / kTileRows;
     p.tiles_n = (right.rows + plan.bn - 1) / plan.bn;
     p.idesc = idesc_mxf8(plan.bn, left.e5m2, right.e5m2);
-    // whole 16-byte pieces of the output's rows
-    p.vec = !plan.swap && reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch * elem % 16 == 0 &&
-            (long)b.rows * elem % 16 == 0;
+    p.vec = vec && !plan.swap;
     const CUtensorMap ta = operand_map(left.q, left.rows, k, kTileRows);
     const CUtensorMap tb = operand_map(right.q, right.rows, k, plan.bn);
     switch (plan.wide ? 1000 + plan.bn : plan.bn) {
@@ -1163,7 +1188,8 @@ void fp8_matmul(const Fp8Operand& a, const Fp8Operand& b, int k, void* out, int 
         case 128: launch_product<128>(ta, tb, p, stream); break;
         case 1128: launch_wide<128>(ta, tb, p, stream); break;
         case 1192: launch_wide<192>(ta, tb, p, stream); break;
-        default: launch_wide<224>(ta, tb, p, stream); break;
+        case 1224: launch_wide<224>(ta, tb, p, stream); break;
+        default: launch_wide<240>(ta, tb, p, stream); break;
     }
 }
 

@@ -158,6 +158,25 @@ def test_product_accumulates(m, n, k):
     check(a, b, torch.float32, out, start)
 
 
+# FP32 outputs of many tiles: 128, 192, 224 and 240 columns per tile, along the output's rows and across them.
+@pytest.mark.parametrize("m, n, k", [(2853, 1452, 532), (658, 3364, 546), (3674, 972, 515), (3643, 1128, 653),
+                                     (1721, 2139, 512), (537, 3733, 527), (790, 3834, 518), (2274, 1677, 644),
+                                     (2274, 1676, 4700), (2274, 1677, 4700)])
+def test_wide_products_in_fp32(m, n, k):
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    a, b = operands(m, n, k)
+    buf = torch.full((m + 1, n + 5), 7.0, device="cuda")
+    D.matmul(a, b, torch.float32, out=buf, status=status)
+    check(a, b, torch.float32, buf[:m, :n])
+    D.matmul(a, b, torch.float32, out=buf, accumulate=True, status=status)
+    assert (buf[m:] == 7).all() and (buf[:, n:] == 7).all() and status.item() == 0
+    start = torch.randn(m, n, generator=torch.Generator().manual_seed(3))
+    out = start.cuda()
+    D.matmul(a, b, torch.float32, out=out, accumulate=True, status=status)
+    check(a, b, torch.float32, out, start)
+    assert status.item() == 0
+
+
 def test_product_is_the_same_every_time():
     a, b = operands(7, 900, 8000)
     first = D.matmul(a, b, torch.float32)
