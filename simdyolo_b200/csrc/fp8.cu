@@ -940,12 +940,12 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                 const uint32_t d = tmem + (acc & 1) * BN + quarter + c_first;
                 if (!RAGGED) {
 #pragma unroll 1
-                    for (int c = 0; c < BN / 2 && n0 + c_first + c < p.rows[1]; c += 32) {
+                    for (int c = 0; c < c_end - c_first && n0 + c_first + c < p.rows[1]; c += 32) {
                         float v[32];
                         uint4 q[4];
                         __syncwarp();
                         tmem_ld16(d + c, v);
-                        if (c + 16 < BN / 2) tmem_ld16(d + c + 16, v + 16);
+                        if (c + 16 < c_end - c_first) tmem_ld16(d + c + 16, v + 16);
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             uint32_t w[4];
@@ -957,8 +957,8 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                     }
                 } else {
 #pragma unroll 1
-                    for (int c = 0; c < BN / 2 && n0 + c_first + c < p.rows[1]; c += 64) {
-                        const int some = min(64, BN / 2 - c);
+                    for (int c = 0; c < c_end - c_first && n0 + c_first + c < p.rows[1]; c += 64) {
+                        const int some = min(64, c_end - c_first - c);
 #pragma unroll
                         for (int k = 0; k < 4; k++)
                             if (16 * k < some) {
@@ -1016,7 +1016,6 @@ Plan plan_product(int m, int n, int kblocks, bool f32, bool vec, int sms) {
     // FP32 outputs whose rows are not whole 16-byte pieces leave with the lanes along them, as the M side.
     for (int swap = f32 && !vec; swap <= (int)f32; swap++)
         for (int bn : {128, 192, 224, 240}) {
-            if (!f32 && bn > 224) continue;
             const long tiles = ((swap ? n : m) + 127L) / 128 * (((swap ? m : n) + bn - 1L) / bn);
             const long waves = (tiles + sms - 1) / sms;
             offer(4000.0 + 8.0 * bn + waves * std::max(block(bn) * kblocks, 8.0 * bn), Plan{swap, bn, 1, 1});
@@ -1073,12 +1072,10 @@ void launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const ProductPara
 template <int BN>
 void launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const ProductParams& p, cudaStream_t stream) {
     if (p.out_type == kTypeF32) return launch_wide<BN, true, false>(ta, tb, p, stream);
-    if constexpr (BN <= 224) {
-        if (p.vec)
-            launch_wide<BN, false, false>(ta, tb, p, stream);
-        else
-            launch_wide<BN, false, true>(ta, tb, p, stream);
-    }
+    if (p.vec)
+        launch_wide<BN, false, false>(ta, tb, p, stream);
+    else
+        launch_wide<BN, false, true>(ta, tb, p, stream);
 }
 
 template <class T>

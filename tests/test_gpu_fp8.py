@@ -177,6 +177,17 @@ def test_wide_products_in_fp32(m, n, k):
     assert status.item() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("m, n, k", [(3785, 904, 527), (537, 3736, 527), (3883, 776, 538), (1552, 2480, 645),
+                                     (1552, 2477, 645), (1000, 4096, 1300)])
+def test_wide_products_in_16_bits(m, n, k, dtype):
+    a, b = operands(m, n, k)
+    buf = torch.full((m + 1, n + 8), 7.0, dtype=dtype, device="cuda")
+    D.matmul(a, b, dtype, out=buf)
+    check(a, b, dtype, buf[:m, :n])
+    assert (buf[m:] == 7).all() and (buf[:, n:] == 7).all()
+
+
 def test_product_is_the_same_every_time():
     a, b = operands(7, 900, 8000)
     first = D.matmul(a, b, torch.float32)
