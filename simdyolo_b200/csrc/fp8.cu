@@ -398,6 +398,17 @@ __global__ void __launch_bounds__(256)
     }
     T* dst = out + row * pitch + c;
     if (c + 16 <= cols) {
+        const uint32_t* w8 = reinterpret_cast<const uint32_t*>(o);
+        if (vec == 2) {   // whole 32-byte sectors
+#pragma unroll
+            for (int i = 0; i < 4 * (int)sizeof(T); i += 8)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
+                                 reinterpret_cast<uint32_t*>(dst) + i),
+                             "r"(w8[i]), "r"(w8[i + 1]), "r"(w8[i + 2]), "r"(w8[i + 3]), "r"(w8[i + 4]), "r"(w8[i + 5]),
+                             "r"(w8[i + 6]), "r"(w8[i + 7])
+                             : "memory");
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T); i++)
             reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(o)[i];
@@ -1172,7 +1183,8 @@ void launch_cast(const CastParams& p, bool e5m2, cudaStream_t stream) {
 template <class T>
 void launch_uncast(const uint8_t* q, const uint8_t* scale, int rows, int cols, bool e5m2, int row_shift, T* out,
                    long pitch, cudaStream_t stream) {
-    const int vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && pitch * sizeof(T) % 16 == 0;
+    const uintptr_t align = reinterpret_cast<uintptr_t>(out) | (uintptr_t)(pitch * sizeof(T));
+    const int vec = align % 32 == 0 ? 2 : align % 16 == 0 ? 1 : 0;   // what the output's rows start on: 32, 16 bytes
     const unsigned blocks = vec ? (unsigned)((rows * ((cols + 15L) / 16) + 255) / 256)
                                 : (unsigned)((rows * ((cols + 511L) / 512) + 7) / 8);
     const int qp = (int)fp8_pitch(cols), sp = (int)fp8_scale_pitch(cols);
