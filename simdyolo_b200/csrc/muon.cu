@@ -1601,7 +1601,7 @@ void muon_update(const MuonMatrix* m, int count, const MuonRule& rule, void* wor
 // Whether an orthogonalisation runs on pairs.  Against 64 bits single fp16 operands leave 1.3e-3 to 1.7e-3 (relative
 // norm), about bf16's own rounding of 1.7e-3 and eight times fp16's; pairs leave 1e-6.  So only bf16 results take single
 // operands, and of those only matrices of more than 64 rows (of X): with fewer, single operands at times cost half as much
-// again as the rounding (a 4 x 2 matrix 3.2e-3 in all, some 2 x 2 ones 2e-2), and pairs cost little (64 x 576: 43 us
+// again as the rounding (a 4 x 2 matrix 3.2e-3 in all, some 2 x 2 ones 2e-2), and pairs cost little (64 x 576: 45 us
 // instead of 35).
 static bool takes_pairs(const Shape& s, int out_type) { return out_type != kTypeBF16 || s.r <= 64; }
 
