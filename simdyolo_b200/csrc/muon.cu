@@ -680,7 +680,8 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
 // those sums in registers; with 512 the error of a 1000 x 333 matrix was 6.6e-6, three times that of FP32 arithmetic.
 
 struct Job : Source {
-    uint8_t *x[2], *a, *b;      // hi tiles; the lo tiles follow at x_bytes / a_bytes
+    uint8_t *x[2], *a, *b;      // hi tiles; the lo tiles follow at x_bytes / a_bytes.  a null: A is kept in the X that the
+                                // iteration writes, whose tiles are at least as many and written after A was last read
     long x_bytes, a_bytes;
     int rb, cb;                 // 128-row blocks of X; 64-column blocks (padded to an even number)
     int splits;                 // parts of X X^T's K
@@ -689,6 +690,7 @@ struct Job : Source {
     int pack0, tile0[3], sum0;
     int part0;                  // and its first part (128 x 128 floats), splits per tile
 };
+__device__ __forceinline__ uint8_t* gram_of(const Job& j, int src) { return j.a ? j.a : j.x[src ^ 1]; }
 template <int N>
 struct Jobs : Settings {
     int count;
@@ -1055,7 +1057,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                 uint4 hi, lo;
                 pack8(v, hi, lo);
                 const int bj = tile / j.rb, bi = tile - bj * j.rb;
-                uint8_t* p = j.a + tile_offset(bi * kTile + row, bj * kTile + col, 2 * j.rb);
+                uint8_t* p = gram_of(j, src) + tile_offset(bi * kTile + row, bj * kTile + col, 2 * j.rb);
                 *reinterpret_cast<uint4*>(p) = hi;
                 if (SPLIT) *reinterpret_cast<uint4*>(p + j.a_bytes) = lo;
             }
@@ -1075,7 +1077,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                 for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
                     const TileAt at = tile_at(q, product, t);
                     const Job& j = q.job[at.job];
-                    const uint8_t* left = product == kGram ? j.x[src] : product == kSquare ? j.a : j.b;
+                    const uint8_t* left = product == kGram ? j.x[src] : product == kSquare ? gram_of(j, src) : j.b;
                     const long left_lo = product == kGram ? j.x_bytes : j.a_bytes;
                     const int lcb = product == kGram ? j.cb : 2 * j.rb;
                     // the columns' operand in pieces of 64, those that exist: column blocks of X, halves of row blocks
@@ -1183,9 +1185,9 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                                     : exp2f((float)-kGramExp) * (product == kSquare ? kNsC : 1.0f);
                 const float g = product == kSquare ? kNsB : kNsA, out_f = exp2f((float)-j.p);
                 const int cb = product == kApply ? j.cb : 2 * j.rb;
-                const uint8_t* old = product == kSquare ? j.a : j.x[src];
+                const uint8_t* old = product == kSquare ? gram_of(j, src) : j.x[src];
                 const long lo = product == kApply ? j.x_bytes : j.a_bytes;
-                uint8_t* dst = product == kGram ? j.a : product == kSquare ? j.b : j.x[src ^ 1];
+                uint8_t* dst = product == kGram ? gram_of(j, src) : product == kSquare ? j.b : j.x[src ^ 1];
                 // whether the 32 columns from c on are wanted, and where they are in the tiles
                 auto wanted = [&](int c) {
                     const int bj = (at.j * bn + c) >> 7;
@@ -1322,7 +1324,8 @@ struct Shape {
         x_bytes = (long)rb * cb * kTileBytes;
         a_bytes = (long)rb * rb * 2 * kTileBytes;
     }
-    long bytes(bool split) const { return (2 * x_bytes + 2 * a_bytes) * (split ? 2 : 1); }
+    // `shared`: A lies in the X that is written after it
+    long bytes(bool split, bool shared) const { return (2 * x_bytes + (shared ? 1 : 2) * a_bytes) * (split ? 2 : 1); }
 };
 
 // Beside the operands: the barrier's counter, partial norms, and the parts of split X X^T (at most one per SM).
@@ -1407,7 +1410,7 @@ TilePlan plan_tiles(const std::vector<Shape>& shapes, int sms) {
 }
 
 template <bool SPLIT, int N>
-void run_tiled(const Settings& set, const std::vector<Source>& list, uint8_t* workspace, cudaStream_t stream) {
+void run_tiled(const Settings& set, const std::vector<Source>& list, bool shared, uint8_t* workspace, cudaStream_t stream) {
     Jobs<N> q{};
     static_cast<Settings&>(q) = set;
     q.barrier = reinterpret_cast<uint32_t*>(workspace);
@@ -1428,9 +1431,10 @@ void run_tiled(const Settings& set, const std::vector<Source>& list, uint8_t* wo
         const int halves = SPLIT ? 2 : 1;
         j.x[0] = at;
         j.x[1] = j.x[0] + halves * s.x_bytes;
-        j.a = j.x[1] + halves * s.x_bytes;
-        j.b = j.a + halves * s.a_bytes;
-        at = j.b + halves * s.a_bytes;
+        at = j.x[1] + halves * s.x_bytes;
+        if (!shared) j.a = at, at += halves * s.a_bytes;
+        j.b = at;
+        at += halves * s.a_bytes;
         j.splits = plan.splits[i];
         j.pack0 = q.packs, j.sum0 = q.sums;
         q.packs += s.rb * s.cb;
@@ -1516,7 +1520,7 @@ void launch_slabs(const Settings& set, const std::vector<SlabJob>& list, cudaStr
 }
 
 template <bool SPLIT>
-void run_sources(const Settings& set, const std::vector<Source>& list, void* workspace, cudaStream_t stream) {
+void run_sources(const Settings& set, const std::vector<Source>& list, bool shared, void* workspace, cudaStream_t stream) {
     std::vector<SlabJob> slabs;
     std::vector<Source> tiled;
     for (const Source& s : list) {
@@ -1547,18 +1551,18 @@ void run_sources(const Settings& set, const std::vector<Source>& list, void* wor
         const std::vector<Source> part(tiled.begin() + first,
                                        tiled.begin() + std::min<size_t>(tiled.size(), first + kMaxJobs));
         if (part.size() == 1)
-            run_tiled<SPLIT, 1>(set, part, at, stream);
+            run_tiled<SPLIT, 1>(set, part, shared, at, stream);
         else
-            run_tiled<SPLIT, kMaxJobs>(set, part, at, stream);
+            run_tiled<SPLIT, kMaxJobs>(set, part, shared, at, stream);
     }
 }
 
 // Workspace of a call.  Matrices on the cluster path need none; whether a shape takes it does not depend on the rest of
 // the list, so a call with part of a list's matrices needs no more.
-size_t workspace_bytes(const std::vector<Shape>& shapes, bool split) {
+size_t workspace_bytes(const std::vector<Shape>& shapes, bool split, bool shared) {
     long sum = 0;
     for (const Shape& s : shapes)
-        if (!slab_ranks(s, split)) sum += s.bytes(split);
+        if (!slab_ranks(s, split)) sum += s.bytes(split, shared);
     return (size_t)(1024 + (sum ? kControlBytes + kNormBytes + kPartBytes + sum : 0));
 }
 
@@ -1572,7 +1576,7 @@ size_t muon_workspace_bytes(const MuonMatrix* m, int count, bool split) {
     std::vector<Shape> shapes;
     for (int i = 0; i < count; i++)
         if (m[i].rows && m[i].cols) shapes.emplace_back(m[i].rows, m[i].cols);
-    return workspace_bytes(shapes, split);
+    return workspace_bytes(shapes, split, false);
 }
 
 void muon_update(const MuonMatrix* m, int count, const MuonRule& rule, void* workspace, int* status,
@@ -1593,22 +1597,23 @@ void muon_update(const MuonMatrix* m, int count, const MuonRule& rule, void* wor
         list.push_back(s);
     }
     if (rule.split)
-        run_sources<true>(set, list, workspace, stream);
+        run_sources<true>(set, list, false, workspace, stream);
     else
-        run_sources<false>(set, list, workspace, stream);
+        run_sources<false>(set, list, false, workspace, stream);
 }
 
-// Whether an orthogonalisation runs on pairs.  Against 64 bits single fp16 operands leave 1.3e-3 to 1.7e-3 (relative
-// norm), about bf16's own rounding of 1.7e-3 and eight times fp16's; pairs leave 1e-6.  So only bf16 results take single
-// operands, and of those only matrices of more than 64 rows (of X): with fewer, single operands at times cost half as much
-// again as the rounding (a 4 x 2 matrix 3.2e-3 in all, some 2 x 2 ones 2e-2), and pairs cost little (64 x 576: 45 us
-// instead of 35).
-static bool takes_pairs(const Shape& s, int out_type) { return out_type != kTypeBF16 || s.r <= 64; }
+// An orthogonalisation runs on pairs whatever its result's type, so that a 16-bit result is the FP32 one rounded once.
+// Single fp16 operands leave 1.1e-3 (relative norm) on nearly white matrices, less than bf16's own rounding of 1.7e-3, but
+// the iteration raises the roundings of weak directions up to 485 times: singular values over three decades then cost
+// 4e-3 to 6e-3, values falling as 1 / i^2 2e-2.  (Muon's caller chooses by sy_muon_options.precision.)
+// bf16 results once ran on single operands in half the memory; their A shares memory with the X written after it, so that
+// their workspace stays below that of the other types, whose size is unchanged.
+static bool shares_gram(int out_type) { return out_type == kTypeBF16; }
 
 size_t orthogonalize_workspace_bytes(int rows, int cols, int out_type) {
     if (rows == 0 || cols == 0) return 0;
     const Shape shape(rows, cols);
-    return workspace_bytes({shape}, takes_pairs(shape, out_type));
+    return workspace_bytes({shape}, true, shares_gram(out_type));
 }
 
 void orthogonalize(const void* in, int in_type, long in_pitch, int rows, int cols, int steps, void* out, int out_type,
@@ -1627,10 +1632,7 @@ void orthogonalize(const void* in, int in_type, long in_pitch, int rows, int col
     const int bytes = in_type == kTypeF32 ? 4 : 2;
     const bool wide = aligned(in, in_pitch * bytes, 4 * bytes) && cols % 4 == 0;
     s.mode = in_type == kTypeF32 ? (wide ? kWide32 : kAny32) : (wide ? kWide16 : kAny16);
-    if (takes_pairs(shape, out_type))
-        run_sources<true>(set, {s}, workspace, stream);
-    else
-        run_sources<false>(set, {s}, workspace, stream);
+    run_sources<true>(set, {s}, shares_gram(out_type), workspace, stream);
 }
 
 }  // namespace sy

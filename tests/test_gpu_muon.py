@@ -236,3 +236,35 @@ def test_an_8_bit_layer_trained_by_muon():
         assert D.rel(cm, want_m) <= 3 * 2.0 ** -24
         want_dw = hdt.values() @ hxt.values().T
         assert ((dw.cpu().double() - want_dw).abs() <= D.product_bound(hdt.values(), hxt.values(), torch.float32, want_dw)).all()
+
+
+def spectrum(rows, cols, kind, seed=0):
+    """A matrix whose singular values fall over three decades, as 1 / i^2, or from eight equal ones to 1 % of them."""
+    g = torch.Generator().manual_seed(seed)
+    basis = lambda n: torch.linalg.qr(torch.randn(n, n, generator=g, dtype=torch.float64))[0]
+    k = min(rows, cols)
+    i = torch.arange(k, dtype=torch.float64)
+    s = {"decades": 10.0 ** (-3 * i / (k - 1)), "squares": 1 / (i + 1) ** 2,
+         "eight": torch.where(i < 8, 1.0, 0.01).double()}[kind]
+    return ((basis(rows)[:, :k] * s) @ basis(cols)[:, :k].T).float()
+
+
+# The weak directions of such a matrix carry the operands' roundings, raised up to 485 times.  An operand of 22 bits is off
+# by at most 2^-21 of its size (2^-22 for the pair, as much for the dropped lo lo), which orthogonal_bound follows through
+# the iterations; a 16-bit result is the FP32 result rounded, bit for bit.
+@pytest.mark.parametrize("kind", ["decades", "squares", "eight"])
+@pytest.mark.parametrize("rows, cols", [(65, 65), (128, 300), (300, 128), (129, 129), (700, 333), (256, 512)])
+def test_orthogonalize_of_steep_spectra_rounds_once(rows, cols, kind):
+    u = spectrum(rows, cols, kind)
+    want = D.orthogonal_reference(u)
+    full = D.orthogonalize(u.cuda(), torch.float32)
+    assert (full.cpu().double() - want).norm() <= D.orthogonal_bound(u, 2.0 ** -21)
+    for out in (torch.bfloat16, torch.float16):
+        assert torch.equal(D.orthogonalize(u.cuda(), out), full.to(out))
+
+
+@pytest.mark.parametrize("rows, cols, steps", [(130, 140, 1), (260, 700, 2), (900, 200, 3), (400, 400, 4), (300, 2000, 16)])
+def test_bf16_results_of_tiled_matrices_are_the_fp32_ones_rounded(rows, cols, steps):
+    u = update(rows, cols, 3).cuda()
+    assert torch.equal(D.orthogonalize(u, torch.bfloat16, steps, pitch=cols + 5)[:, :cols],
+                       D.orthogonalize(u, torch.float32, steps).bfloat16())
