@@ -406,7 +406,8 @@ SY_API sy_status sy_cuda_matmul_fp8_device(int32_t device, const uint8_t *a, con
  * (transposed while it has more rows than columns), then X <- a X + (b A + c A^2) X with A = X X^T and
  * (a, b, c) = (3.4445, -4.7750, 2.0315).  A zero matrix gives zeros, one whose norm is not finite NaN.  The products
  * carry 22 significant bits per operand for every output type: a 16-bit output is the FP32 one rounded once.
- * The workspace (sy_cuda_orthogonalize_workspace bytes, any alignment, no initial contents) is overwritten. */
+ * The workspace (sy_cuda_orthogonalize_workspace bytes, 0 for sizes that the call refuses; any alignment, no initial
+ * contents) is overwritten. */
 SY_API int64_t sy_cuda_orthogonalize_workspace(int32_t rows, int32_t cols, int32_t out_type);
 SY_API sy_status sy_cuda_orthogonalize_device(int32_t device, const void *x, int32_t x_type, int64_t x_pitch, int32_t rows,
                                               int32_t cols, int32_t steps, void *out, int32_t out_type,

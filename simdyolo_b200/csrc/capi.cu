@@ -132,9 +132,14 @@ void check_steps(int steps, const char* what) {
     if (steps < 1 || steps > 16) fail(what, "steps must be 1 .. 16");
 }
 
-// Tile counts of the products are 32-bit: 2^31 tiles of 128 x 128.
+// Tile counts of the products are 32-bit (2^31 tiles of 128 x 128), and so are columns rounded up to whole tiles.
+bool ns_size_fits(int rows, int cols) {
+    return std::min(rows, cols) <= (1 << 20) && std::max(rows, cols) <= (1 << 30) &&
+           (int64_t)rows * cols <= ((int64_t)1 << 40);
+}
+
 void check_ns_size(int rows, int cols, const char* what) {
-    if (std::min(rows, cols) > (1 << 20) || (int64_t)rows * cols > ((int64_t)1 << 40))
+    if (!ns_size_fits(rows, cols))
         throw sy::SyError(SY_ERR_UNSUPPORTED_SHAPE, std::string(what) + ": matrix too large");
 }
 
@@ -1006,7 +1011,9 @@ sy_status sy_cuda_matmul_fp8_device(int32_t device, const uint8_t* a, const uint
 }
 
 int64_t sy_cuda_orthogonalize_workspace(int32_t rows, int32_t cols, int32_t out_type) {
-    return rows < 0 || cols < 0 ? 0 : (int64_t)sy::orthogonalize_workspace_bytes(rows, cols, out_type);
+    return rows < 0 || cols < 0 || !ns_size_fits(rows, cols)
+               ? 0
+               : (int64_t)sy::orthogonalize_workspace_bytes(rows, cols, out_type);
 }
 
 sy_status sy_cuda_orthogonalize_device(int32_t device, const void* x, int32_t x_type, int64_t x_pitch, int32_t rows,

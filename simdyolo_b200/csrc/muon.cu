@@ -1457,6 +1457,7 @@ int slab_ranks(const Shape& s, bool split) {
     const int rows = (s.r + 15) / 16 * 16;
     for (int ranks = 1; ranks <= 8; ranks *= 2) {
         const int width = (s.c + 64 * ranks - 1) / (64 * ranks) * 64;
+        if ((long)rows * width * 2 > kMaxSmem) continue;   // X alone; the bytes of wider slabs may not fit an int
         if (slab_smem(rows, width, ranks, split) <= kMaxSmem - 1024) return ranks;
     }
     return 0;

@@ -177,3 +177,27 @@ def test_host_forms_refuse_bad_arguments():
         sy.muon_update(w, w.copy(), w.copy(), sy.muon_options(0.02, steps=99))
     L = sy.lib()
     assert L.sy_cuda_muon_update(0, None, None, None, 4, 4, C.byref(sy.muon_options(0.02))) == sy.SY_ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("rows, cols", [(1, 1 << 26), (1, 1 << 27), (16, 1 << 26), (128, 1 << 24), (128, (1 << 24) + 64),
+                                        (1 << 26, 5), (1, 1 << 30)])
+def test_workspaces_of_very_long_matrices_hold_their_operands(rows, cols):
+    """Two X of fp16 pairs, 128 rows at least: such a matrix is too long to stay on chip, whatever its row count."""
+    need = 2 * 128 * max(rows, cols) * 4
+    for out in (sy.SY_TYPE_F32, sy.SY_TYPE_BF16):
+        assert sy.orthogonalize_workspace(rows, cols, out) >= need
+        with pytest.raises(sy.InvalidArgument, match="workspace too small"):
+            orthogonalize(rows=rows, cols=cols, x_pitch=cols, out_pitch=cols, out_type=out, workspace_bytes=need - 1)
+    t = sy.muon_tensors([(P, P, P, rows, cols)])
+    assert sy.muon_workspace(t, sy.muon_options(0.02)) >= need
+    assert sy.muon_workspace(t, sy.muon_options(0.02, precision=sy.SY_PRECISION_TF32)) >= need // 2
+
+
+@pytest.mark.parametrize("rows, cols", [(1, (1 << 31) - 1), ((1 << 31) - 64, 1), (3, (1 << 30) + 1)])
+def test_matrices_past_32_bit_columns_are_unsupported(rows, cols):
+    with pytest.raises(sy.UnsupportedShape):
+        orthogonalize(rows=rows, cols=cols, x_pitch=cols, out_pitch=cols, workspace_bytes=1 << 62)
+    with pytest.raises(sy.UnsupportedShape):
+        muon(entry=(P, P, P, rows, cols), bytes=1 << 62)
+    assert sy.orthogonalize_workspace(rows, cols, sy.SY_TYPE_F32) == 0
+    assert sy.muon_workspace(sy.muon_tensors([(P, P, P, rows, cols)]), sy.muon_options(0.02)) == 0

@@ -268,3 +268,9 @@ def test_bf16_results_of_tiled_matrices_are_the_fp32_ones_rounded(rows, cols, st
     u = update(rows, cols, 3).cuda()
     assert torch.equal(D.orthogonalize(u, torch.bfloat16, steps, pitch=cols + 5)[:, :cols],
                        D.orthogonalize(u, torch.float32, steps).bfloat16())
+
+
+@pytest.mark.parametrize("rows, cols", [(3, 2000003), (1500001, 2)])
+def test_orthogonalize_very_long_matrices(rows, cols):
+    u = update(rows, cols, 11)
+    assert D.rel(D.orthogonalize(u.cuda(), torch.float32), D.orthogonal_reference(u)) <= SPLIT_TOL
