@@ -239,7 +239,7 @@ constexpr int kSlabThreads = 512;
 // whose additions would otherwise truncate the hi hi sums twice as often.
 __host__ __device__ constexpr int slab_gram_cols(bool split) { return split ? 256 : 128; }
 __host__ __device__ constexpr int slab_round(bool split) { return split ? 128 : 384; }
-constexpr int kMaxSmem = 227 * 1024;
+constexpr int kMaxSmem = 227 * 1024, kMaxSlabSmem = kMaxSmem - 1024;   // per CTA; dynamic, beside the static arrays
 
 struct SlabJob : Source {
     int rows;                        // r rounded up to 16
@@ -1458,7 +1458,7 @@ int slab_ranks(const Shape& s, bool split) {
     for (int ranks = 1; ranks <= 8; ranks *= 2) {
         const int width = (s.c + 64 * ranks - 1) / (64 * ranks) * 64;
         if ((long)rows * width * 2 > kMaxSmem) continue;   // X alone; the bytes of wider slabs may not fit an int
-        if (slab_smem(rows, width, ranks, split) <= kMaxSmem - 1024) return ranks;
+        if (slab_smem(rows, width, ranks, split) <= kMaxSlabSmem) return ranks;
     }
     return 0;
 }
@@ -1471,20 +1471,24 @@ void set_ranks(SlabJob& j, int ranks) {
 // Deals CTAs to the matrices of a launch.  Narrower slabs shorten every pass over X (64 x 576: 34 us on eight CTAs, 74 on
 // one), so the matrix with the most elements per CTA is given twice as many as long as all matrices fit 128 CTAs, which
 // is what clusters of eight with one CTA per SM can hold at a time (two in each of the GPU's eight groups of SMs).
-void deal_ranks(std::vector<SlabJob>& jobs) {
+// From two CTAs on a matrix needs memory for the exchange of A: 128 x 320 pairs fit on one CTA and on four, not on two.
+void deal_ranks(std::vector<SlabJob>& jobs, bool split) {
     int total = 0;
     for (const SlabJob& j : jobs) total += j.ranks;
     for (;;) {
-        SlabJob* most = nullptr;
+        SlabJob *most = nullptr, dealt{};
         for (SlabJob& j : jobs) {
             SlabJob more = j;
-            set_ranks(more, 2 * j.ranks);
-            if (j.ranks == 8 || total + j.ranks > 128 || more.width == j.width) continue;
-            if (!most || (long)j.rows * j.width > (long)most->rows * most->width) most = &j;
+            do {
+                set_ranks(more, 2 * more.ranks);
+            } while (more.ranks < 8 && slab_smem(more.rows, more.width, more.ranks, split) > kMaxSlabSmem);
+            if (more.ranks > 8 || slab_smem(more.rows, more.width, more.ranks, split) > kMaxSlabSmem) continue;
+            if (total + more.ranks - j.ranks > 128 || more.width == j.width) continue;
+            if (!most || (long)j.rows * j.width > (long)most->rows * most->width) most = &j, dealt = more;
         }
         if (!most) return;
-        total += most->ranks;
-        set_ranks(*most, 2 * most->ranks);
+        total += dealt.ranks - most->ranks;
+        *most = dealt;
     }
 }
 
@@ -1503,7 +1507,7 @@ void launch_slabs(const Settings& set, const std::vector<SlabJob>& list, cudaStr
         smem = std::max(smem, slab_smem(j.rows, j.width, j.ranks, SPLIT));
     }
     static PerDeviceOnce once;
-    once_per_device(once, [] { set_max_dynamic_smem(slab_kernel<SPLIT, N>, kMaxSmem - 1024, "slab_kernel"); });
+    once_per_device(once, [] { set_max_dynamic_smem(slab_kernel<SPLIT, N>, kMaxSlabSmem, "slab_kernel"); });
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((ctas + size - 1) / size * size);
     cfg.blockDim = dim3(kSlabThreads);
@@ -1538,7 +1542,7 @@ void run_sources(const Settings& set, const std::vector<Source>& list, bool shar
     }
     for (size_t first = 0; first < slabs.size(); first += kMaxJobs) {
         std::vector<SlabJob> part(slabs.begin() + first, slabs.begin() + std::min<size_t>(slabs.size(), first + kMaxJobs));
-        deal_ranks(part);
+        deal_ranks(part, SPLIT);
         std::stable_sort(part.begin(), part.end(), [](const SlabJob& a, const SlabJob& b) {
             return a.ranks != b.ranks ? a.ranks > b.ranks : (long)a.rows * a.width > (long)b.rows * b.width;
         });

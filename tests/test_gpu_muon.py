@@ -274,3 +274,10 @@ def test_bf16_results_of_tiled_matrices_are_the_fp32_ones_rounded(rows, cols, st
 def test_orthogonalize_very_long_matrices(rows, cols):
     u = update(rows, cols, 11)
     assert D.rel(D.orthogonalize(u.cuda(), torch.float32), D.orthogonal_reference(u)) <= SPLIT_TOL
+
+
+@pytest.mark.parametrize("shapes", [[(128, 1024)] + [(128, 320)] * 31, [(128, 1024)] * 8 + [(320, 128)] * 24,
+                                    [(128, 1024)] * 15 + [(128, 320)] * 4, [(16, 64)] * 32 + [(120, 300)] * 32])
+def test_muon_lists_whose_matrices_fit_one_or_four_ctas_but_not_two(shapes):
+    """128 x 320 takes 230,400 bytes of shared memory on one CTA and 232,448 on two, which need room for an exchange."""
+    check_muon(shapes, dict(lr=0.02), sy.muon_options(0.02), SPLIT_TOL)
