@@ -311,7 +311,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) cast_tile_kernel(
         } else {
 #pragma unroll
             for (int j = 0; j < 16; j++) {
-                float m = fmaxf(fmaxf(fabsf(v[0].get(j)), fabsf(v[1].get(j))), fmaxf(fabsf(v[2].get(j)), fabsf(v[3].get(j))));
+                float m = 0.0f;   // which NaN does not displace: a column without a finite value is one of zeros
+#pragma unroll
+                for (int i = 0; i < 4; i++) m = fmaxf(m, fabsf(v[i].get(j)));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                 if ((t & 31) < 8) cmax[warp][seg * 16 + j] = m;

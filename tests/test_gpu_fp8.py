@@ -73,6 +73,24 @@ def test_cast_of_extreme_values(fmt, both):
         assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a[~a.isnan()], b[~b.isnan()])
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_cast_of_blocks_without_a_finite_value(dtype, block_rows, fmt):
+    """Rows and columns of a block with nothing but NaN or infinities have scale 1, in both orientations."""
+    nan, inf = float("nan"), float("inf")
+    x = spread(300, 260, 8, dtype)
+    x[:128, 3], x[128:256, 4], x[:, 5] = nan, inf, -inf
+    x[256:, 6], x[:128, 140], x[:127, 141] = inf, torch.tensor([nan, inf] * 64), nan
+    x[7, :128], x[140, 128:256], x[299, 256:] = nan, -inf, inf
+    x[:128, 128:256] = nan if block_rows == 128 else x[:128, 128:256]
+    for got, want in zip(D.quantize(x.cuda(), fmt, block_rows, both=True), (x, x.T)):
+        q, e = D.cast_reference(want, fmt, block_rows)
+        assert torch.equal(got.exponents(), e)
+        a, b = got.data().float(), q.float()
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a[~a.isnan()], b[~b.isnan()])
+
+
 def test_dequantize_takes_any_scale_byte_and_leaves_the_rows_padding():
     h = D.Held(4, 130, "e4m3", 1)
     h.q[:] = torch.arange(4 * h.q.shape[1], dtype=torch.int64, device="cuda").view(4, -1).remainder(127).to(torch.uint8)
