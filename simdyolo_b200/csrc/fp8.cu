@@ -714,6 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int c = 0; c < BN; c += 32) {
             float v[32];
+            __syncwarp();   // lanes come from their own polls, then from their own rows' stores
             if (BN % 32 == 0) {
                 tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + c, v);
             } else {
@@ -776,6 +777,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         __syncthreads();
     }
+    __syncwarp();
     if (warp == 3) {
         tc_fence_after();
         tmem_dealloc(tmem, S::kTmemCols);
@@ -1021,6 +1023,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                 }
             } else {
                 if (ok) ok = mbar_wait(&tfull[acc & 1], (acc >> 1) & 1, p.status, kStatusWait);
+                __syncwarp();
                 tc_fence_after();
                 const uint32_t d = tmem + (acc & 1) * BN + quarter + c_first;
                 if (!RAGGED) {

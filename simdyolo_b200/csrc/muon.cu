@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
         mbar_init(&bar, 1);
         fence_barrier_init();
     }
+    __syncwarp();
     if (warp == 0) {
         tmem_alloc(&tmem_slot, 512);
         tmem_relinquish();
@@ -661,6 +662,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
     }
     if (bad && q.status) atomicExch(q.status, kStatusNonFinite);
     cluster_sync_all();   // no CTA leaves while a peer may read its shared memory
+    __syncwarp();
     if (warp == 0) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -1256,6 +1258,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
 #pragma unroll 1
                     for (int m = 0; m < segments; m++) {
                         if (ok) ok = mbar_wait(&tfull[accs & 1], (accs >> 1) & 1, q.status, kStatusWait);
+                        __syncwarp();
                         tc_fence_after();
                         const uint32_t d = tmem + (accs & 1) * S::kAccCols + c_first + ((uint32_t)((warp & 3) * 32) << 16);
 #pragma unroll
