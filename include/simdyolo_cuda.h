@@ -366,7 +366,8 @@ SY_API sy_status sy_cuda_sgd_update(int32_t device, float *weight, float *veloci
  * alive and unchanged until the stream has passed the call; outputs must not overlap inputs; a workspace serves
  * one call at a time (calls that may overlap on the GPU, and graphs that may replay at the same time, need one each).
  * `status` (optional, int32 the caller sets to 0) receives SY_ERR_DEVICE when a bounded wait inside a kernel gave
- * up and SY_ERR_NONFINITE where a call says so, and is otherwise left alone.
+ * up and SY_ERR_NONFINITE where a call says so (and nothing else was reported before), and is otherwise left alone;
+ * calls may share one.
  * Matrices are row-major; pitches count elements.  Sizes of 0 are allowed.  No counterpart in the reference. */
 #define SY_TYPE_F32 0
 #define SY_TYPE_BF16 1

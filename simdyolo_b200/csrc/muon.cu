@@ -224,6 +224,9 @@ __device__ __noinline__ bool finish16_far(const Settings& q, const Source& j, in
     return bad;
 }
 
+// A report that is there already, of a wait that gave up above all, is kept.
+__device__ __forceinline__ void report_not_finite(int* status) { atomicCAS(status, 0, kStatusNonFinite); }
+
 // ------------------------------------------------------------------ short matrices: one cluster each
 //
 // A matrix of at most 128 rows (of X) stays on chip for the whole call.  The CTAs of a cluster hold a slab of
@@ -660,7 +663,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1) slab_kernel(const __grid_cons
             __syncthreads();
         }
     }
-    if (bad && q.status) atomicExch(q.status, kStatusNonFinite);
+    if (bad && q.status) report_not_finite(q.status);
     cluster_sync_all();   // no CTA leaves while a peer may read its shared memory
     __syncwarp();
     if (warp == 0) {
@@ -1305,7 +1308,7 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
         if (last) break;
         ok = grid_barrier(q.barrier, ++turn, q.status, &s_ok);
     }
-    if (bad && q.status) atomicExch(q.status, kStatusNonFinite);
+    if (bad && q.status) report_not_finite(q.status);
     tc_fence_before();
     __syncthreads();
     if (warp == 3) {

@@ -281,3 +281,15 @@ def test_orthogonalize_very_long_matrices(rows, cols):
 def test_muon_lists_whose_matrices_fit_one_or_four_ctas_but_not_two(shapes):
     """128 x 320 takes 230,400 bytes of shared memory on one CTA and 232,448 on two, which need room for an exchange."""
     check_muon(shapes, dict(lr=0.02), sy.muon_options(0.02), SPLIT_TOL)
+
+
+@pytest.mark.parametrize("shape", [(64, 200), (200, 300)])
+def test_a_report_of_an_earlier_call_is_kept(shape):
+    """Calls that share a status word: a value that is not finite does not hide an earlier SY_ERR_DEVICE."""
+    w, m, d = ([x.cuda() for x in v] for v in lists([shape], 3))
+    d[0][1, 1] = float("nan")
+    for before, after in ((0, sy.SY_ERR_NONFINITE), (sy.SY_ERR_DEVICE, sy.SY_ERR_DEVICE)):
+        status = torch.full((1,), before, dtype=torch.int32, device="cuda")
+        keep = D.muon(w, m, d, sy.muon_options(0.02), status)
+        assert status.item() == after
+        del keep
