@@ -425,8 +425,8 @@ __global__ void __launch_bounds__(256)
 
 constexpr int kTileRows = 128, kBlockK = 128;
 constexpr int kScaleSlots = 4;   // groups of four K blocks whose scale words are in flight
-// Warps: 0, 8 and 9 TMA, 1 MMA, 2 scales, 3 MMA-side waits, 4-7 epilogue.
-constexpr int kThreads = 320, kProducers = 3;
+// Warps: 0, 8 and 9 TMA, 1 MMA, 2 scales, 3 MMA-side waits, 4-7 (and 10-13 where the tile has 128 columns) epilogue.
+constexpr int kProducers = 3;
 constexpr int kStageBar = 1;     // named barrier: a stage is loaded (the waiting warp and the MMA warp)
 
 struct ProductParams {
@@ -439,8 +439,15 @@ struct ProductParams {
     void* out;
     long pitch;
     int out_type, accumulate, swap, vec;   // swap: M side indexes the output's columns
+    int segment;                 // blocks of K per accumulator
     int* status;
 };
+
+// The tensor core's FP32 accumulator cuts off what an addition (an MMA, 32 products) has below its last place: sums of one
+// sign come out low by half a place per addition, 3e-5 to 1.2e-4 after 4,096 of them.  So accumulators end after this many
+// blocks of K and are added in registers, rounded to nearest: 64 additions for FP32 results (2e-6 at most), 128 for 16-bit
+// ones (4e-6; half a step of f16 is 2.4e-4).
+constexpr int kSegment = 16, kSegment16 = 32;
 
 template <int BN>
 struct ProductShape {
@@ -449,9 +456,12 @@ struct ProductShape {
     static constexpr int kStages = BN >= 128 ? 6 : 8;
     static constexpr int kScaleBytes = 512 * (1 + kScaleRows);
     static constexpr int kScaleCols = 4 * (1 + kScaleRows);
-    static constexpr int kCols = BN + kScaleSlots * kScaleCols;
+    // epilogue threads hold their sums in registers: 64 columns each at most (128 spill 680 bytes)
+    static constexpr int kGroups = BN > 64 ? 2 : 1, kPart = BN / kGroups;
+    static constexpr int kThreads = 320 + 128 * (kGroups - 1);
+    static constexpr int kCols = 2 * BN + kScaleSlots * kScaleCols;
     static constexpr int kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
-    static constexpr int kBarriers = 2 * kStages + 2 * kScaleSlots + 1;
+    static constexpr int kBarriers = 2 * kStages + 2 * kScaleSlots + 4;
     static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleSlots * kScaleBytes + kBarriers * 8 + 16;
     // the split sum's partial tile lies over the stages; its row pitch spreads eight rows over all banks
     static constexpr int kPartPitch = BN + 4;
@@ -590,9 +600,9 @@ __device__ __forceinline__ uint4 scale_words(const ProductParams& p, int side, i
 // waits ~1,200 cycles for any shared-memory access, an mbarrier wait included, so another warp does its waiting.  A warp gathers the rows' scale words (four K blocks each) into
 // 512-byte atoms, which the MMA thread copies to TMEM ahead of the MMAs that use them.  K splits form a cluster:
 // each CTA leaves its partial tile in its shared memory and sums a share of the tile over the cluster in rank
-// order, so the result does not depend on timing and no workspace is needed.
+// order, so the result does not depend on timing and no workspace is needed.  Accumulators alternate by segment.
 template <int BN>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(ProductShape<BN>::kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                    const ProductParams p) {
     using S = ProductShape<BN>;
@@ -601,8 +611,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* ssm = smem + S::kStages * S::kStageBytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(ssm + kScaleSlots * S::kScaleBytes);
     uint64_t *full = bars, *empty = bars + S::kStages, *sfull = bars + 2 * S::kStages, *sempty = sfull + kScaleSlots;
-    uint64_t* done = sempty + kScaleSlots;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    uint64_t *tfull = sempty + kScaleSlots, *tempty = tfull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // tile order: bands of 12 row tiles, so that the CTAs of a wave share rows of both operands in L2
@@ -621,7 +631,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sfull[s], 32);
             mbar_init(&sempty[s], 1);
         }
-        mbar_init(done, 1);
+        for (int s = 0; s < 2; s++) {
+            mbar_init(&tfull[s], 1);
+            mbar_init(&tempty[s], 128 * S::kGroups);
+        }
         fence_barrier_init();
     }
     if (warp == 3) {
@@ -633,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 || warp >= 8) {
+    if (warp == 0 || warp == 8 || warp == 9) {
         // The producers take turns.  A wait after a bulk copy holds a thread for ~1,000 cycles, whatever it waits for, more
         // than a stage's copies or MMAs take.  The first stages are free and need no wait.
         if (lane == 0) {
@@ -657,6 +670,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool live = true;
         for (int i = 0, group = 0; i < k1 - k0; i++) {
             const int s = i % S::kStages, kb = k0 + i;
+            if (i % p.segment == 0) {
+                const int acc = i / p.segment;
+                if (live) live = mbar_wait(&tempty[acc & 1], ((acc >> 1) & 1) ^ 1, p.status, kStatusWait);
+            }
             if (live && (i == 0 || (kb & 3) == 0))
                 live = mbar_wait(&sfull[group % kScaleSlots], (group / kScaleSlots) & 1, p.status, kStatusWait);
             if (live) live = mbar_wait(&full[s], (i / S::kStages) & 1, p.status, kStatusWait);
@@ -665,10 +682,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1) {
         const uint32_t st0 = smem_u32(smem), sc0 = smem_u32(ssm);
-        int group = 0;
+        int group = 0, acc = 0, in_segment = 0;
         for (int i = 0; i < k1 - k0; i++) {
             const int s = i % S::kStages, kb = k0 + i, slot = group % kScaleSlots;
-            const uint32_t tsc = tmem + BN + slot * S::kScaleCols;
+            const uint32_t tsc = tmem + 2 * BN + slot * S::kScaleCols, d = tmem + (acc & 1) * BN;
             named_bar_sync(kStageBar, 64);   // stage (and its scales) loaded
             tc_fence_after();
             if (i == 0 || (kb & 3) == 0)
@@ -681,14 +698,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t idesc = p.idesc | (uint32_t)(kb & 3) << 4 | (uint32_t)(kb & 3) << 29;
 #pragma unroll
             for (int k = 0; k < kBlockK / 32; k++)
-                mma_mxf8_elect(tmem, da + 2 * k, db + 2 * k, idesc, tsc, tsc + 4, (i | k) != 0);
+                mma_mxf8_elect(d, da + 2 * k, db + 2 * k, idesc, tsc, tsc + 4, (in_segment | k) != 0);
             mma_commit_elect(&empty[s]);
             if ((kb & 3) == 3) {
                 mma_commit_elect(&sempty[slot]);
                 group++;
             }
+            if (++in_segment == p.segment || i + 1 == k1 - k0) {
+                mma_commit_elect(&tfull[acc & 1]);
+                acc++;
+                in_segment = 0;
+            }
         }
-        mma_commit_elect(done);
     } else if (warp == 2) {
         const int g0 = k0 >> 2, g1 = (k1 + 3) >> 2;
         for (int g = g0; g < g1; g++) {
@@ -706,21 +727,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncwarp();
-    if (warp >= 4 && warp < 8) {
-        const int q = warp & 3, r = q * 32 + lane, i = m0 + r;
-        mbar_wait(done, 0, p.status, kStatusWait);
-        tc_fence_after();
-        float* part = reinterpret_cast<float*>(smem);
+    if ((warp >= 4 && warp < 8) || warp >= 10) {
+        constexpr int kPart = S::kPart;
+        const int q = warp & 3, r = q * 32 + lane, i = m0 + r, group = warp >= 10, c_first = group * kPart;
+        float sum[kPart];
+        const int segments = (k1 - k0 + p.segment - 1) / p.segment;
+        bool ok = true;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
-            float v[32];
-            __syncwarp();   // lanes come from their own polls, then from their own rows' stores
-            if (BN % 32 == 0) {
-                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + c, v);
-            } else {
-                tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+        for (int g = 0; g < segments; g++) {
+            if (ok) ok = mbar_wait(&tfull[g & 1], (g >> 1) & 1, p.status, kStatusWait);
+            __syncwarp();   // lanes come from their own polls
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < kPart; c += 16) {
+                float w[16];
+                tmem_ld16(tmem + (g & 1) * BN + ((uint32_t)(q * 32) << 16) + c_first + c, w);
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    sum[c + k] = g ? sum[c + k] + w[k] : w[k];
+                    asm volatile("" : "+f"(sum[c + k]));   // before the next load: registers are short
+                }
             }
-            constexpr int kPer = BN % 32 == 0 ? 32 : 16;
+            tc_fence_before();
+            mbar_arrive(&tempty[g & 1]);
+        }
+        float* part = reinterpret_cast<float*>(smem);
+        constexpr int kPer = BN % 32 == 0 ? 32 : 16;
+#pragma unroll 1
+        for (int c = c_first; c < c_first + kPart; c += kPer) {
+            const float* v = sum;   // columns from c on
+            __syncwarp();
             if (p.splits > 1) {
 #pragma unroll
                 for (int k = 0; k < kPer; k += 4)
@@ -733,10 +769,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int k = 0; k < kPer; k++)
                         if (i < p.rows[0] && j + k < p.rows[1]) put(p, i, j + k, v[k]);
                 } else if (kPer == 32 && p.vec && j + 32 <= p.rows[1]) {
-                    if (i < p.rows[0]) put_row<32>(p, i, j, v);
+                    if (i < p.rows[0]) put_row<kPer>(p, i, j, v);
                 } else {
                     // the stages are used up: their memory serves for the rows
-                    uint8_t* buf = smem + q * kRaggedBytes;
+                    uint8_t* buf = smem + (4 * group + q) * kRaggedBytes;
                     if (p.out_type == kTypeF32) {
                         for (int k = 0; k < kPer; k += 16) ragged_put<true>(p, buf, k >> 4, v + k);
                         ragged_flush<true>(p, buf, m0 + q * 32, j, kPer);
@@ -746,14 +782,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
+#pragma unroll
+            for (int k = 0; k < kPart - kPer; k++) sum[k] = sum[k + kPer];
         }
-        tc_fence_before();
     }
     if (p.splits > 1) {
         cluster_sync_all();
         const int share = kTileRows / p.splits, first = split * share;
         const uint32_t part = smem_u32(smem);
-        for (int u = threadIdx.x; u < share * BN / 4; u += kThreads) {
+        for (int u = threadIdx.x; u < share * BN / 4; u += S::kThreads) {
             // lanes along the output's rows
             const int r = first + (p.swap ? u % share : u / (BN / 4)), c = (p.swap ? u / share : u % (BN / 4)) * 4;
             if (m0 + r >= p.rows[0] || n0 + c >= p.rows[1]) continue;
@@ -792,7 +829,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Warps: 0 TMA, 1 MMA, 2 scales, 3 waits, from 4 on epilogue, the last a second TMA warp for 16-bit outputs.
 __host__ __device__ constexpr int epilogue_groups(bool f32) { return f32 ? 3 : 2; }
 constexpr int wide_threads(bool f32) { return f32 ? 512 : 416; }
-constexpr int kSegment = 16;
 
 template <int BN, bool RAGGED>
 struct WideShape {
@@ -1132,7 +1168,7 @@ void launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const ProductP
     once_per_device(once, [] { set_max_dynamic_smem(product_kernel<BN>, S::kSmem, "product_kernel"); });
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(p.tiles_m * p.tiles_n, p.splits);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -1265,6 +1301,7 @@ void fp8_matmul(const Fp8Operand& a, const Fp8Operand& b, int k, void* out, int 
     p.tiles_n = (right.rows + plan.bn - 1) / plan.bn;
     p.idesc = idesc_mxf8(plan.bn, left.e5m2, right.e5m2);
     p.vec = vec && !plan.swap;
+    p.segment = out_type == kTypeF32 ? kSegment : kSegment16;
     const CUtensorMap ta = operand_map(left.q, left.rows, k, kTileRows);
     const CUtensorMap tb = operand_map(right.q, right.rows, k, plan.bn);
     switch (plan.wide ? 1000 + plan.bn : plan.bn) {

@@ -302,3 +302,50 @@ def test_a_linear_layers_gradients_against_formula_and_differences():
         step[i, j] = 1.0
         diff = (loss(vx + step) - loss(vx - step)) / 2
         assert abs(dx[i, j].item() - diff) <= bound[i, j] + 1e-9 * loss(vx.abs()).abs()
+
+
+# Long sums of one sign.  Accumulators truncate: an addition (32 products) loses at most 2 * 2^-23 of its partial sum.  They
+# end after 16 blocks of K for FP32 results and 32 for 16-bit ones, 64 and 128 additions, whatever K is: at most 2^-16 and
+# 2^-15 of the sum; adding up to K / (128 * 16) of them and eight splits rounds by 2^-24 each; then the output's rounding,
+# half a step at the result's own size.
+def long_sum_bound(k, dtype, want):
+    full = dtype == torch.float32
+    loss = (2.0 ** -16 if full else 2.0 ** -15) + (k / 2048 + 8) * 2.0 ** -24
+    bits = {torch.float32: 24, torch.float16: 11, torch.bfloat16: 8}[dtype]
+    half_step = 2.0 ** (torch.floor(torch.log2(want)) - bits)
+    if dtype == torch.float16:
+        # f16's exponents end at -14: below 2^-14 (the smallest sums here are 9e-8) its values are multiples of 2^-24
+        half_step = half_step.clamp(min=2.0 ** -25)
+    return want * loss + half_step
+
+
+def one_sign(rows, cols, seed, scale):
+    return spread(rows, cols, seed).abs() * scale
+
+
+def check_long(m, n, k, dtype, rows, accumulate=False):
+    a = D.quantize(one_sign(m, k, 1, 2.0 ** -9).cuda(), "e4m3", 1)
+    b = D.quantize(one_sign(n, k, 2, 2.0 ** -9).cuda(), "e4m3", 1)
+    start = torch.rand(m, n, generator=torch.Generator().manual_seed(4)) if accumulate else None
+    out = start.cuda() if accumulate else None
+    got = D.matmul(a, b, dtype, out=out, accumulate=accumulate)[:rows].cpu().double()
+    a.q, a.scale, a.rows = a.q[:rows], a.scale[:rows], rows
+    want = a.values() @ b.values().T
+    bound = long_sum_bound(k, dtype, want)
+    if accumulate:
+        want = want + start[:rows].double()
+        bound = bound + 2.0 ** -24 * want
+    assert want.max() < 60000
+    assert ((got - want).abs() <= bound).all(), ((got - want) / want).mean()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m, n, k", [(4, 8, 1 << 21), (3, 40, 400000), (64, 576, 40960), (300, 300, 20001), (130, 1000, 20000),
+                                     (1200, 1300, 9000)])
+def test_long_sums_of_few_tiles_do_not_drift(m, n, k, dtype):
+    check_long(m, n, k, dtype, min(m, 64))
+
+
+@pytest.mark.parametrize("m, n, k", [(3, 40, 400000), (300, 301, 20001), (1200, 1300, 9000)])
+def test_long_sums_of_few_tiles_added_to_the_output(m, n, k):
+    check_long(m, n, k, torch.float32, min(m, 64), accumulate=True)
