@@ -444,10 +444,11 @@ struct ProductParams {
 };
 
 // The tensor core's FP32 accumulator cuts off what an addition (an MMA, 32 products) has below its last place: sums of one
-// sign come out low by half a place per addition, 3e-5 to 1.2e-4 after 4,096 of them.  So accumulators end after this many
-// blocks of K and are added in registers, rounded to nearest: 64 additions for FP32 results (2e-6 at most), 128 for 16-bit
-// ones (4e-6; half a step of f16 is 2.4e-4).
-constexpr int kSegment = 16, kSegment16 = 32;
+// sign come out low by half a place per addition, 3e-5 to 1.2e-4 after 4,096 of them.  So accumulators end after kSegment
+// blocks of K (64 additions, 2e-6) and are added in registers, rounded to nearest.  16-bit results take up to kWhole
+// blocks in one (128 additions, 4e-6; half a step of f16 is 2.4e-4 at least), which spares the registers: 4096^3 into
+// bf16 59 us, into FP32 in segments 68; with a longer K segments cost them little (8192^3 423 and 429 us).
+constexpr int kSegment = 16, kWhole = 32;
 
 template <int BN>
 struct ProductShape {
@@ -822,13 +823,14 @@ __global__ void __launch_bounds__(ProductShape<BN>::kThreads, 1)
 }
 
 // The same product for many tiles: persistent CTAs, two accumulators in TMEM, so that the epilogue warps drain one
-// while the other fills (two of 256 columns and the scales exceed TMEM's 512).  The tensor core's FP32 accumulator
-// truncates, which shows in FP32 outputs over a long K; those add sums of kSegment blocks in registers, at most 80 per
-// thread of three groups of epilogue warps (two groups end at 192 columns: 8192^3 512 us, three 438; a weight
-// gradient of 4096 x 1000 over 16,384, whose 240-column tiles make one wave, 82 us and 66).
-// Warps: 0 TMA, 1 MMA, 2 scales, 3 waits, from 4 on epilogue, the last a second TMA warp for 16-bit outputs.
-__host__ __device__ constexpr int epilogue_groups(bool f32) { return f32 ? 3 : 2; }
-constexpr int wide_threads(bool f32) { return f32 ? 512 : 416; }
+// while the other fills (two of 256 columns and the scales exceed TMEM's 512).  Where an accumulator may not take the
+// whole K (kSegment, kWhole) its sums are added in registers, at most 80 per thread of three groups of epilogue warps
+// (two groups end at 192 columns: 8192^3 into FP32 512 us, three 438; a weight gradient of 4096 x 1000 over 16,384, whose
+// 240-column tiles make one wave, 82 us and 66).
+// Warps: 0 TMA, 1 MMA, 2 scales, 3 waits, from 4 on epilogue, the last a second TMA warp where nothing is segmented.
+enum WideKind { kWhole16, kSegments16, kSegmentsF32 };
+__host__ __device__ constexpr int epilogue_groups(WideKind kind) { return kind == kWhole16 ? 2 : 3; }
+constexpr int wide_threads(WideKind kind) { return kind == kWhole16 ? 416 : 512; }
 
 template <int BN, bool RAGGED>
 struct WideShape {
@@ -844,11 +846,12 @@ struct WideShape {
     static_assert(kCols <= 512 && kSmem <= 227 * 1024, "tile too wide");
 };
 
-template <int BN, bool F32, bool RAGGED>
-__global__ void __launch_bounds__(wide_threads(F32), 1)
+template <int BN, WideKind KIND, bool RAGGED>
+__global__ void __launch_bounds__(wide_threads(KIND), 1)
     product_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                         const ProductParams p) {
     using S = WideShape<BN, RAGGED>;
+    constexpr bool F32 = KIND == kSegmentsF32, SEGMENTS = KIND != kWhole16;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint8_t* ssm = smem + S::kStages * S::kStageBytes;
@@ -877,7 +880,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
         }
         for (int s = 0; s < 2; s++) {
             mbar_init(&tfull[s], 1);
-            mbar_init(&tempty[s], epilogue_groups(F32) * 128);
+            mbar_init(&tempty[s], epilogue_groups(KIND) * 128);
         }
         fence_barrier_init();
     }
@@ -890,7 +893,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 || (!F32 && warp == 12)) {
+    if (warp == 0 || (!SEGMENTS && warp == 12)) {
         if (lane == 0) {
             const int total = mine * kb;
             bool ok = true;
@@ -898,7 +901,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                 int m0, n0;
                 place(t, m0, n0);
                 for (int k = 0; k < kb; k++, n++) {
-                    if (!F32 && (n & 1) != (warp == 12)) continue;
+                    if (!SEGMENTS && (n & 1) != (warp == 12)) continue;
                     const int s = n % S::kStages;
                     if (n >= S::kStages &&
                         !(ok = mbar_wait(&empty[s], ((n / S::kStages) & 1) ^ 1, p.status, kStatusWait)))
@@ -916,7 +919,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
         bool live = true;
         for (int t = 0, n = 0, group = 0, acc = 0; t < mine; t++)
             for (int k = 0; k < kb; k++, n++) {
-                if (k == 0 || (F32 && k % kSegment == 0)) {
+                if (k == 0 || (SEGMENTS && k % kSegment == 0)) {
                     if (live) live = mbar_wait(&tempty[acc & 1], ((acc >> 1) & 1) ^ 1, p.status, kStatusWait);
                     acc++;
                 }
@@ -943,7 +946,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                 const uint64_t da = smem_desc(st0 + s * S::kStageBytes, 0, 1024, kLayoutSw128);
                 const uint64_t db = smem_desc(st0 + s * S::kStageBytes + kTileRows * kBlockK, 0, 1024, kLayoutSw128);
                 const uint32_t idesc = p.idesc | (uint32_t)(k & 3) << 4 | (uint32_t)(k & 3) << 29;
-                const int in_segment = F32 ? k % kSegment : k;
+                const int in_segment = SEGMENTS ? k % kSegment : k;
 #pragma unroll
                 for (int i = 0; i < kBlockK / 32; i++)
                     mma_mxf8_elect(d, da + 2 * i, db + 2 * i, idesc, tsc, tsc + 4, (in_segment | i) != 0);
@@ -952,7 +955,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                     mma_commit_elect(&sempty[slot]);
                     group++;
                 }
-                if (k + 1 == kb || (F32 && in_segment + 1 == kSegment)) {
+                if (k + 1 == kb || (SEGMENTS && in_segment + 1 == kSegment)) {
                     mma_commit_elect(&tfull[acc & 1]);
                     acc++;
                 }
@@ -977,7 +980,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
             }
         }
     } else {
-        constexpr int kPart = (BN / epilogue_groups(F32) + 15) / 16 * 16;   // columns of a warp, the last group's fewer
+        constexpr int kPart = (BN / epilogue_groups(KIND) + 15) / 16 * 16;   // columns of a warp, the last group's fewer
         const int r = (warp & 3) * 32 + lane, c_first = ((warp - 4) >> 2) * kPart, c_end = min(BN, c_first + kPart);
         const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
         bool ok = true;
@@ -1014,7 +1017,7 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                         if (row0 + k < p.rows[0]) *reinterpret_cast<uint4*>(o + k * p.pitch) = q[k];
                 }
             };
-            if (F32) {
+            if constexpr (SEGMENTS) {
                 float sum[kPart] = {};
                 const int segments = (kb + kSegment - 1) / kSegment;
                 for (int g = 0; g < segments; g++, acc++) {
@@ -1035,11 +1038,39 @@ __global__ void __launch_bounds__(wide_threads(F32), 1)
                     tc_fence_before();
                     mbar_arrive(&tempty[acc & 1]);
                 }
+                constexpr int kEmit = F32 ? 16 : 32;   // four pieces of 16 bytes
+                uint32_t word[F32 ? 1 : kPart / 2];
+                if constexpr (!F32) {
 #pragma unroll
-                for (int c = 0; c < kPart; c += 16) {
+                    for (int k = 0; k < kPart / 2; k++) {
+                        word[k] = pack2(p, sum[2 * k], sum[2 * k + 1]);
+                        asm volatile("" : "+r"(word[k]));   // here and now: half the registers
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < kPart; c += kEmit) {
                     const int j = n0 + c_first + c;
                     if (c_first + c >= c_end || j >= p.rows[1]) break;
-                    if (!p.swap) {
+                    if constexpr (!F32) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int k = 0; k < 16; k++) w[k] = c / 2 + k < kPart / 2 ? word[(c / 2 + k) % (kPart / 2)] : 0u;
+                        if (!p.swap) {
+                            uint4 q[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) q[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                            emit_pieces(c_first + c, q);
+                        } else if (i < p.rows[0]) {   // lanes run along the output's rows, which may start anywhere
+                            uint16_t* o = static_cast<uint16_t*>(p.out) + j * p.pitch + i;
+                            const int n = min(c_end - c_first - c, p.rows[1] - j);
+#pragma unroll
+                            for (int k = 0; k < 32; k++) {
+                                asm volatile("" : "+l"(o));   // addresses as they are needed
+                                if (k < n) *o = (uint16_t)(w[k / 2] >> 16 * (k & 1));
+                                o += p.pitch;
+                            }
+                        }
+                    } else if (!p.swap) {
                         emit_pieces(c_first + c, reinterpret_cast<uint4*>(sum + c));
                     } else if (i < p.rows[0]) {   // lanes run along the output's rows, which may start anywhere
                         float* o = static_cast<float*>(p.out) + j * p.pitch + i;
@@ -1137,8 +1168,9 @@ Plan plan_product(int m, int n, int kblocks, bool f32, bool vec, int sms) {
                                block(bn) * ((kblocks + splits - 1) / splits)),
                       Plan{swap, bn, splits, 0});
             }
-    // FP32 outputs whose rows are not whole 16-byte pieces leave with the lanes along them, as the M side.
-    for (int swap = f32 && !vec; swap <= (int)f32; swap++)
+    // Segmented outputs whose rows are not whole 16-byte pieces leave with the lanes along them, as the M side.
+    const bool segments = f32 || kblocks > kWhole;
+    for (int swap = segments && !vec; swap <= (int)segments; swap++)
         for (int bn : {128, 192, 224, 240}) {
             const long tiles = ((swap ? n : m) + 127L) / 128 * (((swap ? m : n) + bn - 1L) / bn);
             const long waves = (tiles + sms - 1) / sms;
@@ -1182,24 +1214,25 @@ void launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const ProductP
     launch_check("product_kernel");
 }
 
-template <int BN, bool F32, bool RAGGED>
+template <int BN, WideKind KIND, bool RAGGED>
 void launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const ProductParams& p, cudaStream_t stream) {
     using S = WideShape<BN, RAGGED>;
     static PerDeviceOnce once;
     once_per_device(
-        once, [] { set_max_dynamic_smem(product_wide_kernel<BN, F32, RAGGED>, S::kSmem, "product_wide_kernel"); });
+        once, [] { set_max_dynamic_smem(product_wide_kernel<BN, KIND, RAGGED>, S::kSmem, "product_wide_kernel"); });
     const int grid = std::min(p.tiles_m * p.tiles_n, device_sms());
-    product_wide_kernel<BN, F32, RAGGED><<<grid, wide_threads(F32), S::kSmem, stream>>>(ta, tb, p);
+    product_wide_kernel<BN, KIND, RAGGED><<<grid, wide_threads(KIND), S::kSmem, stream>>>(ta, tb, p);
     launch_check("product_wide_kernel");
 }
 
 template <int BN>
 void launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const ProductParams& p, cudaStream_t stream) {
-    if (p.out_type == kTypeF32) return launch_wide<BN, true, false>(ta, tb, p, stream);
+    if (p.out_type == kTypeF32) return launch_wide<BN, kSegmentsF32, false>(ta, tb, p, stream);
+    if (p.kblocks > kWhole) return launch_wide<BN, kSegments16, false>(ta, tb, p, stream);
     if (p.vec)
-        launch_wide<BN, false, false>(ta, tb, p, stream);
+        launch_wide<BN, kWhole16, false>(ta, tb, p, stream);
     else
-        launch_wide<BN, false, true>(ta, tb, p, stream);
+        launch_wide<BN, kWhole16, true>(ta, tb, p, stream);
 }
 
 template <class T>
@@ -1301,7 +1334,7 @@ void fp8_matmul(const Fp8Operand& a, const Fp8Operand& b, int k, void* out, int 
     p.tiles_n = (right.rows + plan.bn - 1) / plan.bn;
     p.idesc = idesc_mxf8(plan.bn, left.e5m2, right.e5m2);
     p.vec = vec && !plan.swap;
-    p.segment = out_type == kTypeF32 ? kSegment : kSegment16;
+    p.segment = out_type == kTypeF32 || p.kblocks > kWhole * p.splits ? kSegment : kWhole;
     const CUtensorMap ta = operand_map(left.q, left.rows, k, kTileRows);
     const CUtensorMap tb = operand_map(right.q, right.rows, k, plan.bn);
     switch (plan.wide ? 1000 + plan.bn : plan.bn) {

@@ -305,8 +305,8 @@ def test_a_linear_layers_gradients_against_formula_and_differences():
 
 
 # Long sums of one sign.  Accumulators truncate: an addition (32 products) loses at most 2 * 2^-23 of its partial sum.  They
-# end after 16 blocks of K for FP32 results and 32 for 16-bit ones, 64 and 128 additions, whatever K is: at most 2^-16 and
-# 2^-15 of the sum; adding up to K / (128 * 16) of them and eight splits rounds by 2^-24 each; then the output's rounding,
+# end after 16 blocks of K for FP32 results and at most 32 for 16-bit ones, 64 and 128 additions, whatever K is: at most
+# 2^-16 and 2^-15 of the sum; adding up to K / (128 * 16) of them and eight splits rounds by 2^-24 each; then the output's rounding,
 # half a step at the result's own size.
 def long_sum_bound(k, dtype, want):
     full = dtype == torch.float32
@@ -349,3 +349,24 @@ def test_long_sums_of_few_tiles_do_not_drift(m, n, k, dtype):
 @pytest.mark.parametrize("m, n, k", [(3, 40, 400000), (300, 301, 20001), (1200, 1300, 9000)])
 def test_long_sums_of_few_tiles_added_to_the_output(m, n, k):
     check_long(m, n, k, torch.float32, min(m, 64), accumulate=True)
+
+
+# 16-bit outputs of many tiles whose K is more than one accumulator takes: 128, 192, 224 and 240 columns per tile, along
+# the output's rows and across them.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("m, n, k", [(1025, 3888, 4825), (3720, 520, 4750), (1167, 2712, 4948), (1158, 3176, 4821),
+                                     (963, 3715, 4313), (3747, 522, 4940), (3736, 776, 4159), (776, 3755, 4628),
+                                     (3718, 904, 4514), (909, 3718, 4883), (3204, 1208, 4217)])
+def test_wide_products_of_long_sums_in_16_bits(m, n, k, dtype):
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    a, b = operands(m, n, k)
+    buf = torch.full((m + 1, n + 8), 7.0, dtype=dtype, device="cuda")
+    D.matmul(a, b, dtype, out=buf, status=status)
+    check(a, b, dtype, buf[:m, :n])
+    assert (buf[m:] == 7).all() and (buf[:, n:] == 7).all() and status.item() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m, n, k", [(2048, 2048, 65536), (2047, 2041, 65536), (2560, 2048, 8192)])
+def test_long_sums_of_many_tiles_do_not_drift(m, n, k, dtype):
+    check_long(m, n, k, dtype, 8)
