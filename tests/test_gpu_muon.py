@@ -293,3 +293,42 @@ def test_a_report_of_an_earlier_call_is_kept(shape):
         keep = D.muon(w, m, d, sy.muon_options(0.02), status)
         assert status.item() == after
         del keep
+
+
+# ------------------------------------------------------------------ 11-bit operands (SY_PRECISION_TF32)
+
+def orthogonal_in_fp16(u, steps=5):
+    """The iteration in 64 bits with X, A and B rounded to fp16 as the kernels hold them: X times a power of two that puts
+    its entries near 1 (at most 2^15), A and B times 2^14."""
+    x = u.double()
+    if x.shape[0] > x.shape[1]:
+        return orthogonal_in_fp16(u.T, steps).T
+    p = 2.0 ** min(15, int(np.floor(0.5 * np.log2(x.numel()))))
+    half = lambda v, f: (v * f).half().double() / f
+    x = half(x / x.norm(), p)
+    for i in range(steps):
+        a = half(x @ x.T, 2.0 ** 14)
+        b = half(D.NS[1] * a + D.NS[2] * (a @ a), 2.0 ** 14)
+        x = D.NS[0] * x + b @ x
+        if i + 1 < steps:
+            x = half(x, p)
+    return x
+
+
+# Kernel and restatement round at the same places, so they differ where a sum that the tensor core forms in FP32 (off by
+# d = 2^-20 of itself at most: 512 products of 11-bit values at K = 512, half a place of 2^-24 lost per 16) falls on the
+# other side of a rounding.  That happens with probability d / step (step 2^-10 of the value) and costs a step: a
+# root-mean-square error of sqrt(d * step) = 2^-15 per operand, which orthogonal_bound follows through the iterations
+# at the steepest slope.  The bound has to leave an update without its orthogonalisation (error 1) far outside.
+@pytest.mark.parametrize("kind", ["decades", "squares", "eight", "white"])
+@pytest.mark.parametrize("rows, cols", [(64, 64), (64, 576), (80, 720), (120, 50), (200, 300), (300, 140)])
+def test_muon_in_11_bits_follows_its_roundings(rows, cols, kind):
+    u = update(rows, cols, 5) if kind == "white" else spectrum(rows, cols, kind)
+    want = orthogonal_in_fp16(u)
+    w, m = torch.zeros(rows, cols, device="cuda"), torch.zeros(rows, cols, device="cuda")
+    o = sy.muon_options(1.0, momentum=0.0, rms=max(rows, cols) ** -0.5, precision=sy.SY_PRECISION_TF32)
+    keep = D.muon([w], [m], [u.cuda()], o)
+    off, bound = (-w.cpu().double() - want).norm(), D.orthogonal_bound(u, 2.0 ** -15)
+    assert bound < 0.15 * want.norm()
+    assert off <= bound, off / want.norm()
+    del keep
