@@ -125,3 +125,54 @@ def test_image_steps_stay_finite():
         assert np.isfinite([stats.box, stats.cls, stats.dfl]).all()
     assert np.isfinite(s.flat_params()).all()
     s.close()
+
+
+@pytest.mark.parametrize("model", ["yolov8n", "yolo11s"])
+@pytest.mark.parametrize("precision", [sy.SY_PRECISION_TF32, sy.SY_PRECISION_3XTF32], ids=["tf32", "3xtf32"])
+def test_matrices_step_as_the_operator_steps_them(model, precision):
+    """A session's matrices take the very step that muon_update_device gives the same weights, momenta and gradients."""
+    rng = np.random.default_rng(11)
+    s, cfg = session(model, precision=precision)
+    o = sy.muon_options(LR, cfg.momentum, DECAY, grad_scale=0.5, precision=precision)
+    for k in range(3):
+        truth = [[], []] if k == 1 else data.synthetic_batch(rng, 2, 128, cfg.num_classes, boxes=(1, 20), wh=(8.0, 64.0))[1]
+        mats = [t for t in s.params if is_muon(t, lambda t: t["shape"][1] > 1)]
+        get = lambda read: [torch.from_numpy(np.asarray(read(t)).reshape(t["shape"][0], -1)).cuda() for t in mats]
+        w, m = get(lambda t: s.get_tensor(t["index"])), get(lambda t: s.get_optimizer_state(t["index"], 0))
+        stats = s.step_features(features(cfg, 2, rng), truth)
+        grad, starts = s.last_gradients(), np.cumsum([0] + [t["numel"] for t in s.params])
+        flat = {t["index"]: grad[a:a + t["numel"]] for t, a in zip(s.params, starts)}
+        g = get(lambda t: flat[t["index"]])
+        live = [i for i, t in enumerate(mats) if sy.tensor_group(t["name"]) == 0 or stats.box_has_grad]
+        assert 0 < len(live) and (len(live) < len(mats)) == (k == 1)
+        before = [x.clone() for x in w]
+        keep = D.muon(*[[v[i] for i in live] for v in (w, m, g)], o)
+        for i, t in enumerate(mats):
+            assert torch.equal(get(lambda t: s.get_tensor(t["index"]))[i], w[i]), t["name"]
+            assert torch.equal(get(lambda t: s.get_optimizer_state(t["index"], 0))[i], m[i]), t["name"]
+            assert torch.equal(w[i], before[i]) == (i not in live)
+        del keep
+    s.close()
+
+
+def test_a_step_that_is_not_finite_changes_nothing():
+    s, cfg = session()
+    run(s, cfg, 1, 1)
+    rng = np.random.default_rng(4)
+    feats, truth = features(cfg, 2, rng), data.synthetic_batch(rng, 2, 128, cfg.num_classes, boxes=(1, 5), wh=(8.0, 64.0))[1]
+    index = next(t["index"] for t in s.tensors if t["name"] == "cv3.0.0.conv.weight")
+    good = s.get_tensor(index)
+    bad = good.copy()
+    bad.flat[7] = np.nan
+    s.set_tensor(index, bad)
+    state = lambda: [a.tobytes() for a in (s.flat_params(), s.flat_buffers(), s.flat_velocity(0), s.flat_velocity(1))]
+    before, steps = state(), s.optimizer_steps()
+    for _ in range(2):
+        with pytest.raises(sy.NonFinite):
+            s.step_features(feats, truth)
+        assert state() == before and s.optimizer_steps() == steps
+    s.set_tensor(index, good)
+    s.step_features(feats, truth)
+    assert np.isfinite(s.flat_params()).all()
+    s.close()
+
