@@ -907,6 +907,8 @@ def matmul_fp8(a, b, fmt: int = SY_FP8_E4M3, device: int = 0):
     """C = A @ B in 8-bit floating point: A cast in blocks of 1 x 128, B in blocks of 128 x 128."""
     a = np.ascontiguousarray(a, np.float32)
     b = np.ascontiguousarray(b, np.float32)
+    if a.ndim != 2 or b.ndim != 2 or a.shape[1] != b.shape[0]:
+        raise InvalidArgument(SY_ERR_INVALID_ARGUMENT, f"matmul_fp8: shapes {a.shape} and {b.shape} do not multiply")
     m, k = a.shape
     n = b.shape[1]
     c = np.zeros((m, n), np.float32)
@@ -921,7 +923,11 @@ def muon_options(lr: float, momentum: float = 0.95, weight_decay: float = 0.0, r
 
 
 def muon_update(w, m, g, options: MuonOptions, device: int = 0):
-    """The Muon step on float32 matrices w and m in place, beside sgd_update; raises NonFinite like it."""
+    """The Muon step on contiguous float32 matrices w and m in place, beside sgd_update; raises NonFinite like it."""
+    for x in (w, m, g):
+        if x.ndim != 2 or x.shape != w.shape or x.dtype != np.float32 or not x.flags.c_contiguous:
+            raise InvalidArgument(SY_ERR_INVALID_ARGUMENT,
+                                  "muon_update: w, m and g must be contiguous float32 matrices of one shape")
     rows, cols = w.shape
     _check(lib().sy_cuda_muon_update(device, _fp(w), _fp(m), _fp(g), rows, cols, C.byref(options)))
 

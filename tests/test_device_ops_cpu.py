@@ -201,3 +201,16 @@ def test_matrices_past_32_bit_columns_are_unsupported(rows, cols):
         muon(entry=(P, P, P, rows, cols), bytes=1 << 62)
     assert sy.orthogonalize_workspace(rows, cols, sy.SY_TYPE_F32) == 0
     assert sy.muon_workspace(sy.muon_tensors([(P, P, P, rows, cols)]), sy.muon_options(0.02)) == 0
+
+
+def test_host_forms_refuse_arrays_that_the_library_would_misread():
+    """Nothing reaches the library, which sees addresses and sizes only."""
+    w = np.zeros((4, 6), np.float32)
+    for a, b in ((w, w), (w, np.zeros((5, 4), np.float32)), (w[0], w), (w, w[0])):
+        with pytest.raises(sy.InvalidArgument, match="multiply"):
+            sy.matmul_fp8(a, b)
+    o = sy.muon_options(0.02)
+    for bad in (w.astype(np.float64), w[:, ::2], w.T, w[:2].copy(), w.ravel(), np.zeros((8, 6), np.float32)[::2]):
+        for args in ((bad, w, w), (w, bad, w), (w, w, bad)):
+            with pytest.raises(sy.InvalidArgument, match="contiguous"):
+                sy.muon_update(*args, o)
