@@ -1391,9 +1391,12 @@ TilePlan plan_tiles(const std::vector<Shape>& shapes, int sms) {
     for (const Shape& s : shapes) grams += s.rb * s.rb;
     for (const Shape& s : shapes) {
         // X X^T is split while its tiles leave SMs idle, in parts of four stages at least, where the shorter K saves
-        // more than writing and adding the parts takes (about 9,000 cycles).
+        // more cycles than writing and adding the parts takes.  Pairs, five steps, whole and split in us: 333 x 1000 (saves
+        // 9,216) 170 and 172, 1000 x 2049 (12,288) 295 and 303, 768 x 1500 (13,824) 239 and 240, 333 x 1500 (15,360) 186
+        // and 176, 140 x 4096 (46,080) 266 and 195; single operands, 500 x 1500 (10,000) 135 and 142, 500 x 2000 (14,000)
+        // 145 and 148, 140 x 2048 (14,000) 119 and 115, 768 x 3000 (17,500) 207 and 200.
         const int stages = (s.c + 63) / 64, most = std::max(1, std::min(sms / grams, stages / 4));
-        plan.splits.push_back((stages - (stages + most - 1) / most) * stage(128) > 9000 ? most : 1);
+        plan.splits.push_back((stages - (stages + most - 1) / most) * stage(128) > 13900 ? most : 1);
     }
     const bool any_split = *std::max_element(plan.splits.begin(), plan.splits.end()) > 1;
     for (int p = 0; p < 3; p++) {
