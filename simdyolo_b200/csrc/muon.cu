@@ -1477,13 +1477,15 @@ void set_ranks(SlabJob& j, int ranks) {
     j.width = (j.c + 64 * ranks - 1) / (64 * ranks) * 64;
 }
 
-// Deals CTAs to the matrices of a launch.  Narrower slabs shorten every pass over X (64 x 576: 34 us on eight CTAs, 74 on
-// one), so the matrix with the most elements per CTA is given twice as many as long as all matrices fit 128 CTAs, which
-// is what clusters of eight with one CTA per SM can hold at a time (two in each of the GPU's eight groups of SMs).
+// Deals CTAs to the matrices of a launch.  Narrower slabs shorten every pass over X (64 x 576 in pairs: 53 us on eight
+// CTAs, 129 on one; in single operands 43 and 88), so the matrix with the most elements per CTA is given twice as many as
+// long as all fit the GPU at a time, with one CTA per SM: 128 CTAs in clusters of up to four, 15 clusters of eight (of 148
+// SMs; a sixteenth runs after the others: 16 of 80 x 2304 in single operands 155 us, in 15 clusters 115).
 // From two CTAs on a matrix needs memory for the exchange of A: 128 x 320 pairs fit on one CTA and on four, not on two.
 void deal_ranks(std::vector<SlabJob>& jobs, bool split) {
     int total = 0;
-    for (const SlabJob& j : jobs) total += j.ranks;
+    bool eight = false;
+    for (const SlabJob& j : jobs) total += j.ranks, eight |= j.ranks == 8;
     for (;;) {
         SlabJob *most = nullptr, dealt{};
         for (SlabJob& j : jobs) {
@@ -1492,11 +1494,12 @@ void deal_ranks(std::vector<SlabJob>& jobs, bool split) {
                 set_ranks(more, 2 * more.ranks);
             } while (more.ranks < 8 && slab_smem(more.rows, more.width, more.ranks, split) > kMaxSlabSmem);
             if (more.ranks > 8 || slab_smem(more.rows, more.width, more.ranks, split) > kMaxSlabSmem) continue;
-            if (total + more.ranks - j.ranks > 128 || more.width == j.width) continue;
+            const int limit = eight || more.ranks == 8 ? 120 : 128;
+            if (total + more.ranks - j.ranks > limit || more.width == j.width) continue;
             if (!most || (long)j.rows * j.width > (long)most->rows * most->width) most = &j, dealt = more;
         }
         if (!most) return;
-        total += dealt.ranks - most->ranks;
+        total += dealt.ranks - most->ranks, eight |= dealt.ranks == 8;
         *most = dealt;
     }
 }
