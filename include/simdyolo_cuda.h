@@ -89,7 +89,8 @@ typedef struct sy_config {
     sy_block cls_blocks[3][8];  /* cv3.{0,1,2} (and one2one_cv3.{0,1,2} with end_to_end) */
     float bn_eps, bn_momentum;  /* DetectionHead.cs:71 (PT defaults 1e-3 / 0.03) */
     int32_t optimizer;          /* SY_OPT_*.  Muon: nesterov, 5 iterations, rms 0.2 (sy_muon_options), `momentum` and
-                                 * `weight_decay` of the matrices; beta1, beta2, adam_eps of the other parameters;
+                                 * `weight_decay` of the matrices (every dense conv weight, the branches' last 1x1
+                                 * included); beta1, beta2, adam_eps of the other parameters; one lr for both;
                                  * the products' precision follows `precision` */
     float lr, momentum, weight_decay;
     float beta1, beta2, adam_eps;
@@ -219,8 +220,8 @@ SY_API sy_status sy_cuda_eval_loss_features(sy_session *session, const float *co
  * matters for progressive end-to-end heads.  Evaluation always uses epoch 0 (YoloTrainer.cs:243). */
 SY_API sy_status sy_cuda_set_epoch(sy_session *session, int32_t epoch);
 /* AdamW steps (also of SY_OPT_MUON's other parameters) taken per optimizer group: [0] class branches, [1] cv2,
- * [2] one2one_cv2 (a box group steps only when an image connected it).  AdamW is not in the reference; with sy_cuda_get/set_optimizer_state these
- * counts complete the state a resumed AdamW run needs. */
+ * [2] one2one_cv2 (a box group steps only when an image connected it).  AdamW is not in the reference; with
+ * sy_cuda_get/set_optimizer_state these counts complete the state a resumed AdamW run needs. */
 SY_API sy_status sy_cuda_get_optimizer_steps(const sy_session *session, int32_t steps[3]);
 SY_API sy_status sy_cuda_set_optimizer_steps(sy_session *session, const int32_t steps[3]);
 /* Gradient of the last step (summed over the images of every rank, before the update), parameter order. */
@@ -395,8 +396,9 @@ SY_API sy_status sy_cuda_dequantize_fp8_device(int32_t device, const uint8_t *q,
                                                int32_t cols, int32_t format, int32_t block_rows, void *out,
                                                int32_t out_type, int64_t out_pitch, void *stream);
 /* out[m][n] = a[m][k] * b[n][k]^T of two 8-bit matrices, either format and either block_rows each, accumulated in
- * FP32; accumulate adds to what out holds (SY_TYPE_F32 only).  A linear layer y = x w^T with the casts of x, w, dy
- * and their transposes: y = product(x, w), dx = product(dy, wt), dw = product(dyt, xt).  k = 0 gives zeros. */
+ * FP32 (the tensor core, which truncates, sums at most 2,048 values of k, 4,096 for 16-bit outputs; those sums are added
+ * with rounding); accumulate adds to what out holds (SY_TYPE_F32 only).  A linear layer y = x w^T with the casts of x, w,
+ * dy and their transposes: y = product(x, w), dx = product(dy, wt), dw = product(dyt, xt).  k = 0 gives zeros. */
 SY_API sy_status sy_cuda_matmul_fp8_device(int32_t device, const uint8_t *a, const uint8_t *a_scale, int32_t a_format,
                                            int32_t a_block_rows, const uint8_t *b, const uint8_t *b_scale,
                                            int32_t b_format, int32_t b_block_rows, int32_t m, int32_t n, int32_t k,
@@ -430,7 +432,8 @@ typedef struct sy_muon_options {
     int32_t nesterov, steps, precision;
 } sy_muon_options;
 /* The Muon step of `count` matrices in one set of launches (tensors is host memory, read before the call
- * returns).  No tensor's weight or momentum may share memory with anything else in the list.  *status receives SY_ERR_NONFINITE when a new weight is not finite. */
+ * returns).  No tensor's weight or momentum may share memory with anything else in the list.  *status receives
+ * SY_ERR_NONFINITE when a new weight is not finite. */
 SY_API int64_t sy_cuda_muon_workspace(const sy_muon_tensor *tensors, int32_t count, const sy_muon_options *options);
 SY_API sy_status sy_cuda_muon_update_device(int32_t device, const sy_muon_tensor *tensors, int32_t count,
                                             const sy_muon_options *options, void *workspace, int64_t workspace_bytes,

@@ -130,8 +130,8 @@ struct CastParams {
 };
 
 // Sizes of 16-bit values are compared as integers, two at a time: the bits without the sign, those of infinities and NaN
-// (`special`: there are some) taken as 0.  The two-way cast is bound by its instructions: 8192 x 4096 bf16 31 us, with FP32
-// comparisons 35.
+// (`special`: there are some) taken as 0.  8192 x 4096 bf16 both ways 31 us, with FP32 comparisons 35: issue slots are 55 %
+// used, L1 64 %, DRAM 36 %; 80 registers leave 24 warps per SM to hide the loads.
 template <class T>
 __device__ __forceinline__ uint32_t sizes2(uint32_t w, bool special) {
     constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
@@ -598,10 +598,12 @@ __device__ __forceinline__ uint4 scale_words(const ProductParams& p, int side, i
 // c = a b^T on 128 x BN tiles, one CTA per tile and K split.  Both operands stream through shared memory in
 // blocks of 128 along K (one scale per row and block, 128-byte swizzled rows); one warp issues four
 // 128 x BN x 32 block-scaled MMAs per block and touches no shared memory itself: a warp that has MMAs in flight
-// waits ~1,200 cycles for any shared-memory access, an mbarrier wait included, so another warp does its waiting.  A warp gathers the rows' scale words (four K blocks each) into
-// 512-byte atoms, which the MMA thread copies to TMEM ahead of the MMAs that use them.  K splits form a cluster:
+// waits ~1,200 cycles for any shared-memory access, an mbarrier wait included, so another warp does its waiting.
+// A warp gathers the rows' scale words (four K blocks each) into 512-byte atoms, which the MMA thread copies to TMEM
+// ahead of the MMAs that use them.  Two accumulators in TMEM take turns, one per segment of K.  K splits form a cluster:
 // each CTA leaves its partial tile in its shared memory and sums a share of the tile over the cluster in rank
-// order, so the result does not depend on timing and no workspace is needed.  Accumulators alternate by segment.
+// order, so the result does not depend on timing and no workspace is needed.
+// 1 x 4096 x 4096 takes 14 us with the weights in DRAM (floor 2.6): latency of set-up, one pass and the cluster's sum.
 template <int BN>
 __global__ void __launch_bounds__(ProductShape<BN>::kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
@@ -1058,7 +1060,8 @@ __global__ void __launch_bounds__(wide_threads(KIND), 1)
                         if (!p.swap) {
                             uint4 q[4];
 #pragma unroll
-                            for (int k = 0; k < 4; k++) q[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                            for (int k = 0; k < 4; k++)
+                                q[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
                             emit_pieces(c_first + c, q);
                         } else if (i < p.rows[0]) {   // lanes run along the output's rows, which may start anywhere
                             uint16_t* o = static_cast<uint16_t*>(p.out) + j * p.pitch + i;
@@ -1317,7 +1320,8 @@ void fp8_matmul(const Fp8Operand& a, const Fp8Operand& b, int k, void* out, int 
         return;
     }
     // whole 16-byte pieces of the output's rows
-    const bool vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch * elem % 16 == 0 && (long)b.rows * elem % 16 == 0;
+    const bool vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch * elem % 16 == 0 &&
+                     (long)b.rows * elem % 16 == 0;
     const Plan plan = plan_product(a.rows, b.rows, p.kblocks, out_type == kTypeF32, vec, device_sms());
     const Fp8Operand& left = plan.swap ? b : a;
     const Fp8Operand& right = plan.swap ? a : b;

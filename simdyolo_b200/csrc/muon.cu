@@ -1227,7 +1227,8 @@ __global__ void __launch_bounds__(kTiledThreads, 1) tiled_kernel(const __grid_co
                             transpose_pieces(p);
 #pragma unroll
                             for (int k = 0; k < 4; k++)
-                                __stcg(reinterpret_cast<uint4*>(to) + ((r & ~3) + k - r) * (kTile / 4) + 4 * h + (r & 3), p[k]);
+                                __stcg(reinterpret_cast<uint4*>(to) + ((r & ~3) + k - r) * (kTile / 4) + 4 * h + (r & 3),
+                                       p[k]);
                         }
                         return;
                     }
