@@ -84,6 +84,18 @@ void* Session::dalloc(size_t bytes) {
     return p;
 }
 
+// Copies between the host and the session's memory go through its stream, which the legacy default stream does not wait
+// for: a plain cudaMemcpy may land before the memset of a fresh allocation that is still queued there, and be wiped.
+void Session::upload(void* dst, const void* host, size_t bytes) {
+    SY_CUDA(cudaMemcpyAsync(dst, host, bytes, cudaMemcpyHostToDevice, stream_));
+    SY_CUDA(cudaStreamSynchronize(stream_));
+}
+
+void Session::download(void* host, const void* src, size_t bytes) const {
+    SY_CUDA(cudaMemcpyAsync(host, src, bytes, cudaMemcpyDeviceToHost, stream_));
+    SY_CUDA(cudaStreamSynchronize(stream_));
+}
+
 View Session::alloc_view(int channels, const Grid& g) {
     const int pitch = round_up(channels, 4);
     const long rows = (long)B_ * g.rows;
@@ -702,7 +714,7 @@ void Session::build_head() {
             for (auto& hb : br.blocks)
                 if (hb.b.has_bn)
                     for (int c = 0; c < hb.b.oc; c++) init[hb.rv_off + c] = 1.0f;
-        SY_CUDA(cudaMemcpy(buffers_, init.data(), sizeof(float) * n_buffers, cudaMemcpyHostToDevice));
+        upload(buffers_, init.data(), sizeof(float) * n_buffers);
     }
     // optimizer segments: one per parameter tensor; Muon takes its matrices out of them
     std::vector<ParamSegment> segs;
@@ -720,7 +732,7 @@ void Session::build_head() {
         muon_ws_ = dalloc(muon_workspace_bytes(muon_.data(), (int)muon_.size(), cfg.precision == SY_PRECISION_3XTF32));
     nsegs_ = (int)segs.size();
     d_segs_ = static_cast<ParamSegment*>(dalloc(sizeof(ParamSegment) * segs.size()));
-    SY_CUDA(cudaMemcpy(d_segs_, segs.data(), sizeof(ParamSegment) * segs.size(), cudaMemcpyHostToDevice));
+    upload(d_segs_, segs.data(), sizeof(ParamSegment) * segs.size());
     // activations and gradients
     size_t ws = 0;
     size_t bn_part_floats = 0;
@@ -801,7 +813,7 @@ void Session::build_head() {
         n_bn_jobs_ = (int)jobs.size();
         if (n_bn_jobs_ > 0) {
             d_bn_jobs_ = static_cast<BnFoldJob*>(dalloc(sizeof(BnFoldJob) * jobs.size()));
-            SY_CUDA(cudaMemcpy(d_bn_jobs_, jobs.data(), sizeof(BnFoldJob) * jobs.size(), cudaMemcpyHostToDevice));
+            upload(d_bn_jobs_, jobs.data(), sizeof(BnFoldJob) * jobs.size());
         }
     }
     wgrad_ws_ = static_cast<float*>(dalloc(sizeof(float) * ws));
@@ -886,7 +898,7 @@ void Session::refresh_head_weights() {
         n_layout_jobs_ = (int)jobs.size();
         if (n_layout_jobs_ == 0) return;
         d_layout_jobs_ = static_cast<WeightLayoutJob*>(dalloc(sizeof(WeightLayoutJob) * jobs.size()));
-        SY_CUDA(cudaMemcpy(d_layout_jobs_, jobs.data(), sizeof(WeightLayoutJob) * jobs.size(), cudaMemcpyHostToDevice));
+        upload(d_layout_jobs_, jobs.data(), sizeof(WeightLayoutJob) * jobs.size());
     }
     for (auto& branch : branches_)
         for (auto& hb : branch.blocks)
@@ -1835,7 +1847,7 @@ int Session::get_tensor(int index, float* host, long count) const {
     const TensorEntry& t = tensors[index];
     if (count != t.numel || !host) throw SyError(SY_ERR_INVALID_ARGUMENT, "tensor size mismatch");
     const float* src = (t.kind == 0 ? params_ : buffers_) + t.offset;
-    SY_CUDA(cudaMemcpy(host, src, sizeof(float) * count, cudaMemcpyDeviceToHost));
+    download(host, src, sizeof(float) * count);
     return SY_OK;
 }
 
@@ -1846,7 +1858,7 @@ int Session::set_opt_state(int index, int moment, const float* host, long count)
     if (count != t.numel || !host) throw SyError(SY_ERR_INVALID_ARGUMENT, "tensor size mismatch");
     for (long i = 0; i < count; i++)
         if (!std::isfinite(host[i])) throw SyError(SY_ERR_INVALID_ARGUMENT, "optimizer state not finite");
-    SY_CUDA(cudaMemcpy((moment ? vel2_ : vel_) + t.offset, host, sizeof(float) * count, cudaMemcpyHostToDevice));
+    upload((moment ? vel2_ : vel_) + t.offset, host, sizeof(float) * count);
     return SY_OK;
 }
 
@@ -1855,13 +1867,13 @@ int Session::get_opt_state(int index, int moment, float* host, long count) const
         throw SyError(SY_ERR_INVALID_ARGUMENT, "optimizer state index");
     const TensorEntry& t = tensors[index];
     if (count != t.numel || !host) throw SyError(SY_ERR_INVALID_ARGUMENT, "tensor size mismatch");
-    SY_CUDA(cudaMemcpy(host, (moment ? vel2_ : vel_) + t.offset, sizeof(float) * count, cudaMemcpyDeviceToHost));
+    download(host, (moment ? vel2_ : vel_) + t.offset, sizeof(float) * count);
     return SY_OK;
 }
 
 int Session::get_last_gradients(float* host, long count) const {
     if (count != n_params || !host) throw SyError(SY_ERR_INVALID_ARGUMENT, "gradient size mismatch");
-    SY_CUDA(cudaMemcpy(host, last_grads_, sizeof(float) * count, cudaMemcpyDeviceToHost));
+    download(host, last_grads_, sizeof(float) * count);
     return SY_OK;
 }
 

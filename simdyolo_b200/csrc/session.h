@@ -205,6 +205,8 @@ private:
     View split_view(const View& v, int slot_big, View* small);
     const float* split_weights(const float* wk, long n, const float** small);
     void* dalloc(size_t bytes);
+    void upload(void* dst, const void* host, size_t bytes);
+    void download(void* host, const void* src, size_t bytes) const;
 
     int device_ = 0;
     cudaStream_t stream_ = nullptr;
